@@ -283,6 +283,83 @@ int fnx_attn_splits(int nkv);
 int fnx_attn_finish(const float* parts, int nparts, int first_part, const float* qg, float* out, int T, int nq, int h0, int nh,
                     int hd, void* st);
 
+/* ---- several sequences behind page tables: their prompts, their single tokens, their draft trees (no counterpart in the
+ * reference, whose prompt path and batches run on its own engine's buffers).  One call takes the rows of all sequences, packed
+ * one after another; how many rows each has and where it stands is read on the device, so a captured call serves later windows
+ * of other lengths (the host's `rows` is the most there can be).  Rows behind the last sequence's are not read and their
+ * outputs are left as they were.  The K/V rows are f16 and whole on this GPU (a position split over GPUs, and int8 rows, are
+ * refused).  Every pointer 16-byte aligned; hd 128 or 256; at most 16 query heads a KV head.
+ * Bits of *err that these calls set: 32: a position without a page (the pool is used up, a table is full, or its entry names
+ * no page of the pool); 64: a value in device memory that makes no sense (a parent, a kept row, a source). */
+typedef struct FnxSeqs {
+    int nseq, rows;  /* sequences; rows of the call, at most (the packed buffers' extent) */
+    const int* row0; /* device [nseq + 1]: sequence s's rows are row0[s] .. row0[s + 1] - 1, ascending (a sequence may have none) */
+    const int* pos0; /* device [nseq]: the position of its first row = the positions the cache held before */
+    const int* pt;   /* device [nseq][pt_stride]: its page table (FnxKvPages.pt is not used); null: the cache is contiguous */
+    int pt_stride, npages; /* entries a table has; pages the pool has */
+    const int* kv0;  /* pt null: device [nseq], the cache row of its position 0 (null: 0), the cache of FnxKvPages.cap rows */
+    int max_pos;     /* no sequence ends past this position after the call (0: the tables' capacity); it decides how many
+                      * blocks share a sequence's positions, not what is computed */
+} FnxSeqs;
+/* fnx_attn_prep_append for many rows: row t of sequence s, position p = pos0[s] + t - row0[s], is appended at p with the
+ * bits that call gives its K and V rows; with `depth` (device [rows]) the row is rotated as position pos0[s] + depth[t]
+ * (nodes of a draft tree: all lie at their own cache rows, siblings at the same position).  qg, k, v are read only: the normed,
+ * rotated queries go to q16 [rows][nq][hd] in f16. */
+int fnx_attn_seqs_append(const float* qg, const float* k, const float* v, const float* q_norm, const float* k_norm, uint16_t* kc, uint16_t* vc,
+                         FnxKvPages g, const FnxSeqs* sq, const int* depth, uint16_t* q16, float eps, FnxRope rope, int nq, int nkv, int hd,
+                         unsigned* err, void* st);
+/* draft trees: parent[t] (device [rows]) is the index, within its sequence's rows, of the node before row t, always a
+ * lower one; -1: none (the row follows the cache).  anc[t][anc_words] gets a bit for every row of the sequence on the path to
+ * row t, its own among them (bit i % 32 of word i / 32: row i), depth[t] (may be null) the number of rows before it on the
+ * path.  A parent out of range sets bit 64 of *err and is taken as -1; rows past 32 anc_words (at most 32 words) too */
+int fnx_tree_masks(const int* parent, const FnxSeqs* sq, unsigned* anc, int anc_words, int* depth, unsigned* err, void* st);
+/* attention of the rows over the cache, their own K/V rows appended before: out[t][h] = sum_p softmax(q_t . k_p / sqrt(hd)) v_p,
+ * f16 in and out, sums and statistics in 32 bits, the softmax weights rounded to f16 for their product with V.
+ *   fnx_attn_prompt: row t sees positions 0 .. its own (prompts, chunks of prompts after what the cache holds, single tokens);
+ *   fnx_attn_tree:   row t sees the positions before pos0[s] and, of its sequence's rows, those whose bit is set in anc[t].
+ * qg not null: the result times sigmoid(gate), gate the second half of each head of qg [rows][nq][2 hd], as fnx_attn_finish.
+ * q_stride, out_stride: halves from a row to the next (multiples of 8, at least nq hd).  A row that sees nothing gives
+ * zeros.  Table entries that name no page of the pool count as rows of zeros.  scratch: fnx_attn_seqs_scratch_bytes bytes
+ * for these sequences (rows, nseq, max_pos, pt_stride), never read before written; calls that overlap need one each.
+ * Pages hold a multiple of 8 rows. */
+size_t fnx_attn_seqs_scratch_bytes(const FnxSeqs* sq, int nq, int nkv, int hd);
+int fnx_attn_prompt(const uint16_t* q16, int q_stride, const float* qg, const uint16_t* kc, const uint16_t* vc, FnxKvPages g, const FnxSeqs* sq,
+                    uint16_t* out, int out_stride, int nq, int nkv, int hd, void* scratch, void* st);
+int fnx_attn_tree(const uint16_t* q16, int q_stride, const float* qg, const uint16_t* kc, const uint16_t* vc, FnxKvPages g, const FnxSeqs* sq,
+                  const unsigned* anc, int anc_words, uint16_t* out, int out_stride, int nq, int nkv, int hd, void* scratch, void* st);
+
+/* the pool's pages and the sequences' tables, kept on the device.  Invariants: table entries past the pages that len[s]
+ * positions need are -1; ref[p] counts the table entries that name page p (0: free).  All zero and -1 is the empty pool.
+ * `rows` positions a page (FnxKvPages.rows), one table for the K and V pools of every layer ("planes").  nseq at most 4096. */
+typedef struct FnxPagePool {
+    int npages, rows;
+    int* ref; /* [npages] */
+    int nseq;
+    int* pt; /* [nseq][pt_stride] */
+    int pt_stride;
+    int* len; /* [nseq] positions held */
+} FnxPagePool;
+/* scratch of the calls below: zeroed once; calls on one pool go in stream order */
+size_t fnx_pages_scratch_bytes(const FnxPagePool* p);
+/* every sequence s becomes the first min(len, lim[s]) positions of sequence from[s] as it was before the call (lim null: all of
+ * them): from[s] = s keeps it (or cuts it to lim[s]), another one makes s share that sequence's pages, negative empties it.  No
+ * row is copied, pages nobody names any more are free.  from[s] >= nseq sets bit 64 and counts as s */
+int fnx_pages_fork(const FnxPagePool* p, const int* from, const int* lim, void* scratch, unsigned* err, void* st);
+/* room for add[s] >= 0 more positions of every sequence: pos0[s] = len[s] as it was, row0 [nseq + 1] = the sums of add before
+ * s (what FnxSeqs wants), len[s] += add[s].  New pages are the lowest free ones, handed out sequence by sequence; where a
+ * sequence goes on inside a page that others share, it gets a copy of the page's rows so far (in every plane; the copy comes
+ * before its other new pages) - unless all its holders go on in this call and s is the first of them.  When the pool or a table
+ * has no room (or add[s] < 0: bit 64) bit 32 is set and nothing changes, row0 all zero.  planes: device array of nplanes
+ * pool pointers (kc, vc of every layer); g.page, g.q8, nkv and hd say how the rows lie. */
+int fnx_pages_reserve(const FnxPagePool* p, const int* add, int* pos0, int* row0, void* const* planes, int nplanes, FnxKvPages g, int nkv, int hd,
+                      void* scratch, unsigned* err, void* st);
+/* an accepted path's rows move together: of the rows behind pos0[s], those at keep[s][0 .. nkeep[s] - 1] (strictly ascending
+ * offsets) become rows pos0[s] + 0, 1, ...; len[s] = pos0[s] + nkeep[s], the pages behind it go back.  nkeep[s] < 0: the
+ * sequence stays as it is.  A list that is not ascending or leaves the sequence, or rows in a page that another sequence
+ * shares, sets bit 64 and leaves the sequence as it is. */
+int fnx_pages_keep(const FnxPagePool* p, const int* pos0, const int* keep, int keep_stride, const int* nkeep, void* const* planes, int nplanes,
+                   FnxKvPages g, int nkv, int hd, void* scratch, unsigned* err, void* st);
+
 /* ---- the attention layers' block selection (reference src/qsa.cuh; src/kernels.hpp:195-217 qsa_maxsel, qsa_rows, qsa_index,
  * qsa_select, qsa_select_lanes, qsa).  Keys of FNX_QSA_DIM, FNX_QSA_HEADS query heads, blocks of FNX_QSA_POOL positions,
  * the first 64 dimensions rotated; `top` (the reference's 2048 / 4 = 512) is how many blocks a row keeps.
@@ -392,6 +469,19 @@ int fnx_penalize_row(float* row, int n, const int* pen, const float* par, void* 
 /* reference src/kernels.hpp:393-394 top_tokens (src/topk.cuh:17-138) */
 int fnx_top_tokens(float* logits, int n, int T, int v0, const int* pen_tok, const int* pen_cnt, const int* pen_n, int pen_stride,
                    const float* pen_par, float* out_v, int* out_i, unsigned* err, void* st);
+
+/* log probabilities over a slice of n logits a row (rows `stride` floats apart; tokens v0 .. v0 + n - 1), no counterpart in the
+ * reference: lse[t] = log sum e^x, entropy[t] = -sum p log p, lp[t][j] = x[tok[t][j]] - lse for the ntok given tokens (a token
+ * outside the slice: -inf), and the k <= FNX_TOPK_N likeliest tokens, best first, the lower id on a tie: top_lp, top_i
+ * [T][k].  entropy, lp with tok, and top_* with k = 0 may be null.  -inf logits are tokens that cannot come; a NaN or +inf, or
+ * a row of nothing but -inf, sets bit 16 of *err (the row's results are then NaN, or lse -inf and entropy 0).  n >= k.
+ * scratch: fnx_logprobs_scratch_bytes bytes, zeroed once (left usable); calls that overlap need one each. */
+size_t fnx_logprobs_scratch_bytes(int n, int T, int k);
+int fnx_logprobs(const float* logits, size_t stride, int n, int T, int v0, const int* tok, int ntok, int k, float* lse, float* entropy, float* lp,
+                 float* top_lp, int* top_i, void* scratch, unsigned* err, void* st);
+/* the slices' results ([nslice][T]..., host) as those of the whole vocabulary (host): fnx_top_merge's counterpart */
+int fnx_logprobs_merge(const float* lse_s, const float* entropy_s, const float* lp_s, const float* top_lp_s, const int* top_i_s, int nslice, int T,
+                       int ntok, int k, float* lse, float* entropy, float* lp, float* top_lp, int* top_i);
 
 /* ---- the window: every GPU's work for one verify window of T rows over a stack of layers, in stream order.
  * The counterpart of the reference's Engine::enqueue / ffn_half / attention (src/engine.cu:900-1054), without the
@@ -558,6 +648,11 @@ typedef struct FnxSampling {
 } FnxSampling;
 /* rows[0] the last committed token, rows[1..T) the drafts, out[t] row t's argmax: 1 + the matching prefix */
 int fnx_accept_greedy(const int* rows, const int* out, int T);
+/* a draft tree's accepted path (host): node 0 is the committed token, tok[i] node i's token, parent[i] < i the node before it, out[i]
+ * the argmax after node i.  From node 0 on, the path goes to the child whose token is the argmax (the lowest such node):
+ * path[0 ..] = the nodes' indices, their number is returned (>= 1; the tokens emitted are out[path[j]]).  Negative on bad
+ * arguments */
+int fnx_accept_tree(const int* tok, const int* parent, const int* out, int n, int* path);
 /* rejection sampling against fixed (one-hot) drafts over the rows' 64 candidates; rng: a std::mt19937_64 stream made
  * by fnx_rng_new(seed); o receives the emitted tokens; returns their number */
 void* fnx_rng_new(unsigned long long seed);

@@ -2,9 +2,11 @@
 // rows' 64 candidates, and the merge of the GPUs' candidate lists.  Restated from the reference's Session, statement for
 // statement where the arithmetic demands it (src/session.cpp:39-82 make_dist / draw, 469-510 the acceptance loop;
 // src/engine_common.cu:640-653 the merge), as free functions over plain arrays: this is host policy the drop-in keeps,
-// and the reference's own object code is its checker (oracle/ref_accept.cpp).
+// and the reference's own object code is its checker (oracle/ref_accept.cpp).  Without a counterpart there: the walk down a draft
+// tree and the merge of the slices' log probabilities.
 #include <algorithm>
 #include <cmath>
+#include <limits>
 #include <random>
 #include <vector>
 
@@ -160,5 +162,72 @@ int fnx_top_merge(const float* vs, const int* is, int nslice, int T, float* out_
         for (int k = 0; k < FNX_TOPK_N; ++k) out_v[t * FNX_TOPK_N + k] = c[k].first, out_i[t * FNX_TOPK_N + k] = c[k].second;
     }
     return 0;
+}
+
+// the slices' softmax statistics joined: with w_i = e^(lse_i - lse), lse = log sum e^lse_i and, an entropy being lse - sum p x,
+// H = lse - sum w_i (lse_i - H_i).  Sums in double.
+int fnx_logprobs_merge(const float* lse_s, const float* entropy_s, const float* lp_s, const float* top_lp_s, const int* top_i_s, int nslice, int T,
+                       int ntok, int k, float* lse, float* entropy, float* lp, float* top_lp, int* top_i) {
+    constexpr int MOST = 64;
+    const float ninf = -std::numeric_limits<float>::infinity();
+    if (nslice < 1 || nslice > MOST || T < 1 || ntok < 0 || k < 0 || k > FNX_TOPK_N)
+        return fnxk::fail("logprobs_merge: %d slices (1..%d), %d rows, %d tokens, %d alternatives", nslice, MOST, T, ntok, k);
+    if (!lse_s || !lse || (entropy && !entropy_s) || (ntok && (!lp_s || !lp)) || (k && (!top_lp_s || !top_i_s || !top_lp || !top_i)))
+        return fnxk::fail("logprobs_merge: a null buffer");
+    auto raw = [ninf](float l, float z) { return l == ninf ? ninf : l + z; };   // the logit that a log probability was made of
+    for (int t = 0; t < T; ++t) {
+        double m = ninf, z = 0.0, mean = 0.0;
+        bool nan = false;
+        for (int i = 0; i < nslice; ++i) {
+            const double x = lse_s[(size_t) i * T + t];
+            nan = nan || x != x;
+            if (x > m) m = x;
+        }
+        const bool none = !(m > ninf);
+        if (!none && !nan)
+            for (int i = 0; i < nslice; ++i) {
+                const double x = lse_s[(size_t) i * T + t], w = std::exp(x - m);
+                z += w;
+                if (w > 0.0 && entropy) mean += w * (x - (double) entropy_s[(size_t) i * T + t]);
+            }
+        const double all = nan ? std::numeric_limits<double>::quiet_NaN() : none ? (double) ninf : m + std::log(z);
+        lse[t] = (float) all;
+        if (entropy) entropy[t] = nan ? lse[t] : none ? 0.f : (float) (all - mean / z);
+        for (int j = 0; j < ntok; ++j) {
+            double x = ninf;
+            for (int i = 0; i < nslice; ++i) {
+                const size_t at = (size_t) i * T + t;
+                x = std::max(x, (double) raw(lp_s[at * ntok + j], lse_s[at]));
+            }
+            lp[(size_t) t * ntok + j] = nan ? lse[t] : none || x == ninf ? ninf : (float) (x - all);
+        }
+        int head[MOST] = {};
+        for (int j = 0; j < k; ++j) {   // every slice's list is in order: the best of the heads
+            int best = -1, bi = 0;
+            float bx = 0.f;
+            for (int i = 0; i < nslice; ++i) {
+                if (head[i] >= k) continue;
+                const size_t at = (size_t) i * T + t;
+                const float x = raw(top_lp_s[at * k + head[i]], lse_s[at]);
+                const int id = top_i_s[at * k + head[i]];
+                if (best < 0 || x > bx || (x == bx && id < bi)) best = i, bx = x, bi = id;
+            }
+            ++head[best];
+            top_i[(size_t) t * k + j] = bi;
+            top_lp[(size_t) t * k + j] = nan ? lse[t] : none || bx == ninf ? ninf : (float) (bx - all);
+        }
+    }
+    return 0;
+}
+
+int fnx_accept_tree(const int* tok, const int* parent, const int* out, int n, int* path) {
+    if (!tok || !parent || !out || !path || n < 1) return -fnxk::fail("accept_tree: a null buffer or %d nodes", n);
+    for (int i = 1; i < n; ++i)
+        if (parent[i] < -1 || parent[i] >= i) return -fnxk::fail("accept_tree: node %d's parent %d", i, parent[i]);
+    int len = 0, at = 0;
+    path[len++] = 0;
+    for (int i = 1; i < n; ++i)   // a child comes after its parent, so one pass in order finds the path
+        if (parent[i] == at && tok[i] == out[at]) path[len++] = at = i;
+    return len;
 }
 }

@@ -109,10 +109,21 @@ class GdnReplay(C.Structure):
     _fields_ = [("S", C.c_void_p), ("log", C.c_void_p), ("vmap", C.c_void_p), ("nk", C.c_int), ("nv", C.c_int), ("row0", C.c_int), ("n", C.c_int)]
 
 
+class Seqs(C.Structure):
+    _fields_ = [("nseq", C.c_int), ("rows", C.c_int), ("row0", C.c_void_p), ("pos0", C.c_void_p), ("pt", C.c_void_p), ("pt_stride", C.c_int),
+                ("npages", C.c_int), ("kv0", C.c_void_p), ("max_pos", C.c_int)]
+
+
+class PagePool(C.Structure):
+    _fields_ = [("npages", C.c_int), ("rows", C.c_int), ("ref", C.c_void_p), ("nseq", C.c_int), ("pt", C.c_void_p), ("pt_stride", C.c_int),
+                ("len", C.c_void_p)]
+
+
 class CopyJob(C.Structure):
     _fields_ = [("dst", C.c_void_p), ("src", C.c_void_p), ("bytes", C.c_size_t)]
 
 
+byref = C.byref
 _p, _i, _f, _z, _u64 = C.c_void_p, C.c_int, C.c_float, C.c_size_t, C.c_ulonglong
 
 # name -> argument types; every function returns int status unless listed in _OTHER
@@ -154,6 +165,13 @@ _SIGS = {
     "fnx_attn_part_lanes": [_p, _p, _p, KvPages, LaneRows, _p, _i, _i, _i, _i, _i, _i, _p, _p],
     "fnx_attn_partial_cells": [_p, _p, _p, KvPages, LaneRows, _p, _i, _i, _i, _p, _i, _i, _i, _p, _p, _p, _i, _p],
     "fnx_attn_finish": [_p, _i, _i, _p, _p, _i, _i, _i, _i, _i, _p],
+    "fnx_attn_seqs_append": [_p, _p, _p, _p, _p, _p, _p, KvPages, C.POINTER(Seqs), _p, _p, _f, Rope, _i, _i, _i, _p, _p],
+    "fnx_tree_masks": [_p, C.POINTER(Seqs), _p, _i, _p, _p, _p],
+    "fnx_attn_prompt": [_p, _i, _p, _p, _p, KvPages, C.POINTER(Seqs), _p, _i, _i, _i, _i, _p, _p],
+    "fnx_attn_tree": [_p, _i, _p, _p, _p, KvPages, C.POINTER(Seqs), _p, _i, _p, _i, _i, _i, _i, _p, _p],
+    "fnx_pages_fork": [C.POINTER(PagePool), _p, _p, _p, _p, _p],
+    "fnx_pages_reserve": [C.POINTER(PagePool), _p, _p, _p, _p, _i, KvPages, _i, _i, _p, _p, _p],
+    "fnx_pages_keep": [C.POINTER(PagePool), _p, _p, _i, _p, _p, _i, KvPages, _i, _i, _p, _p, _p],
     "fnx_qsa_rows": [],
     "fnx_qsa_maxsel": [_i],
     "fnx_qsa_proj": [_p, _p, _p, _p, _i, _i, _p],
@@ -163,6 +181,8 @@ _SIGS = {
     "fnx_argmax": [_p, _i, _i, _i, _p, _p, _p, _p, _p],
     "fnx_penalize_row": [_p, _i, _p, _p, _p],
     "fnx_top_tokens": [_p, _i, _i, _i, _p, _p, _p, _i, _p, _p, _p, _p, _p],
+    "fnx_logprobs": [_p, _z, _i, _i, _i, _p, _i, _i, _p, _p, _p, _p, _p, _p, _p, _p],
+    "fnx_logprobs_merge": [_p, _p, _p, _p, _p, _i, _i, _i, _i, _p, _p, _p, _p, _p],
     "fnx_repack_q8_0_split": [_p, _p, _p, _z, _z, _p],
     "fnx_repack_q6k_units": [_p, _z, _z, _z, _z, _p, _p, _p, _p, _p],
     "fnx_synth_normal": [_p, _z, _f, _u64, _p],
@@ -196,6 +216,10 @@ _OTHER = {
     "fnx_window_workspace_bytes": (_z, [_p]),
     "fnx_window_plan": (_i, [_p, _p, _p, _i]),
     "fnx_window_buf": (_p, [_p, _p, _i]),
+    "fnx_attn_seqs_scratch_bytes": (_z, [C.POINTER(Seqs), _i, _i, _i]),
+    "fnx_pages_scratch_bytes": (_z, [C.POINTER(PagePool)]),
+    "fnx_logprobs_scratch_bytes": (_z, [_i, _i, _i]),
+    "fnx_accept_tree": (_i, [_p, _p, _p, _i, _p]),
     "fnx_accept_greedy": (_i, [_p, _p, _i]),
     "fnx_lookup_drafts": (_i, [_p, _i, _i, _i, _i, _p]),
     "fnx_trace_begin": (_i, []),
