@@ -349,7 +349,7 @@ int fnx_pages_fork(const FnxPagePool* p, const int* from, const int* lim, void* 
  * s (what FnxSeqs wants), len[s] += add[s].  New pages are the lowest free ones, handed out sequence by sequence; where a
  * sequence goes on inside a page that others share, it gets a copy of the page's rows so far (in every plane; the copy comes
  * before its other new pages) - unless all its holders go on in this call and s is the first of them.  When the pool or a table
- * has no room (or add[s] < 0: bit 64) bit 32 is set and nothing changes, row0 all zero.  planes: device array of nplanes
+ * has no room bit 32 is set, where an add[s] is negative bit 64; then nothing changes, and row0 is all zero.  planes: device array of nplanes
  * pool pointers (kc, vc of every layer); g.page, g.q8, nkv and hd say how the rows lie. */
 int fnx_pages_reserve(const FnxPagePool* p, const int* add, int* pos0, int* row0, void* const* planes, int nplanes, FnxKvPages g, int nkv, int hd,
                       void* scratch, unsigned* err, void* st);
@@ -474,7 +474,7 @@ int fnx_top_tokens(float* logits, int n, int T, int v0, const int* pen_tok, cons
  * reference: lse[t] = log sum e^x, entropy[t] = -sum p log p, lp[t][j] = x[tok[t][j]] - lse for the ntok given tokens (a token
  * outside the slice: -inf), and the k <= FNX_TOPK_N likeliest tokens, best first, the lower id on a tie: top_lp, top_i
  * [T][k].  entropy, lp with tok, and top_* with k = 0 may be null.  -inf logits are tokens that cannot come; a NaN or +inf, or
- * a row of nothing but -inf, sets bit 16 of *err (the row's results are then NaN, or lse -inf and entropy 0).  n >= k.
+ * a row of nothing but -inf, sets bit 16 of *err (the row's results are then NaN and top_i -1, or lse -inf and entropy 0).  n >= k.
  * scratch: fnx_logprobs_scratch_bytes bytes, zeroed once (left usable); calls that overlap need one each. */
 size_t fnx_logprobs_scratch_bytes(int n, int T, int k);
 int fnx_logprobs(const float* logits, size_t stride, int n, int T, int v0, const int* tok, int ntok, int k, float* lse, float* entropy, float* lp,

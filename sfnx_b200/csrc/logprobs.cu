@@ -1,17 +1,17 @@
 // Log probabilities of given tokens, the entropy of their distribution and the likeliest alternatives, in one pass over the
 // logits (no counterpart in the reference, which returns tokens only).
 //
-// With m the row's maximum, z = sum e^(x - m) and s = sum (x - m) e^(x - m):  lse = m + log z,  H = log z - s / z, and a
-// token's log probability is x - lse.  (m, z, s) are kept while the row streams by: a batch whose maximum exceeds m rescales
-// z' = f z, s' = f (s + (m - m') z), f = e^(m - m').  The centred s keeps H free of the cancellation that sum p x - lse has
-// for large logits.
-// The k best are kept beside it: a block holds a list of candidates and a bound, the k-th best so far; of a batch only what
-// exceeds the bound enters, and when the list is full it is sorted and cut to k, which raises the bound.  The first bound
-// costs one batch: it is cut into groups, every group's maximum is an element, so the smallest maximum of at least k groups
-// has k elements at or above it.  Entries are 64-bit composites (the value's order-preserving key, the index's complement), no two
-// equal, so ties go to the lower index whatever order the entries come in.
-// A row goes to one block when there are many, else to as many as fill the GPU (at most 32 or so: their lists meet in the
-// row's last block), each block's part a multiple of a batch.
+// With a reference r, z = sum e^(x - r) and s = sum (x - r) e^(x - r):  lse = r + log z,  H = log z - s / z, and a token's log
+// probability is x - lse.  The reference is raised - z' = f z, s' = f (s + (r - r') z), f = e^(r - r') - only when a value exceeds
+// it by more than 8, so a thread rescales once or twice a row and e^(x - r) stays below e^8.  The centred s keeps H free of the
+// cancellation that sum p x - lse has for large logits.  A NaN or +inf makes z a NaN, which is how the row is found out.
+// The k best: a bound that k values of the row's first batch reach or exceed (the k-th largest or so of the threads'
+// maxima, found by bisection), and of the rest of the row every warp lists what exceeds it, about k / 4096 of the values,
+// without a word to the other warps.  A list that is full (rising logits) is cut to its own k best, which raises that
+// warp's bound.  In the end a bound over the lists' entries leaves little more than k, and an entry's place is the number of
+// larger ones.  Entries are 64-bit composites (the value's order-preserving key, the index's complement), no two equal, so ties go
+// to the lower index whatever order they come in.
+// A row goes to one block when there are many, else to as many as the GPU holds at once; the row's last block joins the parts.
 #include <algorithm>
 
 #include "common.cuh"
@@ -19,12 +19,12 @@
 
 namespace fnxk {
 
-constexpr int LP_THREADS = 512, LP_WARPS = LP_THREADS / 32, LP_PER = 8, LP_BATCH = LP_THREADS * LP_PER, LP_CAP = 2048;
-constexpr int LP_BLOCKS = 2 * 148;   // a call's blocks when it has few rows, so the rows that go to several blocks are fewer
+constexpr int LP_THREADS = 512, LP_WARPS = LP_THREADS / 32, LP_PER = 8, LP_BATCH = LP_THREADS * LP_PER, LP_LIST = 256;
+constexpr int LP_CAP = LP_WARPS * LP_LIST;   // entries of all lists
+constexpr int LP_BLOCKS = 2 * 148;   // blocks the GPU holds at once; rows that go to several blocks are fewer
 
 struct LpPart {   // a block's part of a row
-    float m, z, s;
-    unsigned bad;
+    float r, z, s, pad;
 };
 struct LpArgs {
     const float* logits;
@@ -43,218 +43,281 @@ __device__ __forceinline__ unsigned long long lp_composite(float v, unsigned idx
     return ((unsigned long long) fkey(fadd(v, 0.f)) << 32) | (0xffffffffu - idx);
 }
 
-// (m, z, s) of two parts of a row together
-__device__ __forceinline__ void lp_join(float& m, float& z, float& s, float m2, float z2, float s2) {
-    const float mn = fmaxf(m, m2);
-    if (mn == -INFINITY) return;
-    const float d1 = fmaxf(m - mn, -200.f), d2 = fmaxf(m2 - mn, -200.f);   // e^-200 is zero: a part of nothing (-inf) drops out
+// (r, z, s) of two parts of a row together
+__device__ __forceinline__ void lp_join(float& r, float& z, float& s, float r2, float z2, float s2) {
+    const float rn = fmaxf(r, r2);
+    if (rn == -INFINITY) {   // nothing on either side, but for a NaN
+        z += z2, s += s2;
+        return;
+    }
+    const float d1 = fmaxf(r - rn, -200.f), d2 = fmaxf(r2 - rn, -200.f);   // e^-200 is zero: a part of nothing (-inf) drops out
     const float f1 = __expf(d1), f2 = __expf(d2);
     s = f1 * (s + d1 * z) + f2 * (s2 + d2 * z2);
     z = f1 * z + f2 * z2;
-    m = mn;
+    r = rn;
 }
 
-// descending bitonic sort of list[0 .. n) (n <= LP_CAP), filled up to a power of two with zeros, which are below every entry
-__device__ void lp_sort(unsigned long long* list, unsigned n, int tid) {
-    unsigned p = 1;
-    while (p < n) p <<= 1;
-    for (unsigned i = n + tid; i < p; i += LP_THREADS) list[i] = 0ull;
-    __syncthreads();
-    for (unsigned size = 2; size <= p; size <<= 1)
-        for (unsigned step = size >> 1; step; step >>= 1) {
-            for (unsigned i = tid; i < p / 2; i += LP_THREADS) {
-                const unsigned a = 2 * i - (i & (step - 1)), b = a + step;
-                const unsigned long long x = list[a], y = list[b];
-                if ((x < y) == ((a & size) == 0)) list[a] = y, list[b] = x;
-            }
-            __syncthreads();
+// Bisection by a warp: a bound b that between k and k + slack of the entries reach or exceed (a lane has N; 0: no entry), or 0
+// when there are fewer than k.  Entries are distinct, so it ends after at most 64 steps.
+template <int N> __device__ __forceinline__ unsigned long long lp_bound(const unsigned long long (&e)[N], int k, int slack) {
+    unsigned long long most = 0ull;
+    int have = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        most = e[i] > most ? e[i] : most;
+        have += e[i] != 0ull;
+    }
+    if ((int) __reduce_add_sync(0xffffffffu, (unsigned) have) < k) return 0ull;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        const unsigned long long x = __shfl_xor_sync(0xffffffffu, most, o);
+        most = x > most ? x : most;
+    }
+    unsigned long long lo = 1ull, hi = most;   // at least k reach lo; the answer is not above hi
+    // the k-th best is seldom far below the best: the first guess is half of it
+    unsigned long long mid = hi > (24ull << 55) ? hi - (1ull << 55) : lo + (hi - lo) / 2;
+    while (lo < hi) {
+        unsigned c = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) c += e[i] >= mid;
+        c = __reduce_add_sync(0xffffffffu, c);
+        if ((int) c >= k) {
+            lo = mid;
+            if ((int) c <= k + slack) break;
+        } else {
+            hi = mid - 1ull;
         }
+        mid = lo + (hi - lo + 1ull) / 2;
+    }
+    return lo;
 }
 
-__global__ void __launch_bounds__(LP_THREADS) k_logprobs(const LpArgs a) {
-    __shared__ unsigned long long list[LP_CAP];
-    __shared__ float wm[LP_WARPS], wz[LP_WARPS], ws[LP_WARPS];
-    __shared__ unsigned long long gmin[LP_WARPS];
-    __shared__ unsigned n_list, fail_at, bad_s, last_s;
-    __shared__ float lse_s;
+struct LpShared {
+    unsigned long long list[LP_WARPS][LP_LIST];
+    unsigned long long best[LP_THREADS];   // the threads' maxima; then the entries that are placed
+    float r[LP_WARPS], z[LP_WARPS], s[LP_WARPS];
+    unsigned long long bound;
+    unsigned n, last;
+    float lse;
+};
+
+// the bound that at least k of the threads' maxima reach (0: fewer than k have any)
+__device__ __forceinline__ unsigned long long lp_block_bound(LpShared& sh, unsigned long long mine, int k) {
+    sh.best[threadIdx.x] = mine;
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        unsigned long long e[LP_WARPS];
+#pragma unroll
+        for (int i = 0; i < LP_WARPS; ++i) e[i] = sh.best[i * 32 + threadIdx.x];
+        const unsigned long long b = lp_bound(e, k, 16);
+        if (threadIdx.x == 0) sh.bound = b;
+    }
+    __syncthreads();
+    return sh.bound;
+}
+
+// The k best of the threads' entries (N each, 0: none), in order, at place 0 .. k - 1 of `place`; at least k entries exist.
+template <int N, typename F> __device__ __forceinline__ void lp_best(LpShared& sh, const unsigned long long (&e)[N], int k, F place) {
+    const int tid = threadIdx.x;
+    unsigned long long most = 0ull;
+#pragma unroll
+    for (int i = 0; i < N; ++i) most = e[i] > most ? e[i] : most;
+    if (tid == 0) sh.n = 0u;
+    unsigned long long b = lp_block_bound(sh, most, k);
+    // k + 16 threads at most have entries above the bound, and fewer than k have any where there is none: (k + 16) N entries
+    unsigned long long* all = &sh.list[0][0];   // (the lists are in registers)
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+        if (e[i] && e[i] >= b) all[atomicAdd(&sh.n, 1u)] = e[i];
+    __syncthreads();
+    const unsigned n = min(sh.n, (unsigned) LP_CAP);
+    for (unsigned i = tid; i < n; i += LP_THREADS) {
+        const unsigned long long c = all[i];
+        int at = 0;
+        for (unsigned j = 0; j < n; ++j) at += all[j] > c;
+        if (at < k) place(at, c);
+    }
+}
+
+__global__ void __launch_bounds__(LP_THREADS, 2) k_logprobs(const LpArgs a) {
+    __shared__ LpShared sh;
     const int row = blockIdx.x / a.nsplit, split = blockIdx.x % a.nsplit, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const float* x = a.logits + (size_t) row * a.stride;
-    const int nbatch = (a.n + LP_BATCH - 1) / LP_BATCH, per = (nbatch + a.nsplit - 1) / a.nsplit;
-    const int lo = min((long long) split * per * LP_BATCH, (long long) a.n), hi = (int) min((long long) lo + (long long) per * LP_BATCH, (long long) a.n);
-    if (tid == 0) n_list = 0u, fail_at = 0xffffffffu, bad_s = 0u;
+    // positions are counted from the 16-byte boundary at or before the row's first logit: a thread has two runs of four a batch
+    const int shift = (int) (((uintptr_t) x >> 2) & 3u), end = a.n + shift;
+    const int nbatch = (end + LP_BATCH - 1) / LP_BATCH, per = (nbatch + a.nsplit - 1) / a.nsplit;
+    const int lo = (int) min((long long) split * per * LP_BATCH, (long long) end), hi = (int) min((long long) lo + (long long) per * LP_BATCH, (long long) end);
+    const float* base = x - shift;
+    auto load = [&](int i0, float* v) {
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+            const int p = i0 + g * (LP_BATCH / 2) + tid * 4;
+            if (p >= shift && p + 4 <= hi) {
+                const float4 f = __ldcs(reinterpret_cast<const float4*>(base + p));
+                v[4 * g] = f.x, v[4 * g + 1] = f.y, v[4 * g + 2] = f.z, v[4 * g + 3] = f.w;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[4 * g + e] = p + e >= shift && p + e < hi ? base[p + e] : -INFINITY;
+            }
+        }
+    };
+    auto index = [&](int i0, int j) { return i0 + (j >> 2) * (LP_BATCH / 2) + tid * 4 + (j & 3); };
     pdl_wait();
     pdl_go();
-    __syncthreads();
-    float m = -INFINITY, z = 0.f, s = 0.f, floor_v = -INFINITY;
-    unsigned long long floor_c = 0ull;   // the bound: an entry has to be above it
-    bool bad = false;
-    int group = 1;   // threads of a group: at least k groups in the block
-    while (LP_THREADS / (2 * group) >= a.k && group < 32) group *= 2;
+    float r = -INFINITY, z = 0.f, s = 0.f, bound_v = -INFINITY;
+    unsigned long long bound = 0ull;   // an entry has to be above it
+    int cnt = 0;                       // this warp's list
+    unsigned long long* list = sh.list[warp];
+    float next[LP_PER];
+    load(lo, next);
     for (int i0 = lo; i0 < hi; i0 += LP_BATCH) {
         float v[LP_PER];
-        float mx = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < LP_PER; ++j) {
-            const int i = i0 + j * LP_THREADS + tid;
-            v[j] = i < hi ? __ldcs(x + i) : -INFINITY;
-        }
+        for (int j = 0; j < LP_PER; ++j) v[j] = next[j];
+        if (i0 + LP_BATCH < hi) load(i0 + LP_BATCH, next);
+        float mx = v[0];
 #pragma unroll
-        for (int j = 0; j < LP_PER; ++j) {
-            bad = bad || !(v[j] < INFINITY);   // +inf or NaN
-            mx = fmaxf(mx, v[j]);
-        }
-        if (mx > m) {
-            const float d = fmaxf(m - mx, -200.f), f = __expf(d);
+        for (int j = 1; j < LP_PER; ++j) mx = fmaxf(mx, v[j]);
+        if (mx > r + 8.f || (r == -INFINITY && mx > -INFINITY)) {
+            const float d = fmaxf(r - mx, -200.f), f = __expf(d);
             s = f * (s + d * z);
             z *= f;
-            m = mx;
+            r = mx;
         }
-        if (mx != -INFINITY) {
+        const float ref = r == -INFINITY ? 0.f : r;
 #pragma unroll
-            for (int j = 0; j < LP_PER; ++j) {
-                const float d = fmaxf(v[j] - m, -200.f), e = __expf(d);
-                z += e;
-                s += e * d;
-            }
+        for (int j = 0; j < LP_PER; ++j) {
+            const float d = v[j] - ref, e = __expf(d);
+            z += e;
+            s = fmaf(e, fmaxf(d, -200.f), s);
         }
         if (!a.k) continue;
-        if (i0 == lo) {   // the first bound
-            unsigned long long best = 0ull;
+        if (i0 == lo) {
+            unsigned long long most = 0ull;
 #pragma unroll
             for (int j = 0; j < LP_PER; ++j) {
-                const int i = i0 + j * LP_THREADS + tid;
-                const unsigned long long c = i < hi ? lp_composite(v[j], (unsigned) i) : 0ull;
-                best = c > best ? c : best;
+                const int p = index(i0, j);
+                const unsigned long long c = p >= shift && p < hi && v[j] == v[j] ? lp_composite(v[j], (unsigned) (p - shift)) : 0ull;
+                most = c > most ? c : most;
             }
-            for (int o = 1; o < group; o <<= 1) {
-                const unsigned long long other = __shfl_xor_sync(0xffffffffu, best, o);
-                best = other > best ? other : best;
-            }
-#pragma unroll
-            for (int o = 16; o; o >>= 1) {
-                const unsigned long long other = __shfl_xor_sync(0xffffffffu, best, o);
-                best = other < best ? other : best;
-            }
-            if (lane == 0) gmin[warp] = best;
-            __syncthreads();
-            best = gmin[0];
-            for (int w = 1; w < LP_WARPS; ++w) best = gmin[w] < best ? gmin[w] : best;
-            floor_c = best ? best - 1ull : 0ull;   // the bound itself may enter
-            floor_v = best ? fkey_inv((unsigned) (floor_c >> 32)) : -INFINITY;
-            if (floor_v != floor_v) floor_v = -INFINITY;   // (a NaN's key)
+            bound = lp_block_bound(sh, most, a.k);
+            bound_v = bound ? fkey_inv((unsigned) (bound >> 32)) : -INFINITY;
+            bound -= bound != 0ull;   // the bound itself may enter
         }
-        bool todo = true;   // this warp's entries of the batch are still to be written
-        while (true) {
-            if (todo) {
-                unsigned mine = 0;
-                if (!(mx < floor_v) || bad) {
+        if (!__any_sync(0xffffffffu, mx >= bound_v)) continue;
 #pragma unroll
-                    for (int j = 0; j < LP_PER; ++j) {
-                        const int i = i0 + j * LP_THREADS + tid;
-                        if (i < hi && lp_composite(v[j], (unsigned) i) > floor_c) mine |= 1u << j;
-                    }
+        for (int j = 0; j < LP_PER; ++j) {
+            const int p = index(i0, j);
+            bool in = v[j] >= bound_v && p >= shift && p < hi;
+            unsigned who = __ballot_sync(0xffffffffu, in);
+            if (!who) continue;
+            if (cnt + 32 > LP_LIST) {   // full: its best k stay
+                unsigned long long e[LP_LIST / 32];
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < LP_LIST / 32; ++i) e[i] = i * 32 + lane < cnt ? list[i * 32 + lane] : 0ull;
+                const unsigned long long b = lp_bound(e, a.k, 0);
+                __syncwarp();
+                cnt = 0;
+#pragma unroll
+                for (int i = 0; i < LP_LIST / 32; ++i) {
+                    const bool keep = e[i] >= b;
+                    const unsigned kept = __ballot_sync(0xffffffffu, keep);
+                    if (keep) list[cnt + __popc(kept & ((1u << lane) - 1u))] = e[i];
+                    cnt += __popc(kept);
                 }
-                if (__any_sync(0xffffffffu, mine)) {
-                    unsigned before = (unsigned) __popc(mine), total;   // inclusive, then exclusive count over the lanes
-#pragma unroll
-                    for (int o = 1; o < 32; o <<= 1) {
-                        const unsigned y = __shfl_up_sync(0xffffffffu, before, o);
-                        if (lane >= o) before += y;
-                    }
-                    total = __shfl_sync(0xffffffffu, before, 31);
-                    before -= (unsigned) __popc(mine);
-                    unsigned base = 0;
-                    if (lane == 0) base = atomicAdd(&n_list, total);
-                    base = __shfl_sync(0xffffffffu, base, 0);
-                    if (base + total <= LP_CAP) {
-#pragma unroll
-                        for (int j = 0; j < LP_PER; ++j)
-                            if (mine >> j & 1u) list[base + before++] = lp_composite(v[j], (unsigned) (i0 + j * LP_THREADS + tid));
-                        todo = false;
-                    } else if (lane == 0) {
-                        atomicMin(&fail_at, base);   // places are handed out in order: below the first failure all is written
-                    }
-                } else {
-                    todo = false;
-                }
+                bound = b, bound_v = fkey_inv((unsigned) (b >> 32));
             }
-            if (!__syncthreads_or(todo)) break;
-            // the list is full: its best k stay, the last of them is the bound.  A list cut to k (at most 64) takes at least one
-            // warp's entries (at most 256), so the batch is through after LP_WARPS rounds
-            const unsigned have = fail_at;
-            lp_sort(list, have, tid);
-            floor_c = list[a.k - 1];
-            floor_v = fkey_inv((unsigned) (floor_c >> 32));
-            if (floor_v != floor_v) floor_v = -INFINITY;
-            __syncthreads();
-            if (tid == 0) n_list = (unsigned) a.k, fail_at = 0xffffffffu;
-            __syncthreads();
+            const unsigned long long c = lp_composite(v[j], (unsigned) (p - shift));
+            in = in && c > bound;
+            who = __ballot_sync(0xffffffffu, in);
+            if (in) list[cnt + __popc(who & ((1u << lane) - 1u))] = c;
+            cnt += __popc(who);
         }
     }
     // ---- the block's statistics
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
-        const float m2 = __shfl_xor_sync(0xffffffffu, m, o), z2 = __shfl_xor_sync(0xffffffffu, z, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
-        lp_join(m, z, s, m2, z2, s2);
+        const float r2 = __shfl_xor_sync(0xffffffffu, r, o), z2 = __shfl_xor_sync(0xffffffffu, z, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
+        lp_join(r, z, s, r2, z2, s2);
     }
-    if (lane == 0) wm[warp] = m, wz[warp] = z, ws[warp] = s;
-    if (bad) bad_s = 1u;
+    if (lane == 0) sh.r[warp] = r, sh.z[warp] = z, sh.s[warp] = s;
+    unsigned long long e[LP_LIST / 32];
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < LP_LIST / 32; ++i) e[i] = i * 32 + lane < cnt ? list[i * 32 + lane] : 0ull;
     __syncthreads();
-    m = wm[0], z = wz[0], s = ws[0];
-    for (int w = 1; w < LP_WARPS; ++w) lp_join(m, z, s, wm[w], wz[w], ws[w]);
-    bool any_bad = bad_s != 0u;
-    unsigned have = min(n_list, (unsigned) LP_CAP);
-    if (a.k) lp_sort(list, have, tid);
-    if (a.nsplit > 1) {   // the row's last block joins the parts
-        LpPart* parts = a.part + (size_t) row * a.nsplit;
-        unsigned long long* cands = a.cand + (size_t) row * a.nsplit * a.k;
-        for (int i = tid; i < a.k; i += LP_THREADS) cands[(size_t) split * a.k + i] = (unsigned) i < have ? list[i] : 0ull;
-        if (tid == 0) parts[split] = LpPart{m, z, s, any_bad ? 1u : 0u};
-        __threadfence();
-        __syncthreads();
-        if (tid == 0) last_s = atomicAdd(&a.count[row], 1u) == (unsigned) a.nsplit - 1u;
-        __syncthreads();
-        if (!last_s) return;
-        __threadfence();
-        m = -INFINITY, z = 0.f, s = 0.f, any_bad = false;
-        for (int i = 0; i < a.nsplit; ++i) {
-            const LpPart p = parts[i];
-            lp_join(m, z, s, p.m, p.z, p.s);
-            any_bad = any_bad || p.bad;
+    const bool many = a.nsplit > 1;
+    LpPart* parts = a.part + (size_t) row * a.nsplit;
+    unsigned long long* cands = a.cand + (size_t) row * a.nsplit * a.k;
+    if (warp == 0) {
+        r = lane < LP_WARPS ? sh.r[lane] : -INFINITY, z = lane < LP_WARPS ? sh.z[lane] : 0.f, s = lane < LP_WARPS ? sh.s[lane] : 0.f;
+#pragma unroll
+        for (int o = LP_WARPS / 2; o; o >>= 1) {
+            const float r2 = __shfl_xor_sync(0xffffffffu, r, o), z2 = __shfl_xor_sync(0xffffffffu, z, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
+            lp_join(r, z, s, r2, z2, s2);
         }
-        have = (unsigned) (a.nsplit * a.k);
-        for (unsigned i = tid; i < have; i += LP_THREADS) list[i] = cands[i];
+        if (many && lane == 0) parts[split] = LpPart{r, z, s, 0.f};
+    }
+    if (many) {   // the row's last block joins the parts
+        if (a.k) {
+            for (int i = tid; i < a.k; i += LP_THREADS) cands[(size_t) split * a.k + i] = 0ull;
+            __syncthreads();
+            lp_best(sh, e, a.k, [&](int at, unsigned long long c) { cands[(size_t) split * a.k + at] = c; });
+        }
+        __threadfence();
         __syncthreads();
-        if (a.k) lp_sort(list, have, tid);
+        if (tid == 0) sh.last = atomicAdd(&a.count[row], 1u) == (unsigned) a.nsplit - 1u;
+        __syncthreads();
+        if (!sh.last) return;
+        __threadfence();
+        if (warp == 0) {
+            r = -INFINITY, z = 0.f, s = 0.f;
+            for (int i = lane; i < a.nsplit; i += 32) {
+                const LpPart p = parts[i];
+                lp_join(r, z, s, p.r, p.z, p.s);
+            }
+#pragma unroll
+            for (int o = 16; o; o >>= 1) {
+                const float r2 = __shfl_xor_sync(0xffffffffu, r, o), z2 = __shfl_xor_sync(0xffffffffu, z, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
+                lp_join(r, z, s, r2, z2, s2);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < LP_LIST / 32; ++i) e[i] = i * LP_THREADS + tid < a.nsplit * a.k ? cands[i * LP_THREADS + tid] : 0ull;
         if (tid == 0) a.count[row] = 0u;
     }
-    const bool none = m == -INFINITY && !any_bad;
     if (tid == 0) {
-        if (any_bad || none) atomicOr(a.err, 16u);
+        const bool bad = z != z, none = r == -INFINITY && !bad;
+        if (bad || none) atomicOr(a.err, 16u);
         const float lz = logf(z);
-        lse_s = any_bad ? NAN : none ? -INFINITY : m + lz;
-        a.lse[row] = lse_s;
-        if (a.ent) a.ent[row] = any_bad ? NAN : none ? 0.f : fmaxf(lz - s / z, 0.f);
+        sh.lse = bad ? NAN : none ? -INFINITY : r + lz;
+        a.lse[row] = sh.lse;
+        if (a.ent) a.ent[row] = bad ? NAN : none ? 0.f : fmaxf(lz - s / z, 0.f);
     }
     __syncthreads();
-    const float lse = lse_s;
+    const float lse = sh.lse;
+    const bool bad = lse != lse, none = lse == -INFINITY;
     for (int j = tid; j < a.ntok; j += LP_THREADS) {
         const long long t = (long long) a.tok[(size_t) row * a.ntok + j] - a.v0;
         const bool in = t >= 0 && t < a.n;
-        a.lp[(size_t) row * a.ntok + j] = !in ? -INFINITY : any_bad ? NAN : none ? -INFINITY : x[t] - lse;
+        a.lp[(size_t) row * a.ntok + j] = !in ? -INFINITY : bad ? NAN : none ? -INFINITY : x[t] - lse;
     }
-    for (int j = tid; j < a.k; j += LP_THREADS) {
-        const unsigned long long c = list[j];
-        a.top_i[(size_t) row * a.k + j] = a.v0 + (int) (0xffffffffu - (unsigned) (c & 0xffffffffu));
-        a.top_lp[(size_t) row * a.k + j] = any_bad ? NAN : none ? -INFINITY : fkey_inv((unsigned) (c >> 32)) - lse;
+    if (!a.k) return;
+    if (bad) {   // no order to speak of
+        for (int j = tid; j < a.k; j += LP_THREADS) a.top_i[(size_t) row * a.k + j] = -1, a.top_lp[(size_t) row * a.k + j] = NAN;
+        return;
     }
+    lp_best(sh, e, a.k, [&](int at, unsigned long long c) {
+        a.top_i[(size_t) row * a.k + at] = a.v0 + (int) (0xffffffffu - (unsigned) (c & 0xffffffffu));
+        a.top_lp[(size_t) row * a.k + at] = none ? -INFINITY : fkey_inv((unsigned) (c >> 32)) - lse;
+    });
 }
 
-// blocks a row: enough that the GPU has about two a multiprocessor, each with a batch at least; the lists of a row's blocks
-// together fit the last block's
+// blocks a row: as many as the GPU holds at once, each with a batch of the row at least; their k best have room in one block
 static int lp_splits(int n, int T, int k) {
-    const int batches = (n + LP_BATCH - 1) / LP_BATCH, want = (LP_BLOCKS + T - 1) / T;
-    int s = std::max(1, std::min(want, std::min(batches, LP_CAP / std::max(k, LP_CAP / 64))));
+    const int batches = (n + 3 + LP_BATCH - 1) / LP_BATCH, want = std::max(1, LP_BLOCKS / T);   // n + 3: a row may begin inside a 16-byte run
+    const int s = std::max(1, std::min(want, std::min(batches, std::min(64, LP_CAP / std::max(k, 1)))));
     const int per = (batches + s - 1) / s;
     return (batches + per - 1) / per;   // no empty block
 }

@@ -150,6 +150,30 @@ def test_logprobs_rows_without_a_distribution():
     _check({k: v[good] if k != "err" else v for k, v in r.items()}, x[good], tok[good], 4)
 
 
+@pytest.mark.parametrize("T,n", [(1, 40000), (400, 9000)])
+def test_logprobs_a_nan_among_masked_values(T, n):
+    x = torch.full((T, n), -float("inf"), device=DEV)
+    x[0, n - 7] = float("nan")
+    r = _run(x, torch.zeros(T, 1, dtype=torch.int32, device=DEV), 3)
+    assert int(r["err"]) == 16 and torch.isnan(r["lse"][0]) and r["ti"][0].tolist() == [-1] * 3
+    assert (r["lse"][1:] == -float("inf")).all()
+
+
+@pytest.mark.parametrize("shift", [1, 2, 3])
+@pytest.mark.parametrize("T,n", [(3, 20001), (400, 4095), (1, 5)])
+def test_logprobs_rows_that_begin_anywhere(T, n, shift):
+    whole = torch.full((T * (n + 6) + 8,), 1e4, device=DEV)
+    x = whole[shift:shift + T * (n + 6)].view(T, n + 6)
+    x[:, :n] = torch.randn(T, n, device=DEV)
+    k = min(n, 20)
+    r = {"lse": torch.zeros(T, device=DEV), "ent": torch.zeros(T, device=DEV), "tv": torch.zeros(T, k, device=DEV), "ti": torch.zeros(T, k, dtype=torch.int32, device=DEV)}
+    err, scratch = torch.zeros(1, dtype=torch.int32, device=DEV), torch.zeros(L.load().fnx_logprobs_scratch_bytes(n, T, k), dtype=torch.uint8, device=DEV)
+    L.call("fnx_logprobs", x.data_ptr(), n + 6, n, T, 0, None, 0, k, r["lse"].data_ptr(), r["ent"].data_ptr(), None, r["tv"].data_ptr(), r["ti"].data_ptr(),
+           scratch.data_ptr(), err.data_ptr(), L.stream())
+    assert int(err) == 0
+    _check(r, x[:, :n].contiguous(), None, k)
+
+
 def test_logprobs_one_scratch_for_calls_of_all_sizes_and_a_graph():
     scratch = torch.zeros(max(L.load().fnx_logprobs_scratch_bytes(n, T, 64) for T, n in ((16, 151936), (290, 40000), (1, 9000))), dtype=torch.uint8, device=DEV)
     for T, n, k in ((16, 151936, 64), (290, 40000, 3), (1, 9000, 20), (16, 151936, 0), (200, 40000, 64)):
