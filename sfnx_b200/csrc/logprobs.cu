@@ -109,7 +109,7 @@ __device__ __forceinline__ unsigned long long lp_block_bound(LpShared& sh, unsig
         unsigned long long e[LP_WARPS];
 #pragma unroll
         for (int i = 0; i < LP_WARPS; ++i) e[i] = sh.best[i * 32 + threadIdx.x];
-        const unsigned long long b = lp_bound(e, k, 16);
+        const unsigned long long b = lp_bound(e, k, 2 + k / 8);
         if (threadIdx.x == 0) sh.bound = b;
     }
     __syncthreads();
@@ -124,7 +124,7 @@ template <int N, typename F> __device__ __forceinline__ void lp_best(LpShared& s
     for (int i = 0; i < N; ++i) most = e[i] > most ? e[i] : most;
     if (tid == 0) sh.n = 0u;
     unsigned long long b = lp_block_bound(sh, most, k);
-    // k + 16 threads at most have entries above the bound, and fewer than k have any where there is none: (k + 16) N entries
+    // k + 2 + k / 8 threads at most have entries above the bound, and fewer than k have any where there is none
     unsigned long long* all = &sh.list[0][0];   // (the lists are in registers)
 #pragma unroll
     for (int i = 0; i < N; ++i)
@@ -164,7 +164,8 @@ __global__ void __launch_bounds__(LP_THREADS, 2) k_logprobs(const LpArgs a) {
     auto index = [&](int i0, int j) { return i0 + (j >> 2) * (LP_BATCH / 2) + tid * 4 + (j & 3); };
     pdl_wait();
     pdl_go();
-    float r = -INFINITY, z = 0.f, s = 0.f, bound_v = -INFINITY;
+    float r = -INFINITY, bound_v = -INFINITY;
+    float2 z2 = make_float2(0.f, 0.f), s2 = make_float2(0.f, 0.f);   // the sums of the even and the odd values
     unsigned long long bound = 0ull;   // an entry has to be above it
     int cnt = 0;                       // this warp's list
     unsigned long long* list = sh.list[warp];
@@ -180,16 +181,18 @@ __global__ void __launch_bounds__(LP_THREADS, 2) k_logprobs(const LpArgs a) {
         for (int j = 1; j < LP_PER; ++j) mx = fmaxf(mx, v[j]);
         if (mx > r + 8.f || (r == -INFINITY && mx > -INFINITY)) {
             const float d = fmaxf(r - mx, -200.f), f = __expf(d);
-            s = f * (s + d * z);
-            z *= f;
+            s2.x = f * (s2.x + d * z2.x), s2.y = f * (s2.y + d * z2.y);
+            z2.x *= f, z2.y *= f;
             r = mx;
         }
-        const float ref = r == -INFINITY ? 0.f : r;
+        const float less = r == -INFINITY ? 0.f : -r;
 #pragma unroll
-        for (int j = 0; j < LP_PER; ++j) {
-            const float d = v[j] - ref, e = __expf(d);
-            z += e;
-            s = fmaf(e, fmaxf(d, -200.f), s);
+        for (int j = 0; j < LP_PER; j += 2) {
+            float2 d = add2(make_float2(v[j], v[j + 1]), make_float2(less, less)), e = mul2(d, make_float2(1.44269504f, 1.44269504f));
+            e.x = ex2_ftz(e.x), e.y = ex2_ftz(e.y);
+            d.x = fmaxf(d.x, -200.f), d.y = fmaxf(d.y, -200.f);
+            z2 = add2(z2, e);
+            s2 = fma2(e, d, s2);
         }
         if (!a.k) continue;
         if (i0 == lo) {
@@ -205,12 +208,15 @@ __global__ void __launch_bounds__(LP_THREADS, 2) k_logprobs(const LpArgs a) {
             bound -= bound != 0ull;   // the bound itself may enter
         }
         if (!__any_sync(0xffffffffu, mx >= bound_v)) continue;
+        unsigned any = 0u;
+#pragma unroll
+        for (int j = 0; j < LP_PER; ++j) any |= v[j] >= bound_v ? 1u << j : 0u;
+        any = __reduce_or_sync(0xffffffffu, any);
 #pragma unroll
         for (int j = 0; j < LP_PER; ++j) {
+            if (!(any >> j & 1u)) continue;
             const int p = index(i0, j);
             bool in = v[j] >= bound_v && p >= shift && p < hi;
-            unsigned who = __ballot_sync(0xffffffffu, in);
-            if (!who) continue;
             if (cnt + 32 > LP_LIST) {   // full: its best k stay
                 unsigned long long e[LP_LIST / 32];
                 __syncwarp();
@@ -230,16 +236,17 @@ __global__ void __launch_bounds__(LP_THREADS, 2) k_logprobs(const LpArgs a) {
             }
             const unsigned long long c = lp_composite(v[j], (unsigned) (p - shift));
             in = in && c > bound;
-            who = __ballot_sync(0xffffffffu, in);
+            const unsigned who = __ballot_sync(0xffffffffu, in);
             if (in) list[cnt + __popc(who & ((1u << lane) - 1u))] = c;
             cnt += __popc(who);
         }
     }
     // ---- the block's statistics
+    float z = z2.x + z2.y, s = s2.x + s2.y;
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
-        const float r2 = __shfl_xor_sync(0xffffffffu, r, o), z2 = __shfl_xor_sync(0xffffffffu, z, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
-        lp_join(r, z, s, r2, z2, s2);
+        const float ro = __shfl_xor_sync(0xffffffffu, r, o), zo = __shfl_xor_sync(0xffffffffu, z, o), so = __shfl_xor_sync(0xffffffffu, s, o);
+        lp_join(r, z, s, ro, zo, so);
     }
     if (lane == 0) sh.r[warp] = r, sh.z[warp] = z, sh.s[warp] = s;
     unsigned long long e[LP_LIST / 32];

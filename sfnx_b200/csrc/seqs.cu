@@ -77,35 +77,43 @@ template <int E> __device__ __forceinline__ void sa_store(uint16_t* p, const SaV
 }
 
 template <int HD>
-__global__ void __launch_bounds__(SA_THREADS) k_seqs_append(const __grid_constant__ SaArgs a) {
+__global__ void __launch_bounds__(SA_THREADS, 3) k_seqs_append(const __grid_constant__ SaArgs a) {
     constexpr int E = HD / 32;
-    __shared__ float sn[64], cs[64], rot[SA_WARPS][128];
+    __shared__ __align__(16) float sn[64], cs[64];
+    __shared__ float rot[SA_WARPS][128];
     const int t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nh = a.nq + 2 * a.nkv;
     pdl_wait();
     pdl_go();
     const int s = sq_find(a.sq.row0, a.sq.nseq, t);
     if (s < 0) return;   // behind the last sequence (the whole block agrees)
+    const size_t row_elems = (size_t) a.nkv * HD;
+    auto source = [&](int h) {
+        return (h < a.nq ? a.qg + ((size_t) t * a.nq + h) * 2 * HD : h < a.nq + a.nkv ? a.k + (size_t) t * row_elems + (size_t) (h - a.nq) * HD
+                                                                                        : a.v + (size_t) t * row_elems + (size_t) (h - a.nq - a.nkv) * HD) + lane * E;
+    };
+    SaVec<E> x[SA_HEADS];
+    auto ask = [&](int h0) {
+#pragma unroll
+        for (int b = 0; b < SA_HEADS; ++b)
+            if (h0 + b * SA_WARPS < nh) x[b] = sa_load<E>(source(h0 + b * SA_WARPS));
+    };
+    ask(warp);   // on their way while the row's place and angles are worked out
     const int i0 = t - a.sq.row0[s], p0 = a.sq.pos0[s];
-    const long long cell = sq_cell(a.sq, a.g, s, p0 < 0 || i0 > INT_MAX - p0 ? -1 : p0 + i0);
     const int turn = max(0, p0) + (a.depth ? max(0, a.depth[t]) : i0);
     if (threadIdx.x < a.nrot / 2) {
         const float theta = fmul((float) turn, a.freq[threadIdx.x]);
         ex_sincos((double) theta, &sn[threadIdx.x], &cs[threadIdx.x]);
     }
+    const long long cell = sq_cell(a.sq, a.g, s, p0 < 0 || i0 > INT_MAX - p0 ? -1 : p0 + i0);
     if (threadIdx.x == 0 && cell < 0) atomicOr(a.err, SQ_ERR_ROOM);
-    const size_t row_elems = (size_t) a.nkv * HD, at = cell < 0 ? 0 : sq_at(a.sq, a.g, cell, row_elems);
-    auto source = [&](int h) {
-        return (h < a.nq ? a.qg + ((size_t) t * a.nq + h) * 2 * HD : (h < a.nq + a.nkv ? a.k : a.v) + (size_t) t * row_elems + (size_t) ((h - a.nq) % a.nkv) * HD) +
-               lane * E;
-    };
-    SaVec<E> w[2];
-    w[0] = sa_load<E>(a.qn + lane * E), w[1] = sa_load<E>(a.kn + lane * E);
+    const size_t at = cell < 0 ? 0 : sq_at(a.sq, a.g, cell, row_elems);
     __syncthreads();
+    // element i < nrot pairs with i -+ half: y = c x + d x', d negative for the lower one.  Whole lanes apart (half a multiple of
+    // E) the partner comes by a shuffle, else through shared memory
+    const int half = a.nrot / 2, apart = half % E ? 0 : half / E;
+    const bool turned = lane * E < a.nrot, lower = lane * E < half;
     for (int h0 = warp; h0 < nh; h0 += SA_HEADS * SA_WARPS) {
-        SaVec<E> x[SA_HEADS];
-#pragma unroll
-        for (int b = 0; b < SA_HEADS; ++b)
-            if (h0 + b * SA_WARPS < nh) x[b] = sa_load<E>(source(h0 + b * SA_WARPS));
+        if (h0 != warp) ask(h0);
 #pragma unroll
         for (int b = 0; b < SA_HEADS; ++b) {
             const int h = h0 + b * SA_WARPS;
@@ -126,25 +134,38 @@ __global__ void __launch_bounds__(SA_THREADS) k_seqs_append(const __grid_constan
                 float tot = 0.f;
 #pragma unroll
                 for (int g = 0; g < E; ++g) tot = fadd(tot, __shfl_sync(0xffffffffu, q[0], g * (32 / E)));
-                const float r = ex_rsqrt(fadd(fdiv(tot, (float) HD), a.eps));
-                const SaVec<E>& wt = w[h < a.nq ? 0 : 1];
+                const float r = ex_rsqrt(fadd(fmul(tot, 1.0f / (float) HD), a.eps));   // (HD is a power of two: the quotient's bits)
+                const SaVec<E> wt = sa_load<E>((h < a.nq ? a.qn : a.kn) + lane * E);
 #pragma unroll
                 for (int e = 0; e < E; ++e) x[b].x[e] = fmul(fmul(x[b].x[e], r), wt.x[e]);
-                const int half = a.nrot / 2;
-                if (lane * E < a.nrot)
+                if (apart) {
+                    float other[E];
 #pragma unroll
-                    for (int e = 0; e < E; ++e) rot[warp][lane * E + e] = x[b].x[e];
-                __syncwarp();
+                    for (int e = 0; e < E; ++e) other[e] = __shfl_sync(0xffffffffu, x[b].x[e], lower ? lane + apart : lane - apart);
+                    if (turned) {
+                        const SaVec<E> c = sa_load<E>(&cs[lane * E - (lower ? 0 : half)]), d = sa_load<E>(&sn[lane * E - (lower ? 0 : half)]);
 #pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    const int i = lane * E + e;
-                    if (i < half) x[b].x[e] = ffma(-rot[warp][i + half], sn[i], fmul(x[b].x[e], cs[i]));
-                    else if (i < a.nrot) x[b].x[e] = ffma(x[b].x[e], cs[i - half], fmul(rot[warp][i - half], sn[i - half]));
+                        for (int e = 0; e < E; ++e)
+                            x[b].x[e] = lower ? ffma(-other[e], d.x[e], fmul(x[b].x[e], c.x[e])) : ffma(x[b].x[e], c.x[e], fmul(other[e], d.x[e]));
+                    }
+                } else {
+                    if (turned)
+#pragma unroll
+                        for (int e = 0; e < E; ++e) rot[warp][lane * E + e] = x[b].x[e];
+                    __syncwarp();
+#pragma unroll
+                    for (int e = 0; e < E; ++e) {
+                        const int i = lane * E + e;
+                        if (i < half) x[b].x[e] = ffma(-rot[warp][i + half], sn[i], fmul(x[b].x[e], cs[i]));
+                        else if (i < a.nrot) x[b].x[e] = ffma(x[b].x[e], cs[i - half], fmul(rot[warp][i - half], sn[i - half]));
+                    }
+                    __syncwarp();
                 }
-                __syncwarp();
             }
             if (h < a.nq) sa_store<E>(a.q16 + ((size_t) t * a.nq + h) * HD + lane * E, x[b]);
-            else if (cell >= 0) sa_store<E>((h < a.nq + a.nkv ? a.kc : a.vc) + at + (size_t) ((h - a.nq) % a.nkv) * HD + lane * E, x[b]);
+            else if (h < a.nq + a.nkv) {
+                if (cell >= 0) sa_store<E>(a.kc + at + (size_t) (h - a.nq) * HD + lane * E, x[b]);
+            } else if (cell >= 0) sa_store<E>(a.vc + at + (size_t) (h - a.nq - a.nkv) * HD + lane * E, x[b]);
         }
     }
 }

@@ -63,11 +63,6 @@ __device__ __forceinline__ void sa_init(unsigned long long* bar, unsigned n) {
 __device__ __forceinline__ void sa_arrive(unsigned long long* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(um_s32(bar)) : "memory");
 }
-__device__ __forceinline__ float sa_ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 __device__ __forceinline__ void sa_tma3d(unsigned dst, const CUtensorMap* map, int x, int y, int z, unsigned long long* bar) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(map),
                  "r"(x), "r"(y), "r"(z), "r"(um_s32(bar))
@@ -368,7 +363,7 @@ __global__ void __launch_bounds__(SA_THREADS, 1) k_attn_seqs(const __grid_consta
             mx = fmaxf(mx, xmax[(half ^ 1) * SA_ROWS + m]) * scale;
             asm volatile("bar.sync 2, %0;" ::"n"(SA_SOFT) : "memory");   // read before the next tile's are written
             const bool up = mx > ref + 8.0f || (ref == -INFINITY && mx != -INFINITY);
-            const float f = !up ? 1.0f : ref == -INFINITY ? 0.f : sa_ex2(ref - mx);
+            const float f = !up ? 1.0f : ref == -INFINITY ? 0.f : ex2_ftz(ref - mx);
             if (up) ref = mx;
             z *= f;
             if (i > 0 && __any_sync(0xffffffffu, up)) {   // O row *= f, this half's columns
@@ -389,7 +384,7 @@ __global__ void __launch_bounds__(SA_THREADS, 1) k_attn_seqs(const __grid_consta
             float s0 = 0.f, s1 = 0.f;
 #pragma unroll
             for (int j = 0; j < 32; ++j) {
-                const float p = sa_ex2(fmaf(x[2 * j], scale, -base)), q = sa_ex2(fmaf(x[2 * j + 1], scale, -base));
+                const float p = ex2_ftz(fmaf(x[2 * j], scale, -base)), q = ex2_ftz(fmaf(x[2 * j + 1], scale, -base));
                 s0 += p, s1 += q;
                 const __half2 h = __floats2half2_rn(p, q);
                 pk[j] = *reinterpret_cast<const unsigned*>(&h);
@@ -476,7 +471,7 @@ template <int HD> __global__ void __launch_bounds__(128) k_attn_seqs_join(const 
         if (n <= 0) break;
         const float2 x = *reinterpret_cast<const float2*>(mz + ((size_t) p * all + cell) * 2);
         if (x.x == -INFINITY) continue;   // the row sees nothing there
-        const float rn = fmaxf(ref, x.x), f0 = sa_ex2(ref - rn), f1 = sa_ex2(x.x - rn);
+        const float rn = fmaxf(ref, x.x), f0 = ex2_ftz(ref - rn), f1 = ex2_ftz(x.x - rn);
         z = z * f0 + x.y * f1;
         ref = rn;
         const float* src = a.part + ((size_t) p * all + cell) * HD + lane * E;
