@@ -1,26 +1,34 @@
 // Attention of several sequences' rows over the f16 cache: prompts, chunks of prompts, single tokens and draft trees (no
 // counterpart in the reference's windows), on the fifth-generation tensor cores.
 //
-// A CTA takes one KV head, up to 128 query rows of one sequence - 128 / qpk tokens (qpk query heads a KV head, rounded down), row
-// m = token m / qpk, head m % qpk, so that one pass over K and V serves all heads that share them and single tokens fill more
-// than one row - and a range of that sequence's positions in tiles of 128.  S = Q K^T (128 x 128 fp32, operands in shared memory)
-// and O += P V (P in tensor memory as the A operand, V as it lies: dims contiguous, "MN-major") both accumulate in tensor
-// memory.  Roles: warp 0 copies (TMA, K and V boxes found through the page table), warp 1 issues the MMAs, warps 4 - 11 take the
-// softmax step: a thread has one row and half of a tile's columns, the halves of a row agree on the maximum through shared
-// memory.
+// A unit of work is one KV head, up to 256 query rows of one sequence - 2 x 128 / qpk tokens (qpk query heads a KV head, rounded
+// down); row m of each 128 is token m / qpk, head m % qpk, so that one pass over K and V serves all heads that share them and
+// single tokens fill more than one row - and the positions they see, in tiles of 128.  A pair of CTAs on neighbouring
+// multiprocessors takes it (cta_group::2): each holds 128 of the rows, and half of every K tile (64 positions) and V tile (half of
+// the dims), which the pair's MMAs read from both, so a tile crosses from L2 once for 256 rows.  (One CTA a unit moved 128 KB
+// of K and V a tile and 128 rows, 11 TB/s out of L2 at 880 TFLOP/s, and was bound by it.)
+// The work of all units, one after another, is dealt to the pairs (one on every two multiprocessors, persistent) in equal runs,
+// whatever the sequences' lengths; where a run begins or ends inside a unit the pair leaves its part of the result, (O,
+// reference, z), and a second kernel joins the parts.
+// S = Q K^T (256 x 128 fp32, operands in shared memory) and O += P V (P in tensor memory as the A operand, V as it lies: dims
+// contiguous, "MN-major") both accumulate in tensor memory, each CTA's rows in its own.  Roles: warp 0 copies (TMA, K and V
+// boxes found through the page table), warp 2 tells the pair's first CTA what has landed, warp 1 of that CTA issues the MMAs,
+// warps 4 - 11 take the softmax step: a thread has one row and half of a tile's columns, the halves of a row agree on the
+// maximum through shared memory.
 //   tensor memory: O (HD columns), one S tile (128), two P tiles (64 columns each, f16 pairs).  S(i + 1) is issued when the softmax
 //   warps have S(i) in registers, so the tensor core computes it - and, when P(i) is written, O += P(i) V(i) - while they take
-//   exponentials: a tile costs the longer of the two, not the sum.
-//   shared memory: Q, and a ring of 32 KB slots (for HD 256 half a K tile: 128 rows x 128 dims, or half a V tile: 64 rows x 256
-//   dims) that are asked for in the order of their use: K(0), K(1), V(0), K(2), V(1), ...
+//   exponentials: a tile costs the longer of the two, not the sum.  The next unit's copies and first scores run while the
+//   softmax warps write this one's rows.
+//   shared memory: Q, a ring of slots of half a tile each, asked for in the order of their use: K(0), K(1), V(0), K(2), V(1), ...,
+//   and a strip a softmax warp to turn rows into whole lines on their way out.
 // Softmax: x = s log2 e / sqrt(hd); weights 2^(x - ref) against a reference that is raised - and O and the sums rescaled - only when
 // a row's maximum has grown by more than 8 over it, so weights stay below 2^8 and (O, ref, z) is an exact partial for any
 // reference.  z sums the weights in 32 bits before they are rounded to f16 for the product (2^-11 of a weight: the
 // result's own rounding is as large; f16 queries, keys and values enter exactly).
-// Positions past a CTA's last visible one are not loaded beyond their box; V rows there are cleared in shared memory, since a
+// Positions past a unit's last visible one are not loaded beyond their box; V rows there are cleared in shared memory, since a
 // weight of zero times a stray NaN is a NaN.
-// Few rows over many positions: nsplit CTAs share a sequence's positions, their (O, ref, z) are joined by a second kernel.
 // Every wait on an mbarrier is bounded; on a timeout the fault word is set and the CTA ends with nothing in flight.
+#include <algorithm>
 #include <cstring>
 
 #include "exact_math.cuh"
@@ -30,14 +38,15 @@
 
 namespace fnxk {
 
-constexpr int SA_ROWS = 128, SA_KT = 128, SA_SLOT = 32768, SA_THREADS = 384, SA_SOFT = 256;
+constexpr int SA_ROWS = 128, SA_KT = 128, SA_THREADS = 384, SA_SOFT = 256, SA_STRIP = 4096;
+constexpr int SA_COST = 256;    // what a unit's beginning and end cost, in positions
+constexpr int SA_LEAST = 256;   // work a pair gets at least, in positions
 template <int HD> struct SaShape {
-    static constexpr int HALVES = HD / 128;                 // slots a K or V tile takes
-    static constexpr int VROWS = SA_KT / HALVES;            // V rows a slot holds
     static constexpr int QBYTES = SA_ROWS * HD * 2;
-    static constexpr int SLOTS = HD == 256 ? 5 : 6;
+    static constexpr int SLOT = SA_KT / 2 * HD * 2;         // half a K or V tile
+    static constexpr int SLOTS = HD == 256 ? 4 : 8;
     static constexpr int COL_S = HD, COL_P = HD + SA_KT;    // tensor memory columns; O from 0
-    static constexpr size_t SMEM = (size_t) QBYTES + (size_t) SLOTS * SA_SLOT + 1024 /* alignment */ + 2 * SA_ROWS * 4 + 256;
+    static constexpr size_t SMEM = (size_t) QBYTES + (size_t) SLOTS * SLOT + SA_SOFT / 32 * SA_STRIP + 4 * SA_ROWS * 4 + 512;
 };
 
 struct SqMaps {
@@ -50,10 +59,10 @@ struct SqAttn {
     const unsigned* anc;
     uint16_t* out;
     int out_stride, nq, nkv, words;
-    int tok;      // tokens a CTA takes: 128 / qpk
+    int tok;      // tokens of a CTA's rows: 128 / qpk
     int box;      // cache rows a copy brings: a power of two that divides a page's rows
-    int nsplit;
-    float* part;  // [nsplit][rows][nq][HD], then (ref, z) [nsplit][rows][nq][2]
+    int pairs;    // the scan's pairs of CTAs
+    float* part;  // [2 pairs][2][128][HD] parts of units, then (ref, z) [2 pairs][2][128][2]
     unsigned* fault;
 };
 
@@ -63,15 +72,44 @@ __device__ __forceinline__ void sa_init(unsigned long long* bar, unsigned n) {
 __device__ __forceinline__ void sa_arrive(unsigned long long* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(um_s32(bar)) : "memory");
 }
+// arrives at the barrier of the pair's first CTA that lies where `bar` does in this one: for what was written to shared memory,
+// and for tensor memory, whose accesses are ordered by the tcgen05 fences (a release to the cluster takes 1000 cycles)
+__device__ __forceinline__ void sa_tell_shared(unsigned long long* bar) {
+    asm volatile("{\n\t.reg .b32 r;\n\tmapa.shared::cluster.u32 r, %0, 0;\n\tmbarrier.arrive.release.cluster.shared::cluster.b64 _, [r];\n\t}" ::"r"(um_s32(bar))
+                 : "memory");
+}
+__device__ __forceinline__ void sa_tell(unsigned long long* bar) {
+    asm volatile("{\n\t.reg .b32 r;\n\tmapa.shared::cluster.u32 r, %0, 0;\n\tmbarrier.arrive.shared::cluster.b64 _, [r];\n\t}" ::"r"(um_s32(bar)) : "memory");
+}
+__device__ __forceinline__ void sa_cluster() {   // both CTAs of the pair, every thread
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void sa_tma4d(unsigned dst, const CUtensorMap* map, int x, int y, int z, int w, unsigned long long* bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst), "l"(map),
+                 "r"(x), "r"(y), "r"(z), "r"(w), "r"(um_s32(bar))
+                 : "memory");
+}
 __device__ __forceinline__ void sa_tma3d(unsigned dst, const CUtensorMap* map, int x, int y, int z, unsigned long long* bar) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(map),
                  "r"(x), "r"(y), "r"(z), "r"(um_s32(bar))
                  : "memory");
 }
-// D[tmem] (+)= A B with A in tensor memory (a lane a row, two f16 a column)
-__device__ __forceinline__ void sa_mma_ts(unsigned tmem, unsigned a, unsigned long long db, unsigned idesc, unsigned accumulate) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem), "r"(a), "l"(db),
+// the pair's MMAs, 256 rows: D[tmem] (+)= A B, each CTA's half of A's rows and of B's columns in its own memories
+__device__ __forceinline__ void sa_mma(unsigned tmem, unsigned long long da, unsigned long long db, unsigned idesc, unsigned accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem), "l"(da), "l"(db),
                  "r"(idesc), "r"(accumulate)
+                 : "memory");
+}
+// the same with A in tensor memory (a lane a row, two f16 a column)
+__device__ __forceinline__ void sa_mma_ts(unsigned tmem, unsigned a, unsigned long long db, unsigned idesc, unsigned accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem), "r"(a), "l"(db),
+                 "r"(idesc), "r"(accumulate)
+                 : "memory");
+}
+// `bar` of both CTAs gets one arrival when every MMA that this thread has issued is done
+__device__ __forceinline__ void sa_commit(unsigned long long* bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(um_s32(bar)), "h"((unsigned short) 3)
                  : "memory");
 }
 // 32 columns of the calling thread's lane of tensor memory
@@ -98,47 +136,134 @@ __device__ __forceinline__ void sa_wait_st() { asm volatile("tcgen05.wait::st.sy
 __device__ __forceinline__ void sa_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void sa_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-// Unit u of the call, a KV head of a sequence's token block: the sequences' blocks one after another, a sequence's last (its
-// longest) first.  false: there are not that many.  Called by a converged warp.
+// A unit: a KV head of a sequence's block of 2 tok tokens.  Units follow one another head by head, block by block, sequence by
+// sequence; a unit's work is counted as SA_COST and the positions it sees.
 struct SqUnit {
-    int s, tok0, ntok, head, kv_len, pos0, row;   // sequence, first token, tokens, KV head, positions the CTA's rows see, packed row
+    int s, r0, len, pos0;   // sequence, its first packed row, its rows, the positions before them
+    int tok0, head;         // first token, KV head
+    int end, kv_len;        // positions the unit's rows see; those of them that the cache has room for
 };
-__device__ __forceinline__ bool sq_unit(const SqAttn& a, int u, SqUnit& w) {
+__device__ __forceinline__ void sq_seq(const SqAttn& a, int s, int& r0, int& len, int& pos0) {
+    r0 = max(a.sq.row0[s], 0), len = max(min(a.sq.row0[s + 1], a.sq.rows) - r0, 0), pos0 = min(max(a.sq.pos0[s], 0), 1 << 30);
+}
+// work of a KV head's first b blocks (all but a sequence's last are whole)
+__device__ __forceinline__ long long sq_blocks(const SqAttn& a, int len, int pos0, int b) {
+    const long long n = b, each = (long long) pos0 + SA_COST + (a.anc ? len : 0);
+    return n * each + (a.anc ? 0 : n * (n + 1) * a.tok);
+}
+__device__ __forceinline__ long long sq_work(const SqAttn& a, int len, int pos0) {   // of a sequence
+    return len ? (sq_blocks(a, len, pos0, (len - 1) / (2 * a.tok)) + pos0 + len + SA_COST) * a.nkv : 0;
+}
+__device__ __forceinline__ void sq_fill(const SqAttn& a, SqUnit& u) {
+    u.end = u.pos0 + (a.anc ? u.len : min(u.tok0 + 2 * a.tok, u.len));
+    u.kv_len = (int) min((long long) u.end, a.sq.pt ? (long long) a.sq.pt_stride * a.g.rows : (long long) a.g.cap);
+}
+__device__ __forceinline__ long long sq_shfl(long long v, int lane) { return __shfl_sync(0xffffffffu, v, lane); }
+// how the work is dealt: all of it, and the pairs that get any
+__device__ __forceinline__ long long sq_div(long long x, unsigned d) { return x >> 32 ? x / d : (long long) ((unsigned) x / d); }   // x >= 0
+struct SqPlan {
+    long long total, each;   // each = total / pairs
+    int pairs;
+    __device__ __forceinline__ long long begin(int g) const { return each * g + (unsigned) (total - each * pairs) * (unsigned) g / (unsigned) pairs; }
+};
+__device__ __forceinline__ SqPlan sq_plan(const SqAttn& a) {   // called by a converged warp
     const int lane = threadIdx.x & 31;
-    int t = u / a.nkv;
-    w.head = u % a.nkv;
-    for (int s0 = 0; s0 < a.sq.nseq; s0 += 32) {
+    long long w = 0;
+    for (int s = lane; s < a.sq.nseq; s += 32) {
+        int r0, len, pos0;
+        sq_seq(a, s, r0, len, pos0);
+        w += sq_work(a, len, pos0);
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
+    SqPlan p;
+    p.total = w;
+    p.pairs = (int) min((long long) a.pairs, w ? max(1ll, w / SA_LEAST) : 0ll);   // a run is never shorter than a tile
+    p.each = p.pairs ? sq_div(w, p.pairs) : 0;
+    return p;
+}
+// the unit that work item `at` (below the plan's total) belongs to; `at` is left relative to the unit.  Called by a converged warp
+__device__ __forceinline__ SqUnit sq_locate(const SqAttn& a, long long& at) {
+    const int lane = threadIdx.x & 31;
+    SqUnit u;
+    for (int s0 = 0;; s0 += 32) {   // the sequence
         const int s = s0 + lane;
-        int r0 = 0, len = 0;
-        if (s < a.sq.nseq) r0 = max(a.sq.row0[s], 0), len = max(min(a.sq.row0[s + 1], a.sq.rows) - r0, 0);
-        const int mine = (len + a.tok - 1) / a.tok;
-        int upto = mine;
+        int r0 = 0, len = 0, pos0 = 0;
+        if (s < a.sq.nseq) sq_seq(a, s, r0, len, pos0);
+        const long long mine = sq_work(a, len, pos0);
+        long long w = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int y = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += y;
+            const long long y = __shfl_up_sync(0xffffffffu, w, o);
+            if (lane >= o) w += y;
         }
-        const unsigned past = __ballot_sync(0xffffffffu, upto > t);
-        if (past) {
-            const int l = __ffs(past) - 1;
-            const int b = __shfl_sync(0xffffffffu, upto, l) - 1 - t;   // blocks from the sequence's last back
-            len = __shfl_sync(0xffffffffu, len, l), r0 = __shfl_sync(0xffffffffu, r0, l);
-            w.s = s0 + l, w.tok0 = b * a.tok, w.ntok = min(a.tok, len - w.tok0), w.row = r0 + w.tok0;
-            w.pos0 = max(a.sq.pos0[w.s], 0);
-            const long long cap = a.sq.pt ? (long long) a.sq.pt_stride * a.g.rows : (long long) a.g.cap;
-            w.kv_len = (int) min((long long) w.pos0 + (a.anc ? len : w.tok0 + w.ntok), cap);
-            return true;
+        const unsigned past = __ballot_sync(0xffffffffu, w > at);
+        if (past || s0 + 32 >= a.sq.nseq) {
+            const int l = past ? __ffs(past) - 1 : 0;
+            at -= sq_shfl(w - mine, l);
+            u.s = s0 + l, u.r0 = __shfl_sync(0xffffffffu, r0, l), u.len = __shfl_sync(0xffffffffu, len, l), u.pos0 = __shfl_sync(0xffffffffu, pos0, l);
+            break;
         }
-        t -= __shfl_sync(0xffffffffu, upto, 31);
+        at -= sq_shfl(w, 31);
     }
-    return false;
+    int lo = 0, hi = (u.len + 2 * a.tok - 1) / (2 * a.tok);   // the block: the last that does not begin past `at`
+    while (hi - lo > 1) {
+        const int step = (hi - lo + 31) / 32, b = lo + lane * step;
+        const unsigned in = __ballot_sync(0xffffffffu, b < hi && sq_blocks(a, u.len, u.pos0, b) * a.nkv <= at);
+        lo += (__popc(in) - 1) * step;
+        hi = min(hi, lo + step);
+    }
+    at -= sq_blocks(a, u.len, u.pos0, lo) * a.nkv;
+    u.tok0 = lo * 2 * a.tok;
+    sq_fill(a, u);
+    u.head = (int) sq_div(at, u.end + SA_COST);
+    at -= (long long) u.head * (u.end + SA_COST);
+    return u;
 }
-// the range of tiles that split `split` of a unit takes
-__device__ __forceinline__ void sq_range(int kv_len, int split, int nsplit, int& first, int& n) {
-    const int tiles = (kv_len + SA_KT - 1) / SA_KT, per = (tiles + nsplit - 1) / nsplit;
-    first = min(split * per, tiles);
-    n = min(per, tiles - first);
+__device__ __forceinline__ void sq_next(const SqAttn& a, SqUnit& u) {   // there is one
+    if (++u.head < a.nkv) return;
+    u.head = 0;
+    u.tok0 += 2 * a.tok;
+    while (u.tok0 >= u.len && u.s + 1 < a.sq.nseq) {
+        ++u.s;
+        u.tok0 = 0;
+        sq_seq(a, u.s, u.r0, u.len, u.pos0);
+    }
+    sq_fill(a, u);
 }
+// the tile of a unit that work item x of it stands for: a run that ends at x ends before that tile
+__device__ __forceinline__ int sq_tile(long long x) { return x <= SA_COST ? 0 : (int) ((x - SA_COST) / SA_KT); }
+
+// A pair's run of work as segments, one a unit: tiles [t0, t0 + n) of it, n 0 where the cache ends before them
+struct SqRun {
+    SqUnit u;
+    long long left;   // from the unit's beginning to the run's end
+    int t0, n;
+    int cut, first;   // the segment is part of its unit only; it is the run's first
+    // field by field: a struct copied whole would live on the stack, 300 cycles from the MMAs' issue
+    __device__ __forceinline__ void put(volatile int* w) const {
+        w[0] = u.s, w[1] = u.r0, w[2] = u.len, w[3] = u.pos0, w[4] = u.tok0, w[5] = u.head, w[6] = u.end, w[7] = u.kv_len;
+        w[8] = (int) left, w[9] = (int) (left >> 32), w[10] = t0, w[11] = n, w[12] = cut, w[13] = first;
+    }
+    __device__ __forceinline__ void get(const volatile int* w) {
+        u.s = w[0], u.r0 = w[1], u.len = w[2], u.pos0 = w[3], u.tok0 = w[4], u.head = w[5], u.end = w[6], u.kv_len = w[7];
+        left = (long long) ((unsigned long long) (unsigned) w[8] | ((unsigned long long) (unsigned) w[9] << 32)), t0 = w[10], n = w[11], cut = w[12], first = w[13];
+    }
+    __device__ __forceinline__ bool measure(int from) {
+        const int tiles = (u.end + SA_KT - 1) / SA_KT, to = left >= u.end + SA_COST ? tiles : sq_tile(left);
+        t0 = from;
+        n = max(0, min(to, (u.kv_len + SA_KT - 1) / SA_KT) - t0);
+        cut = from > 0 || to < tiles;
+        return to > from;
+    }
+    __device__ __forceinline__ bool next(const SqAttn& a) {
+        left -= u.end + SA_COST;
+        if (left <= 0) return false;
+        sq_next(a, u);
+        first = 0;
+        return measure(0);
+    }
+};
 
 // 32 positions' visibility of a tree's row, from position rel past the sequence's pos0 on
 __device__ __forceinline__ unsigned sq_tree_bits(const unsigned* anc, int words, int rel) {
@@ -150,378 +275,551 @@ __device__ __forceinline__ unsigned sq_tree_bits(const unsigned* anc, int words,
 }
 __device__ __forceinline__ unsigned sq_first(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
 
+// Waits for a phase of `bar`, at most `spins` polls of up to 16 us (asleep: warps that poll without a break keep the barriers'
+// unit from the one that issues the MMAs); a wait that ran out is reported, and later ones of the thread do not linger
+constexpr int SA_SPINS = 1 << 16;
+__device__ __forceinline__ bool sa_wait(unsigned long long* bar, unsigned parity, int& spins, unsigned* fault) {
+    unsigned ok = 0;
+    for (int spin = 0; spin < spins && !ok; ++spin)
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                     : "=r"(ok)
+                     : "r"(um_s32(bar)), "r"(parity), "r"(16384u)
+                     : "memory");
+    if (!ok) spins = 1, atomicOr(fault, 8u);
+    return ok != 0;
+}
+// the same by one lane for its warp (all lanes get the answer)
+__device__ __forceinline__ bool sa_wait_warp(unsigned long long* bar, unsigned parity, int& spins, unsigned* fault) {
+    bool ok = true;
+    if (um_elect()) ok = sa_wait(bar, parity, spins, fault);
+    return __all_sync(0xffffffffu, ok);
+}
+
 template <int HD>
-__global__ void __launch_bounds__(SA_THREADS, 1) k_attn_seqs(const __grid_constant__ SqMaps maps, const __grid_constant__ SqAttn a) {
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(SA_THREADS, 1) k_attn_seqs(const __grid_constant__ SqMaps maps, const __grid_constant__ SqAttn a) {
     using S = SaShape<HD>;
-    extern __shared__ unsigned char sa_smem[];
-    unsigned char* Q = sa_smem + ((1024u - (um_s32(sa_smem) & 1023u)) & 1023u);
-    unsigned char* ring = Q + S::QBYTES;
-    float* xmax = reinterpret_cast<float*>(ring + S::SLOTS * SA_SLOT);   // [2][128] the halves' maxima (at the end: their sums)
-    unsigned long long* bars = reinterpret_cast<unsigned long long*>(xmax + 2 * SA_ROWS);
-    unsigned long long *full = bars, *empty = bars + S::SLOTS, *q_full = empty + S::SLOTS, *s_full = q_full + 1, *s_free = q_full + 2, *p_full = q_full + 3,
-                       *o_full = q_full + 5, *idle = q_full + 7;
-    volatile unsigned* tmem_at = reinterpret_cast<unsigned*>(q_full + 8);
-    const int tid = threadIdx.x, warp = (int) um_uniform(tid >> 5), lane = tid & 31;
-    pdl_wait();
-    pdl_go();
-    SqUnit w;
-    if (!sq_unit(a, blockIdx.x, w)) return;
-    int first, n;
-    sq_range(w.kv_len, blockIdx.y, a.nsplit, first, n);
-    if (n <= 0 && a.nsplit > 1) return;   // (the join knows)
-    const int qpk = a.nq / a.nkv;
+    extern __shared__ __align__(1024) unsigned char sa_smem[];
+    unsigned char *Q = sa_smem, *ring = Q + S::QBYTES, *strips = ring + S::SLOTS * S::SLOT;
+    float* xmax = reinterpret_cast<float*>(strips + SA_SOFT / 32 * SA_STRIP);   // [2][2][128] the halves' maxima, of odd and even tiles
+    unsigned long long* bars = reinterpret_cast<unsigned long long*>(xmax + 4 * SA_ROWS);
+    // full, q_full: this CTA's copies have landed.  ready, q_ready, s_free, p_full, o_free count both CTAs', in the first one's
+    // memory.  empty, q_empty, s_full, o_full: MMAs are done, told to both
+    unsigned long long *full = bars, *empty = full + S::SLOTS, *ready = empty + S::SLOTS, *q_full = ready + S::SLOTS, *q_ready = q_full + 1, *q_empty = q_full + 2,
+                       *s_full = q_full + 3, *s_free = q_full + 4, *o_free = q_full + 5, *idle = q_full + 6, *p_full = q_full + 7, *o_full = q_full + 9;
+    volatile int* run_at = reinterpret_cast<int*>(q_full + 12);
+    volatile unsigned *tmem_at = reinterpret_cast<unsigned*>(q_full + 11), *work_at = tmem_at + 1;
+    const int tid = threadIdx.x, warp = (int) um_uniform(tid >> 5), lane = tid & 31, rank = blockIdx.x & 1, g = blockIdx.x >> 1;
     if (tid == 0) {
-        for (int i = 0; i < S::SLOTS; ++i) sa_init(&full[i], 1), sa_init(&empty[i], 1);
-        sa_init(q_full, 1), sa_init(s_full, 1), sa_init(s_free, SA_SOFT / 32), sa_init(idle, 1);
-        for (int i = 0; i < 2; ++i) sa_init(&p_full[i], SA_SOFT / 32), sa_init(&o_full[i], 1);
+        for (int i = 0; i < S::SLOTS; ++i) sa_init(&full[i], 1), sa_init(&empty[i], 1), sa_init(&ready[i], 2);
+        sa_init(q_full, 1), sa_init(q_ready, 2), sa_init(q_empty, 1), sa_init(s_full, 1), sa_init(s_free, 2 * SA_SOFT / 32), sa_init(o_free, 2 * SA_SOFT / 32);
+        sa_init(idle, 1);
+        for (int i = 0; i < 2; ++i) sa_init(&p_full[i], 2 * SA_SOFT / 32), sa_init(&o_full[i], 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    if (warp == 0 && um_elect()) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.q) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.k) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.v) : "memory");
+    }
     if (warp == 2) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(um_s32((const void*) tmem_at)), "r"(512));
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(um_s32((const void*) tmem_at)), "r"(512));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    }
+    pdl_wait();
+    pdl_go();
+    if (warp == 3) {   // the pair's run of work
+        const SqPlan plan = sq_plan(a);
+        const bool any = g < plan.pairs;
+        SqRun r = {};
+        bool some = false;
+        if (any) {
+            const long long lo = plan.begin(g);
+            long long at = lo;
+            r.u = sq_locate(a, at);
+            r.left = plan.begin(g + 1) - lo + at;
+            r.first = 1;
+            some = r.measure(sq_tile(at));
+            if (!some) r.left = 0;
+        }
+        if (lane == 0) {
+            r.put(run_at);
+            *work_at = some;
+        }
     }
     sa_before();
-    __syncthreads();
+    sa_cluster();   // barriers and tensor memory of both CTAs are there
     sa_after();
     const unsigned tm = um_uniform(*tmem_at);
-    bool alive = true;
-
+    const int qpk = a.nq / a.nkv;
+    int spins = SA_SPINS;
+    const bool work = um_uniform(*work_at) != 0;
+    auto leave = [&]() {
+        sa_before();
+        asm volatile("bar.sync 0, %0;" ::"n"(SA_THREADS) : "memory");
+        sa_cluster();   // the pair's MMAs read both CTAs' memories
+        if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tm), "r"(512));
+    };
+    // the softmax warps hold 64 scores and 32 packed weights a thread: they take registers from the first four warps (128 x 72 +
+    // 256 x 216 of the launch's 384 x 168)
+    if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (warp == 0) {
-        // ---- copies.  Load number c of the ring takes slot c % SLOTS; tile i's K loads come before tile i - 1's V loads
-        int c = 0;
-        const int boxes = SA_KT / a.box;
-        auto acquire = [&]() {
-            const int slot = c % S::SLOTS;
-            if (c >= S::SLOTS) alive = alive && __all_sync(0xffffffffu, um_wait(&empty[slot], (unsigned) (c / S::SLOTS - 1) & 1u, a.fault));
-            return slot;
-        };
-        // lane j < boxes: where box j of a tile lies (row in the page, page)
-        auto place = [&](int tile, int& y, int& z) {
+        // ---- copies.  Load number c of the ring takes slot c % SLOTS; tile i's K load comes before tile i - 1's V load.  A slot
+        // holds groups of 64 rows, each as column blocks of 64 dims (8 KB, swizzled)
+        int c = 0, nseg = 0, kv0 = 0;
+        bool alive = true;
+        SqRun r;
+        r.get(run_at);
+        // lane j looks after box j of a tile: the table's entry, asked for a tile ahead, and with it where the box lies
+        auto entry = [&](int tile) {
             const int p = tile * SA_KT + lane * a.box;
-            y = z = 0;
-            if (lane >= boxes || p >= w.kv_len) return;
-            if (!a.sq.pt) {
-                y = (a.sq.kv0 ? a.sq.kv0[w.s] : 0) + p;
-                return;
-            }
-            const int page = a.sq.pt[(size_t) w.s * a.sq.pt_stride + p / a.g.rows];
-            y = p % a.g.rows, z = page >= 0 && page < a.sq.npages ? page : a.sq.npages;   // past the pool: zeros
+            return a.sq.pt && lane * a.box < SA_KT && p < r.u.kv_len ? a.sq.pt[(size_t) r.u.s * a.sq.pt_stride + p / a.g.rows] : 0;
         };
-        // rows lo .. hi - 1 of a tile, column blocks of 64 dims cb .. cb + nb - 1, into a slot; a block's rows are `stride` bytes apart from the next's
-        auto load = [&](const CUtensorMap* map, int tile, int y, int z, int lo, int hi, int cb, int nb, int stride) {
+        auto place = [&](int tile, int e, int& y, int& z) {   // row in the page, page (past the pool: zeros)
+            const int p = tile * SA_KT + lane * a.box;
+            y = a.sq.pt ? p % a.g.rows : kv0 + p, z = !a.sq.pt ? 0 : e >= 0 && e < a.sq.npages ? e : a.sq.npages;
+        };
+        // rows lo .. lo + rows - 1 of a tile, nb column blocks from block x on, into the next slot
+        auto load = [&](const CUtensorMap* map, int tile, int y, int z, int lo, int rows, int x, int nb) {
+            const int slot = c % S::SLOTS;
+            if (c >= S::SLOTS) alive = alive && sa_wait_warp(&empty[slot], (unsigned) (c / S::SLOTS - 1) & 1u, spins, a.fault);
             if (!alive) return;
-            const int slot = acquire();
-            if (!alive) return;
-            const int have = min(hi, w.kv_len - tile * SA_KT) - lo, nbox = max(0, (have + a.box - 1) / a.box);
-            const unsigned dst = um_s32(ring) + slot * SA_SLOT;
-            const bool elected = um_elect();
-            if (elected) um_expect_tx(&full[slot], (unsigned) (nbox * nb * a.box * 128));
-            for (int j = 0; j < nbox; ++j) {
-                const int at = lo / a.box + j, yj = __shfl_sync(0xffffffffu, y, at), zj = __shfl_sync(0xffffffffu, z, at);
-                if (elected)
-                    for (int b = 0; b < nb; ++b) sa_tma3d(dst + b * stride + j * a.box * 128, map, w.head * HD + (cb + b) * 64, yj, zj, &full[slot]);
+            const int have = min(rows, r.u.kv_len - tile * SA_KT - lo);
+            const unsigned dst = um_s32(ring) + slot * S::SLOT;
+            if (a.box == 64) {   // a box is a group, with its column blocks
+                const int y0 = __shfl_sync(0xffffffffu, y, lo / 64), z0 = __shfl_sync(0xffffffffu, z, lo / 64), y1 = __shfl_sync(0xffffffffu, y, 1),
+                          z1 = __shfl_sync(0xffffffffu, z, 1);
+                if (um_elect()) {
+                    um_expect_tx(&full[slot], (unsigned) (have > 64 ? 2 : have > 0 ? 1 : 0) * nb * 8192);
+                    if (have > 0) sa_tma4d(dst, map, 0, y0, x, z0, &full[slot]);
+                    if (have > 64) sa_tma4d(dst + nb * 8192, map, 0, y1, x, z1, &full[slot]);
+                }
+            } else {
+                const int nbox = max(0, (have + a.box - 1) / a.box);
+                const bool elected = um_elect();
+                if (elected) um_expect_tx(&full[slot], (unsigned) (nbox * nb * a.box * 128));
+                for (int j = 0; j < nbox; ++j) {
+                    const int at = lo / a.box + j, yj = __shfl_sync(0xffffffffu, y, at), zj = __shfl_sync(0xffffffffu, z, at), row = j * a.box;
+                    if (elected)
+                        for (int b = 0; b < nb; ++b) sa_tma4d(dst + (row / 64 * nb + b) * 8192 + row % 64 * 128, map, 0, yj, x + b, zj, &full[slot]);
+                }
             }
             __syncwarp();
             ++c;
         };
-        if (n > 0 && um_elect()) {
-            um_expect_tx(q_full, (unsigned) (a.tok * qpk * HD * 2));
-            for (int b = 0; b < HD / 64; ++b) sa_tma3d(um_s32(Q) + b * (SA_ROWS * 128), &maps.q, b * 64, w.head * qpk, w.row, q_full);
-        }
-        __syncwarp();
-        int y0, z0, y1, z1;
-        if (n > 0) place(first, y0, z0);
-        for (int i = 0; i < n && alive; ++i) {
-            if (i == 0)
-                for (int h = 0; h < S::HALVES; ++h) load(&maps.k, first, y0, z0, 0, SA_KT, 2 * h, 2, SA_KT * 128);
-            if (i + 1 < n) {
-                place(first + i + 1, y1, z1);
-                for (int h = 0; h < S::HALVES; ++h) load(&maps.k, first + i + 1, y1, z1, 0, SA_KT, 2 * h, 2, SA_KT * 128);
+        auto load_k = [&](int t, int y, int z) { load(&maps.k, t, y, z, rank * (SA_KT / 2), SA_KT / 2, r.u.head * (HD / 64), HD / 64); };
+        auto load_v = [&](int t, int y, int z) { load(&maps.v, t, y, z, 0, SA_KT, r.u.head * (HD / 64) + rank * (HD / 128), HD / 128); };
+        for (bool more = work; more && alive; more = r.next(a)) {
+            if (!r.n) continue;
+            kv0 = !a.sq.pt && a.sq.kv0 ? a.sq.kv0[r.u.s] : 0;
+            int e = entry(r.t0), y0, z0, y1 = 0, z1 = 0;
+            if (nseg) alive = sa_wait_warp(q_empty, (unsigned) (nseg - 1) & 1u, spins, a.fault);   // the scores before are done
+            if (!alive) break;
+            if (um_elect()) {
+                const int tok0 = r.u.tok0 + rank * a.tok;
+                if (tok0 < r.u.len) {
+                    um_expect_tx(q_full, (unsigned) (a.tok * qpk * HD * 2));
+                    for (int b = 0; b < HD / 64; ++b) sa_tma3d(um_s32(Q) + b * (SA_ROWS * 128), &maps.q, b * 64, r.u.head * qpk, r.u.r0 + tok0, q_full);
+                } else {
+                    sa_arrive(q_full);   // no rows of this CTA's
+                }
             }
-            for (int h = 0; h < S::HALVES; ++h) load(&maps.v, first + i, y0, z0, h * S::VROWS, (h + 1) * S::VROWS, 0, HD / 64, S::VROWS * 128);
-            y0 = y1, z0 = z1;
+            __syncwarp();
+            ++nseg;
+            place(r.t0, e, y0, z0);
+            e = entry(r.t0 + 1);
+            load_k(r.t0, y0, z0);
+            for (int t = r.t0; t < r.t0 + r.n && alive; ++t) {
+                if (t + 1 < r.t0 + r.n) {
+                    place(t + 1, e, y1, z1);
+                    e = entry(t + 2);
+                    load_k(t + 1, y1, z1);
+                }
+                load_v(t, y0, z0);
+                y0 = y1, z0 = z1;
+            }
         }
-        // nothing is in flight when the block ends: the last load into every slot has landed (loads over another waited for its use)
-        if (n > 0 && lane == 0) um_wait(q_full, 0u, a.fault);
-        for (int k = max(0, c - S::SLOTS); k < c; ++k)
-            if (lane == 0) um_wait(&full[k % S::SLOTS], (unsigned) (k / S::SLOTS) & 1u, a.fault);
+        // nothing is in flight when the block ends: the last loads have landed (a load over another waited for that one's use)
+        if (lane == 0) {
+            spins = SA_SPINS;
+            if (nseg) sa_wait(q_full, (unsigned) (nseg - 1) & 1u, spins, a.fault);
+            for (int k = max(0, c - S::SLOTS); k < c; ++k) sa_wait(&full[k % S::SLOTS], (unsigned) (k / S::SLOTS) & 1u, spins, a.fault);
+        }
         __syncwarp();
-    } else if (warp == 1) {
-        // ---- the MMAs
-        int c = 0;   // slots used, in the order of their loads
-        const unsigned idesc_s = (1u << 4) | ((SA_KT >> 3) << 17) | ((128u >> 4) << 24);                // S: both operands K-major
-        const unsigned idesc_o = (1u << 4) | (1u << 16) | ((HD >> 3) << 17) | ((128u >> 4) << 24);   // O: B MN-major
+    } else if (warp == 2) {
+        // ---- what has landed here, told to the first CTA in the order of the loads; V rows past the newest position cleared first
+        int c = 0, nseg = 0;
+        bool alive = true;
+        SqRun r;
+        r.get(run_at);
+        auto landed = [&](int clear, int upto) {
+            const int slot = c % S::SLOTS;
+            alive = alive && sa_wait_warp(&full[slot], (unsigned) (c / S::SLOTS) & 1u, spins, a.fault);
+            if (!alive) return;
+            if (clear < upto) {
+                for (int x = clear; x < upto; ++x)
+                    for (int y = lane; y < HD / 16; y += 32)
+                        *reinterpret_cast<uint4*>(ring + slot * S::SLOT + ((x >> 6) * (HD / 128) + (y >> 3)) * 8192 + (x & 63) * 128 + (y & 7) * 16) =
+                            make_uint4(0u, 0u, 0u, 0u);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) sa_tell_shared(&ready[slot]);
+            } else if (lane == 0) {
+                sa_tell(&ready[slot]);
+            }
+            ++c;
+        };
+        for (bool more = work; more && alive; more = r.next(a)) {
+            if (!r.n) continue;
+            alive = sa_wait_warp(q_full, (unsigned) nseg & 1u, spins, a.fault);
+            if (!alive) break;
+            if (lane == 0) sa_tell(q_ready);
+            ++nseg;
+            landed(0, 0);
+            for (int t = r.t0; t < r.t0 + r.n && alive; ++t) {
+                if (t + 1 < r.t0 + r.n) landed(0, 0);
+                const int have = min(SA_KT, r.u.kv_len - t * SA_KT);
+                landed(have, (have + 15) / 16 * 16);   // of the last step of 16 positions
+            }
+        }
+    } else if (warp == 1 && rank == 0) {
+        // ---- the pair's MMAs, one lane's work from wait to commit
+        int c = 0, j = 0, nseg = 0;   // slots used in the order of their loads; tiles; segments
+        bool alive = true;            // the elected lane's
+        SqRun r;
+        r.get(run_at);
+        const unsigned idesc_s = (1u << 4) | ((SA_KT >> 3) << 17) | ((256u >> 4) << 24);             // S: both operands K-major
+        const unsigned idesc_o = (1u << 4) | (1u << 16) | ((HD >> 3) << 17) | ((256u >> 4) << 24);   // O: B MN-major
         auto wait = [&](unsigned long long* bar, unsigned parity) {
-            alive = alive && __all_sync(0xffffffffu, um_wait(bar, parity, a.fault));
+            alive = alive && sa_wait(bar, parity, spins, a.fault);
             sa_after();
         };
-        auto scores = [&]() {
-            const unsigned long long dq = um_desc(um_s32(Q));
+        // short loops: an MMA takes the tensor core 64 or 128 cycles, and a long body would have to be fetched again every time, the
+        // softmax warps' code having gone over it
+        auto scores = [&](bool last) {
+            const int slot = c % S::SLOTS;
+            if (um_elect()) {
+                wait(&ready[slot], (unsigned) (c / S::SLOTS) & 1u);
+                if (alive) {
+                    unsigned long long dq = um_desc(um_s32(Q)), dk = um_desc(um_s32(ring) + slot * S::SLOT);
 #pragma unroll 1
-            for (int h = 0; h < S::HALVES; ++h, ++c) {
-                const int slot = c % S::SLOTS;
-                wait(&full[slot], (unsigned) (c / S::SLOTS) & 1u);
-                if (!alive) return;
-                const unsigned long long dk = um_desc(um_s32(ring) + slot * SA_SLOT);
-                if (um_elect()) {
+                    for (int b = 0; b < HD / 64; ++b, dq += SA_ROWS * 128 >> 4, dk += 8192 >> 4)
 #pragma unroll
-                    for (int b = 0; b < 2; ++b)
-#pragma unroll
-                        for (int ks = 0; ks < 4; ++ks)
-                            um_mma(tm + S::COL_S, dq + (unsigned long long) (((2 * h + b) * (SA_ROWS * 128) + ks * 32) >> 4),
-                                   dk + (unsigned long long) ((b * (SA_KT * 128) + ks * 32) >> 4), idesc_s, (unsigned) (h | b | ks));
-                    um_commit(&empty[slot]);
-                    if (h == S::HALVES - 1) um_commit(s_full);
+                        for (int ks = 0; ks < 4; ++ks) sa_mma(tm + S::COL_S, dq + (ks * 32 >> 4), dk + (ks * 32 >> 4), idesc_s, (unsigned) (b | ks));
+                    sa_commit(&empty[slot]);
+                    sa_commit(s_full);
+                    if (last) sa_commit(q_empty);
                 }
-                __syncwarp();
             }
+            ++c;
+            __syncwarp();
         };
-        auto output = [&](int i) {
-            const int left = w.kv_len - (first + i) * SA_KT;   // positions of the tile that exist
+        auto output = [&](int t) {
+            const int slot = c % S::SLOTS, steps = (min(r.u.kv_len - t * SA_KT, SA_KT) + 15) / 16;   // of 16 positions that exist
+            if (um_elect()) {
+                wait(&ready[slot], (unsigned) (c / S::SLOTS) & 1u);
+                if (alive) {
+                    unsigned long long dv = um_desc_x(um_s32(ring) + slot * S::SLOT, 8192, 1024, 2);
+                    unsigned dp = tm + S::COL_P + (j & 1) * (SA_KT / 2), more = (unsigned) (t - r.t0);
+                    int ks = 0;
 #pragma unroll 1
-            for (int h = 0; h < S::HALVES; ++h, ++c) {
-                const int slot = c % S::SLOTS, have = min(left - h * S::VROWS, S::VROWS), steps = (have + 15) / 16;
-                wait(&full[slot], (unsigned) (c / S::SLOTS) & 1u);
-                if (!alive) return;
-                unsigned char* v = ring + slot * SA_SLOT;
-                if (have > 0 && have % 16) {   // rows of the last step past the newest position
-                    for (int r = have; r < 16 * steps; ++r)
-                        for (int x = lane; x < HD / 8; x += 32) *reinterpret_cast<uint4*>(v + (x >> 3) * (S::VROWS * 128) + r * 128 + (x & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    __syncwarp();
+                    for (; ks + 4 <= steps; ks += 4, dv += HD / 128 * 8192 >> 4, dp += 32, more = 1u)   // a group of 64 positions
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) sa_mma_ts(tm, dp + i * 8, dv + (i * 2048 >> 4), idesc_o, more | (unsigned) i);
+#pragma unroll 1
+                    for (; ks < steps; ++ks, dv += 2048 >> 4, dp += 8, more = 1u) sa_mma_ts(tm, dp, dv, idesc_o, more);
+                    sa_commit(&empty[slot]);
+                    sa_commit(&o_full[j & 1]);
                 }
-                const unsigned long long dv = um_desc_x(um_s32(v), S::VROWS * 128, 1024, 2);
-                if (um_elect()) {
-                    for (int ks = 0; ks < steps; ++ks)
-                        sa_mma_ts(tm, tm + S::COL_P + (i & 1) * (SA_KT / 2) + (h * S::VROWS + ks * 16) / 2, dv + (unsigned long long) (ks * 2048 >> 4), idesc_o,
-                                  (unsigned) (i | h | ks));
-                    um_commit(&empty[slot]);
-                    if (h == S::HALVES - 1) um_commit(&o_full[i & 1]);
-                }
-                __syncwarp();
             }
+            ++c;
+            __syncwarp();
         };
-        if (n > 0) {
-            wait(q_full, 0u);
-            if (alive) scores();
-        }
-        for (int i = 0; i < n && alive; ++i) {
-            if (i + 1 < n) {
-                wait(s_free, (unsigned) i & 1u);   // S(i) is in registers
-                if (alive) scores();
+        auto when = [&](unsigned long long* bar, unsigned parity) {   // the elected lane's wait
+            if (um_elect()) wait(bar, parity);
+            __syncwarp();
+        };
+        for (bool more = work; more; more = r.next(a)) {
+            if (!r.n) continue;
+            when(q_ready, (unsigned) nseg & 1u);
+            if (j) when(s_free, (unsigned) (j - 1) & 1u);
+            scores(r.n == 1);
+            for (int t = r.t0; t < r.t0 + r.n; ++t, ++j) {
+                if (t + 1 < r.t0 + r.n) {
+                    when(s_free, (unsigned) j & 1u);   // S(t) is in registers
+                    scores(t + 2 == r.t0 + r.n);
+                }
+                when(&p_full[j & 1], (unsigned) (j >> 1) & 1u);
+                if (t == r.t0 && nseg) when(o_free, (unsigned) (nseg - 1) & 1u);   // the rows before are out of O
+                output(t);
             }
-            if (alive) wait(&p_full[i & 1], (unsigned) (i >> 1) & 1u);
-            if (alive) output(i);
+            ++nseg;
         }
-        // nothing is under way when the block ends, also after a wait that ran out
-        if (um_elect()) um_commit(idle);
+        // nothing is under way when the blocks end, also after a wait that ran out
+        if (um_elect()) {
+            sa_commit(idle);
+            spins = SA_SPINS;
+            sa_wait(idle, 0u, spins, a.fault);
+        }
         __syncwarp();
-        um_wait(idle, 0u, a.fault);
-    } else if (warp >= 4) {
+    }
+    leave();
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         // ---- softmax: row m, columns 64 half .. + 63 of every tile
         const int half = (warp - 4) >> 2, m = (warp & 3) * 32 + lane, token = m / qpk, hh = m % qpk;
-        const bool real = token < w.ntok;
         const unsigned tl = tm + ((unsigned) ((warp & 3) * 32) << 16);
         const float scale = 1.44269504f / sqrtf((float) HD);
-        const int row = w.row + token;   // packed row
-        // positions this row sees: the causal count, or all, with a mask from pos0 on
-        const int lim = !real ? 0 : a.anc ? w.kv_len : min(w.kv_len, w.pos0 + w.tok0 + token + 1);
-        const int clear = a.anc ? w.pos0 : w.pos0 + w.tok0 + 1;   // positions below are seen by every row
-        const unsigned* anc = a.anc ? a.anc + (size_t) (real ? row : w.row) * a.words : nullptr;
-        float ref = -INFINITY, z = 0.f;   // this row's reference (in units of log2) and this half's sum
+        const int inv_qpk = (65536 + qpk - 1) / qpk;   // x / qpk = x inv_qpk >> 16 for x < 128
+        unsigned char* strip = strips + (warp - 4) * SA_STRIP;
+        int j = 0;   // tiles
+        SqRun r;
+        r.get(run_at);
         auto wait = [&](unsigned long long* bar, unsigned parity) {
-            alive = alive && __all_sync(0xffffffffu, um_wait(bar, parity, a.fault));
+            if (um_elect()) sa_wait(bar, parity, spins, a.fault);
+            __syncwarp();
             sa_after();
         };
+        for (bool more = work; more; more = r.next(a)) {
+            const SqUnit& u = r.u;
+            const int tok0 = u.tok0 + rank * a.tok, first_row = u.r0 + tok0;   // this CTA's
+            const bool real = token < a.tok && tok0 + token < u.len;
+            if (a.qg && !r.cut && real)   // the gate will be wanted
+                for (int i = half * (HD / 2); i < (half + 1) * (HD / 2); i += 32)
+                    l2_ask(a.qg + ((size_t) (first_row + token) * a.nq + u.head * qpk + hh) * 2 * HD + HD + i);
+            // positions this row sees: the causal count, or all, with a mask from pos0 on
+            const int lim = !real ? 0 : a.anc ? u.kv_len : min(u.kv_len, u.pos0 + tok0 + token + 1);
+            const int clear = min(u.kv_len, a.anc ? u.pos0 : u.pos0 + tok0 + 1);   // positions below are seen by every row
+            const unsigned* anc = a.anc ? a.anc + (size_t) (real ? first_row + token : u.r0) * a.words : nullptr;
+            float ref = -INFINITY, z = 0.f;   // this row's reference (in units of log2) and this half's sum
 #pragma unroll 1
-        for (int i = 0; i < n; ++i) {
-            if (alive) wait(s_full, (unsigned) i & 1u);
-            float x[64];
-            if (alive) {
+            for (int i = 0; i < r.n; ++i, ++j) {
+                wait(s_full, (unsigned) j & 1u);
+                float x[64];
                 sa_ld32(reinterpret_cast<unsigned*>(x), tl + S::COL_S + half * 64);
                 sa_ld32(reinterpret_cast<unsigned*>(x) + 32, tl + S::COL_S + half * 64 + 32);
                 sa_wait_ld();
-            }
-            sa_before();
-            __syncwarp();
-            if (lane == 0) sa_arrive(s_free);
-            const int p0 = (first + i) * SA_KT + half * 64;
-            if (p0 + 64 > min(clear, w.kv_len)) {
-                unsigned see0 = sq_first(lim - p0), see1 = sq_first(lim - p0 - 32);
-                if (a.anc) see0 &= sq_tree_bits(anc, a.words, p0 - w.pos0), see1 &= sq_tree_bits(anc, a.words, p0 + 32 - w.pos0);
+                sa_before();
+                __syncwarp();
+                if (lane == 0) sa_tell(s_free);
+                const int p0 = (r.t0 + i) * SA_KT + half * 64;
+                if (p0 + 64 > clear) {
+                    unsigned see0 = sq_first(lim - p0), see1 = sq_first(lim - p0 - 32);
+                    if (a.anc) see0 &= sq_tree_bits(anc, a.words, p0 - u.pos0), see1 &= sq_tree_bits(anc, a.words, p0 + 32 - u.pos0);
 #pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                    if (!(see0 >> j & 1u)) x[j] = -INFINITY;
-                    if (!(see1 >> j & 1u)) x[32 + j] = -INFINITY;
+                    for (int k = 0; k < 32; ++k) {
+                        if (!(see0 >> k & 1u)) x[k] = -INFINITY;
+                        if (!(see1 >> k & 1u)) x[32 + k] = -INFINITY;
+                    }
                 }
-            }
-            float mx = x[0];
+                float mq[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-            for (int j = 1; j < 64; ++j) mx = fmaxf(mx, x[j]);
-            xmax[half * SA_ROWS + m] = mx;
+                for (int k = 4; k < 64; ++k) mq[k & 3] = fmaxf(mq[k & 3], x[k]);
+                float mx = fmaxf(fmaxf(mq[0], mq[1]), fmaxf(mq[2], mq[3]));
+                float* xm = xmax + (j & 1) * 2 * SA_ROWS;
+                xm[half * SA_ROWS + m] = mx;
+                asm volatile("bar.sync 1, %0;" ::"n"(SA_SOFT) : "memory");
+                mx = fmaxf(mx, xm[(half ^ 1) * SA_ROWS + m]) * scale;
+                const bool up = mx > ref + 8.0f || (ref == -INFINITY && mx != -INFINITY);
+                if (__any_sync(0xffffffffu, up)) {
+                    const float f = !up ? 1.0f : ref == -INFINITY ? 0.f : ex2_ftz(ref - mx);
+                    if (up) ref = mx;
+                    z *= f;
+                    if (i > 0) {   // O row *= f, this half's columns
+                        wait(&o_full[(j - 1) & 1], (unsigned) ((j - 1) >> 1) & 1u);
+#pragma unroll 1
+                        for (int cb = 0; cb < HD / 2; cb += 32) {
+                            unsigned o[32];
+                            sa_ld32(o, tl + half * (HD / 2) + cb);
+                            sa_wait_ld();
+#pragma unroll
+                            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+                            sa_st32(tl + half * (HD / 2) + cb, o);
+                        }
+                    }
+                }
+                const float less = ref == -INFINITY ? 0.f : -ref;
+                unsigned pk[32];
+                float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+                for (int k = 0; k < 32; ++k) {
+                    float2 e = fma2(make_float2(x[2 * k], x[2 * k + 1]), make_float2(scale, scale), make_float2(less, less));
+                    e.x = ex2_ftz(e.x), e.y = ex2_ftz(e.y);
+                    sum = add2(sum, e);
+                    const __half2 h = __floats2half2_rn(e.x, e.y);
+                    pk[k] = *reinterpret_cast<const unsigned*>(&h);
+                }
+                z += sum.x + sum.y;
+                if (j > 1) wait(&o_full[j & 1], (unsigned) ((j >> 1) - 1) & 1u);   // the P tile's last reader is done
+                sa_st32(tl + S::COL_P + (j & 1) * (SA_KT / 2) + half * 32, pk);
+                sa_wait_st();
+                sa_before();
+                __syncwarp();
+                if (lane == 0) sa_tell(&p_full[j & 1]);
+            }
+            // ---- the rows' results: through the warp's strip, so that a line of 32 columns leaves (and its gates come) whole
+            float* xm = xmax + (j & 1) * 2 * SA_ROWS;   // the last tile's are in the other half
+            xm[half * SA_ROWS + m] = z;
             asm volatile("bar.sync 1, %0;" ::"n"(SA_SOFT) : "memory");
-            mx = fmaxf(mx, xmax[(half ^ 1) * SA_ROWS + m]) * scale;
-            asm volatile("bar.sync 2, %0;" ::"n"(SA_SOFT) : "memory");   // read before the next tile's are written
-            const bool up = mx > ref + 8.0f || (ref == -INFINITY && mx != -INFINITY);
-            const float f = !up ? 1.0f : ref == -INFINITY ? 0.f : ex2_ftz(ref - mx);
-            if (up) ref = mx;
-            z *= f;
-            if (i > 0 && __any_sync(0xffffffffu, up)) {   // O row *= f, this half's columns
-                if (alive) wait(&o_full[(i - 1) & 1], (unsigned) ((i - 1) >> 1) & 1u);
-                if (alive)
+            z += xm[(half ^ 1) * SA_ROWS + m];
+            asm volatile("bar.sync 1, %0;" ::"n"(SA_SOFT) : "memory");   // (a segment without tiles would write there again)
+            const float inv = r.cut ? 1.0f : z > 0.f ? 1.0f / z : 0.f;
+            const size_t slot = ((size_t) (2 * g + (r.first ? 0 : 1)) * 2 + rank) * SA_ROWS;   // of the parts, this CTA's first row
+            // lane l's part of row 4 k + l / 8 of this warp's: columns 4 (l % 8) .. + 3 of every 32
+            const int sub = lane >> 3, col = 4 * (lane & 7), rows = min(a.tok, u.len - tok0) * qpk - (warp & 3) * 32;   // rows of the warp that are real
+            auto place = [&](int k, int& t, int& h) {
+                const int mm = (warp & 3) * 32 + 4 * k + sub;
+                t = mm * inv_qpk >> 16, h = u.head * qpk + mm - t * qpk;
+                return 4 * k + sub < rows;
+            };
+            constexpr int CHUNKS = HD / 64;   // of 32 columns, this half's
+            float4 gate[8];
+            auto ask = [&](int ch) {
+                if (r.cut || !a.qg) return;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    int t, h;
+                    if (place(k, t, h))
+                        gate[k] = *reinterpret_cast<const float4*>(a.qg + ((size_t) (first_row + t) * a.nq + h) * 2 * HD + HD + half * (HD / 2) + ch * 32 + col);
+                }
+            };
+            if (r.n) wait(&o_full[(j - 1) & 1], (unsigned) ((j - 1) >> 1) & 1u);
 #pragma unroll 1
-                    for (int cb = 0; cb < HD / 2; cb += 32) {
-                        unsigned r[32];
-                        sa_ld32(r, tl + half * (HD / 2) + cb);
-                        sa_wait_ld();
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * f);
-                        sa_st32(tl + half * (HD / 2) + cb, r);
+            for (int ch = 0; ch < CHUNKS; ++ch) {
+                const int cb = half * (HD / 2) + ch * 32;
+                ask(ch);
+                unsigned o[32];
+                if (r.n) {
+                    sa_ld32(o, tl + cb);
+                    sa_wait_ld();
+                    if (ch == CHUNKS - 1) {   // O is in registers
+                        sa_before();
+                        __syncwarp();
+                        if (lane == 0) sa_tell(o_free);
                     }
-            }
-            const float base = ref == -INFINITY ? 0.f : ref;
-            unsigned pk[32];
-            float s0 = 0.f, s1 = 0.f;
+                }
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
-                const float p = ex2_ftz(fmaf(x[2 * j], scale, -base)), q = ex2_ftz(fmaf(x[2 * j + 1], scale, -base));
-                s0 += p, s1 += q;
-                const __half2 h = __floats2half2_rn(p, q);
-                pk[j] = *reinterpret_cast<const unsigned*>(&h);
-            }
-            z += s0 + s1;
-            if (i > 1 && alive) wait(&o_full[i & 1], (unsigned) ((i >> 1) - 1) & 1u);   // the P tile's last reader is done
-            if (alive) sa_st32(tl + S::COL_P + (i & 1) * (SA_KT / 2) + half * 32, pk);
-            sa_wait_st();
-            sa_before();
-            __syncwarp();
-            if (lane == 0) sa_arrive(&p_full[i & 1]);
-        }
-        // ---- the rows' results
-        xmax[half * SA_ROWS + m] = z;
-        asm volatile("bar.sync 1, %0;" ::"n"(SA_SOFT) : "memory");
-        z += xmax[(half ^ 1) * SA_ROWS + m];
-        if (n > 0 && alive) wait(&o_full[(n - 1) & 1], (unsigned) ((n - 1) >> 1) & 1u);
-        const float inv = z > 0.f ? 1.0f / z : 0.f;
-        const int head = w.head * qpk + hh;
-        const size_t cell = (size_t) row * a.nq + head, all = (size_t) a.sq.rows * a.nq;
-#pragma unroll 1
-        for (int cb = half * (HD / 2); cb < (half + 1) * (HD / 2); cb += 32) {
-            unsigned r[32];
+                for (int k = 0; k < 8; ++k) {
+                    float4 y = make_float4(__uint_as_float(o[4 * k]) * inv, __uint_as_float(o[4 * k + 1]) * inv, __uint_as_float(o[4 * k + 2]) * inv,
+                                           __uint_as_float(o[4 * k + 3]) * inv);
+                    if (!r.n || (!r.cut && !(z > 0.f))) y = make_float4(0.f, 0.f, 0.f, 0.f);
+                    *reinterpret_cast<float4*>(strip + lane * 128 + ((k ^ (lane & 7)) << 4)) = y;
+                }
+                __syncwarp();
 #pragma unroll
-            for (int j = 0; j < 32; ++j) r[j] = 0u;
-            if (n > 0 && alive) {
-                sa_ld32(r, tl + cb);
-                sa_wait_ld();
-            }
-            if (!real) continue;
-            if (a.nsplit > 1) {
-                float* o = a.part + ((size_t) blockIdx.y * all + cell) * HD + cb;
-#pragma unroll
-                for (int j = 0; j < 32; j += 4) *reinterpret_cast<uint4*>(o + j) = make_uint4(r[j], r[j + 1], r[j + 2], r[j + 3]);
-                continue;
-            }
-            uint16_t* o = a.out + (size_t) row * a.out_stride + (size_t) head * HD + cb;
-            const float* gate = a.qg ? a.qg + cell * 2 * HD + HD + cb : nullptr;
-#pragma unroll
-            for (int j = 0; j < 32; j += 8) {
-                float y[8];
-                unsigned u[4];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) y[e] = z > 0.f ? __uint_as_float(r[j + e]) * inv : 0.f;
-                if (gate)
-#pragma unroll
-                    for (int e = 0; e < 8; e += 4) {
-                        const float4 t = *reinterpret_cast<const float4*>(gate + j + e);
-                        y[e] = __fdividef(y[e], 1.0f + __expf(-t.x)), y[e + 1] = __fdividef(y[e + 1], 1.0f + __expf(-t.y));
-                        y[e + 2] = __fdividef(y[e + 2], 1.0f + __expf(-t.z)), y[e + 3] = __fdividef(y[e + 3], 1.0f + __expf(-t.w));
+                for (int k = 0; k < 8; ++k) {
+                    const int l = 4 * k + sub;
+                    float4 y = *reinterpret_cast<const float4*>(strip + l * 128 + (((lane & 7) ^ (l & 7)) << 4));
+                    int t, h;
+                    if (!place(k, t, h)) continue;
+                    if (r.cut) {
+                        *reinterpret_cast<float4*>(a.part + (slot + (warp & 3) * 32 + l) * HD + cb + col) = y;
+                        continue;
                     }
-#pragma unroll
-                for (int e = 0; e < 4; ++e) u[e] = (unsigned) f2h(y[2 * e]) | ((unsigned) f2h(y[2 * e + 1]) << 16);
-                *reinterpret_cast<uint4*>(o + j) = make_uint4(u[0], u[1], u[2], u[3]);
+                    if (a.qg) {
+                        const float4 q = gate[k];
+                        y.x = __fdividef(y.x, 1.0f + __expf(-q.x)), y.y = __fdividef(y.y, 1.0f + __expf(-q.y));
+                        y.z = __fdividef(y.z, 1.0f + __expf(-q.z)), y.w = __fdividef(y.w, 1.0f + __expf(-q.w));
+                    }
+                    *reinterpret_cast<uint2*>(a.out + (size_t) (first_row + t) * a.out_stride + (size_t) h * HD + cb + col) =
+                        make_uint2((unsigned) f2h(y.x) | ((unsigned) f2h(y.y) << 16), (unsigned) f2h(y.z) | ((unsigned) f2h(y.w) << 16));
+                }
+                __syncwarp();
             }
+            if (r.cut && real && half == 0)
+                *reinterpret_cast<float2*>(a.part + (size_t) 4 * a.pairs * SA_ROWS * HD + (slot + m) * 2) = make_float2(ref, z);
         }
-        if (a.nsplit > 1 && real && half == 0)
-            *reinterpret_cast<float2*>(a.part + (size_t) a.nsplit * all * HD + ((size_t) blockIdx.y * all + cell) * 2) = make_float2(ref, z);
+        leave();
     }
-    sa_before();
-    __syncthreads();
-    if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "r"(512));
 }
 
-// the splits' partials of row t, head h joined (a warp a head), gated and rounded
-template <int HD> __global__ void __launch_bounds__(128) k_attn_seqs_join(const __grid_constant__ SqAttn a) {
+// The parts of a unit that was cut, joined: block (boundary between pairs g and g + 1, eight rows), where that boundary is the
+// first inside its unit; a warp a row.
+template <int HD> __global__ void __launch_bounds__(256) k_attn_seqs_join(const __grid_constant__ SqAttn a) {
     constexpr int E = HD / 32;
-    const int t = blockIdx.x, h = blockIdx.y * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const int g = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = blockIdx.y / (SA_ROWS / 8), m = blockIdx.y % (SA_ROWS / 8) * 8 + warp;
     pdl_wait();
     pdl_go();
-    const int s = sq_find(a.sq.row0, a.sq.nseq, t);
-    if (s < 0 || h >= a.nq) return;
-    const int r0 = max(a.sq.row0[s], 0), len = min(a.sq.row0[s + 1], a.sq.rows) - r0, i0 = t - r0, pos0 = max(a.sq.pos0[s], 0);
-    const long long cap = a.sq.pt ? (long long) a.sq.pt_stride * a.g.rows : (long long) a.g.cap;
-    const int kv_len = (int) min((long long) pos0 + (a.anc ? len : min(len, (i0 / a.tok + 1) * a.tok)), cap);   // as the row's CTAs had it
-    const size_t all = (size_t) a.sq.rows * a.nq, cell = (size_t) t * a.nq + h;
-    const float* mz = a.part + (size_t) a.nsplit * all * HD;
-    float ref = -INFINITY, z = 0.f, o[E];
+    const SqPlan plan = sq_plan(a);
+    if (g + 1 >= plan.pairs) return;
+    const long long cut = plan.begin(g + 1);
+    long long at = cut;
+    const SqUnit u = sq_locate(a, at);
+    const int qpk = a.nq / a.nkv, tok0 = u.tok0 + rank * a.tok;
+    if (!sq_tile(at) || m >= min(a.tok, u.len - tok0) * qpk) return;   // no cut here; no such row
+    const long long begin = cut - at;
+    // the tile of the unit that the run of pair p begins with
+    auto tile = [&](int p) { return plan.begin(p) <= begin ? 0 : sq_tile(plan.begin(p) - begin); };
+    if (tile(g)) return;   // not the unit's first cut
+    int parts = 2;
+    while (g + parts < plan.pairs && plan.begin(g + parts) < begin + u.end + SA_COST) ++parts;
+    // pair g's part is its run's first where the run does not begin in a unit before; the later pairs' runs begin inside the unit
+    const size_t slot0 = 2 * g + (plan.begin(g) >= begin ? 0 : 1);
+    auto slot = [&](int p) { return ((p ? (size_t) 2 * (g + p) : slot0) * 2 + rank) * SA_ROWS + m; };
+    const float* mz = a.part + (size_t) 4 * a.pairs * SA_ROWS * HD;
+    float top = -INFINITY;
+    for (int p = lane; p < parts; p += 32) top = fmaxf(top, mz[slot(p) * 2]);
 #pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = 0.f;
-    for (int p = 0; p < a.nsplit; ++p) {
-        int first, n;
-        sq_range(kv_len, p, a.nsplit, first, n);
-        if (n <= 0) break;
-        const float2 x = *reinterpret_cast<const float2*>(mz + ((size_t) p * all + cell) * 2);
-        if (x.x == -INFINITY) continue;   // the row sees nothing there
-        const float rn = fmaxf(ref, x.x), f0 = ex2_ftz(ref - rn), f1 = ex2_ftz(x.x - rn);
-        z = z * f0 + x.y * f1;
-        ref = rn;
-        const float* src = a.part + ((size_t) p * all + cell) * HD + lane * E;
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    float z = 0.f, acc[E];
 #pragma unroll
-        for (int e = 0; e < E; e += 4) {
-            const float4 v = *reinterpret_cast<const float4*>(src + e);
-            o[e] = o[e] * f0 + v.x * f1, o[e + 1] = o[e + 1] * f0 + v.y * f1, o[e + 2] = o[e + 2] * f0 + v.z * f1, o[e + 3] = o[e + 3] * f0 + v.w * f1;
+    for (int e = 0; e < E; ++e) acc[e] = 0.f;
+    for (int p0 = 0; p0 < parts; p0 += 32) {
+        float w = 0.f;
+        if (p0 + lane < parts) {
+            const float2 x = *reinterpret_cast<const float2*>(mz + slot(p0 + lane) * 2);
+            w = x.x == -INFINITY ? 0.f : ex2_ftz(x.x - top);   // -inf: the row sees nothing there
+            z += w * x.y;
+        }
+        const int n = min(32, parts - p0);
+#pragma unroll 4
+        for (int p = 0; p < n; ++p) {
+            const float f = __shfl_sync(0xffffffffu, w, p);
+            const float* src = a.part + slot(p0 + p) * HD + lane * E;
+#pragma unroll
+            for (int e = 0; e < E; e += 4) {
+                const float4 v = *reinterpret_cast<const float4*>(src + e);
+                acc[e] = fmaf(v.x, f, acc[e]), acc[e + 1] = fmaf(v.y, f, acc[e + 1]), acc[e + 2] = fmaf(v.z, f, acc[e + 2]), acc[e + 3] = fmaf(v.w, f, acc[e + 3]);
+            }
         }
     }
-    const float inv = z > 0.f ? 1.0f / z : 0.f;
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        float y = o[e] * inv;
-        if (a.qg) y = __fdividef(y, 1.0f + __expf(-a.qg[cell * 2 * HD + HD + lane * E + e]));
-        a.out[(size_t) t * a.out_stride + (size_t) h * HD + lane * E + e] = f2h(y);
+    for (int o = 16; o; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
+    const float inv = z > 0.f ? 1.0f / z : 0.f;
+    const int row = u.r0 + tok0 + m / qpk, h = u.head * qpk + m % qpk;
+    const float* gate = a.qg ? a.qg + ((size_t) row * a.nq + h) * 2 * HD + HD + lane * E : nullptr;
+    uint16_t* out = a.out + (size_t) row * a.out_stride + (size_t) h * HD + lane * E;
+#pragma unroll
+    for (int e = 0; e < E; e += 4) {
+        float4 t = make_float4(0.f, 0.f, 0.f, 0.f), y = make_float4(acc[e] * inv, acc[e + 1] * inv, acc[e + 2] * inv, acc[e + 3] * inv);
+        if (gate) {
+            t = *reinterpret_cast<const float4*>(gate + e);
+            y.x = __fdividef(y.x, 1.0f + __expf(-t.x)), y.y = __fdividef(y.y, 1.0f + __expf(-t.y)), y.z = __fdividef(y.z, 1.0f + __expf(-t.z)),
+            y.w = __fdividef(y.w, 1.0f + __expf(-t.w));
+        }
+        *reinterpret_cast<uint2*>(out + e) = make_uint2((unsigned) f2h(y.x) | ((unsigned) f2h(y.y) << 16), (unsigned) f2h(y.z) | ((unsigned) f2h(y.w) << 16));
     }
 }
 
-// CTAs that share a unit's positions: as many as make the fewest rounds of the GPU's 148, a round's length taken as the longest
-// split's tiles and three more for a CTA's beginning and end
-static int sq_splits(long long units, long long positions) {
-    const long long tiles = (positions + SA_KT - 1) / SA_KT;
-    long long best = 0;
-    int ns = 1;
-    for (int s = 1; s <= 64 && s <= tiles; ++s) {
-        const long long per = (tiles + s - 1) / s;
-        if ((tiles + per - 1) / per != s) continue;   // the same longest split with fewer
-        const long long cost = (units * s + 147) / 148 * (per + 3) + (s > 1 ? 3 : 0);
-        if (s == 1 || cost < best) best = cost, ns = s;
-    }
-    return ns;
-}
 static long long sq_units(const FnxSeqs* sq, int tok, int nkv) {   // at most
-    const long long blocks = (long long) sq->rows / tok + sq->nseq;
+    const long long blocks = (long long) sq->rows / (2 * tok) + sq->nseq;
     return (blocks < sq->rows ? blocks : (long long) sq->rows) * nkv;
 }
-// what a split is decided by: the units at most, and the positions a sequence has at most - where the caller does not say, 64 a
-// page (the scratch is sized from the same struct, which does not know a page's rows), and one split without pages
-static int sq_plan(const FnxSeqs* sq, int nq, int nkv) {
-    const int tok = SA_ROWS / (nq / nkv);
-    return sq_splits(sq_units(sq, tok, nkv), sq->max_pos ? sq->max_pos : sq->pt ? (long long) sq->pt_stride * 64 : 0);
+static int sq_processors() {   // multiprocessors of the current device
+    static int n[64] = {};   // written without a lock: every writer stores the same value
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+    if (!n[dev] && cudaDeviceGetAttribute(&n[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) n[dev] = 148;
+    return n[dev];
 }
 
-template <int HD> static int sq_launch(const SqMaps& maps, const SqAttn& a, long long units, const char* what, cudaStream_t st) {
+template <int HD> static int sq_launch(const SqMaps& maps, const SqAttn& a, const char* what, cudaStream_t st) {
     if (cudaFuncSetAttribute(k_attn_seqs<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) SaShape<HD>::SMEM) != cudaSuccess)
         return fail("%s: shared memory opt-in: %s", what, cudaGetErrorString(cudaGetLastError()));
-    launch(0, k_attn_seqs<HD>, dim3((unsigned) units, a.nsplit), SA_THREADS, SaShape<HD>::SMEM, st, maps, a);
+    launch(0, k_attn_seqs<HD>, dim3(2 * a.pairs), SA_THREADS, SaShape<HD>::SMEM, st, maps, a);
     if (launch_ok(what)) return 1;
-    if (a.nsplit == 1) return 0;
-    launch(0, k_attn_seqs_join<HD>, dim3(a.sq.rows, (a.nq + 3) / 4), 128, 0, st, a);
+    if (a.pairs == 1) return 0;
+    launch(0, k_attn_seqs_join<HD>, dim3(a.pairs - 1, 2 * SA_ROWS / 8), 256, 0, st, a);
     return launch_ok(what);
 }
 
@@ -542,23 +840,24 @@ static int attn_seqs(const uint16_t* q16, int q_stride, const float* qg, const u
     FNX_REQUIRE(fault && enc, "%s: no fault word or no tensor-map encoder", what);
     SqMaps maps;
     memset(&maps, 0, sizeof(maps));
-    const cuuint32_t es[3] = {1, 1, 1};
+    const cuuint32_t es[4] = {1, 1, 1, 1};
+    // queries: dims, heads, rows.  The cache: 64 dims, rows of a page, column blocks, pages
     const cuuint64_t qd[3] = {(cuuint64_t) hd, (cuuint64_t) nq, (cuuint64_t) sq->rows}, qs[2] = {(cuuint64_t) hd * 2, (cuuint64_t) q_stride * 2};
     const cuuint32_t qb[3] = {64, (cuuint32_t) qpk, (cuuint32_t) tok};
     const cuuint64_t row = (cuuint64_t) nkv * hd, rows = sq->pt ? g.rows : g.cap;
-    const cuuint64_t kd[3] = {row, rows, (cuuint64_t) (sq->pt ? sq->npages : 1)}, ks[2] = {row * 2, sq->pt ? (cuuint64_t) g.page * 2 : rows * row * 2};
-    const cuuint32_t kb[3] = {64, (cuuint32_t) box, 1};
-    auto encode = [&](CUtensorMap* m, const void* p, const cuuint64_t* d, const cuuint64_t* s, const cuuint32_t* b) {
-        return enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void*>(p), d, s, b, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+    const cuuint64_t kd[4] = {64, rows, row / 64, (cuuint64_t) (sq->pt ? sq->npages : 1)}, ks[3] = {row * 2, 128, sq->pt ? (cuuint64_t) g.page * 2 : rows * row * 2};
+    const cuuint32_t kb[4] = {64, (cuuint32_t) box, (cuuint32_t) (box == 64 ? hd / 64 : 1), 1}, vb[4] = {64, (cuuint32_t) box, (cuuint32_t) (box == 64 ? hd / 128 : 1), 1};
+    auto encode = [&](CUtensorMap* m, int n, const void* p, const cuuint64_t* d, const cuuint64_t* s, const cuuint32_t* b) {
+        return enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT16, n, const_cast<void*>(p), d, s, b, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
     };
-    FNX_REQUIRE(encode(&maps.q, q16, qd, qs, qb) && encode(&maps.k, kc, kd, ks, kb) && encode(&maps.v, vc, kd, ks, kb),
+    FNX_REQUIRE(encode(&maps.q, 3, q16, qd, qs, qb) && encode(&maps.k, 4, kc, kd, ks, kb) && encode(&maps.v, 4, vc, kd, ks, vb),
                 "%s: no tensor map for %d rows %d apart or %d pages of %zu halves", what, sq->rows, q_stride, sq->npages, g.page);
-    const long long units = sq_units(sq, tok, nkv);
-    FNX_REQUIRE(units < (1ll << 31), "%s: %d rows of %d KV heads", what, sq->rows, nkv);
-    const int ns = sq_plan(sq, nq, nkv);
-    const SqAttn a{qg, g, *sq, anc, out, out_stride, nq, nkv, words, tok, box, ns, (float*) scratch, fault};
-    return hd == 256 ? sq_launch<256>(maps, a, units, what, strm(st)) : sq_launch<128>(maps, a, units, what, strm(st));
+    // no more pairs than there can be work for
+    const long long units = sq_units(sq, tok, nkv), most = sq->max_pos ? units * (sq->max_pos + SA_COST) : 1ll << 60;
+    const int pairs = (int) std::max(1ll, std::min((long long) sq_processors() / 2, (most + SA_LEAST - 1) / SA_LEAST));
+    const SqAttn a{qg, g, *sq, anc, out, out_stride, nq, nkv, words, tok, box, pairs, (float*) scratch, fault};
+    return hd == 256 ? sq_launch<256>(maps, a, what, strm(st)) : sq_launch<128>(maps, a, what, strm(st));
 }
 
 }  // namespace fnxk
@@ -568,9 +867,8 @@ using namespace fnxk;
 extern "C" {
 
 size_t fnx_attn_seqs_scratch_bytes(const FnxSeqs* sq, int nq, int nkv, int hd) {
-    if (!sq || nq < 1 || nkv < 1 || hd < 1 || nq % nkv || nq / nkv > 16 || sq->nseq < 1 || sq->rows < 1) return 0;
-    const int ns = sq_plan(sq, nq, nkv);
-    return ns == 1 ? 16 : (size_t) ns * sq->rows * nq * (hd + 2) * 4;
+    if (!sq || nq < 1 || nkv < 1 || hd < 1) return 0;
+    return (size_t) 4 * std::max(1, sq_processors() / 2) * SA_ROWS * (hd + 2) * 4;
 }
 
 int fnx_attn_prompt(const uint16_t* q16, int q_stride, const float* qg, const uint16_t* kc, const uint16_t* vc, FnxKvPages g, const FnxSeqs* sq,
