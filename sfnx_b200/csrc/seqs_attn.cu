@@ -16,15 +16,17 @@
 // warps 4 - 11 take the softmax step: a thread has one row and half of a tile's columns, the halves of a row agree on the
 // maximum through shared memory.
 //   tensor memory: O (HD columns), one S tile (128), two P tiles (64 columns each, f16 pairs).  S(i + 1) is issued when the softmax
-//   warps have S(i) in registers, so the tensor core computes it - and, when P(i) is written, O += P(i) V(i) - while they take
-//   exponentials: a tile costs the longer of the two, not the sum.  The next unit's copies and first scores run while the
-//   softmax warps write this one's rows.
-//   shared memory: Q, a ring of slots of half a tile each, asked for in the order of their use: K(0), K(1), V(0), K(2), V(1), ...,
-//   and a strip a softmax warp to turn rows into whole lines on their way out.
+//   warps have S(i) in registers, and O += P(i - 1) V(i - 1) behind it, so the tensor core has both to do while they take
+//   exponentials: a tile costs the longer of the two, not the sum.  (With O += P(i) V(i) issued as soon as P(i) is written, S(i + 1)
+//   came behind it and the softmax warps waited for it every other tile: 2500 and 3600 cycles a tile.)  The next unit's copies
+//   and first scores run while the softmax warps write this one's rows.
+//   shared memory: Q, a ring of slots of half a tile each, asked for in the order of their use: K(0), K(1), K(2), V(0), K(3),
+//   V(1), ..., and a strip a softmax warp to turn rows into whole lines on their way out.
 // Softmax: x = s log2 e / sqrt(hd); weights 2^(x - ref) against a reference that is raised - and O and the sums rescaled - only when
 // a row's maximum has grown by more than 8 over it, so weights stay below 2^8 and (O, ref, z) is an exact partial for any
 // reference.  z sums the weights in 32 bits before they are rounded to f16 for the product (2^-11 of a weight: the
-// result's own rounding is as large; f16 queries, keys and values enter exactly).
+// result's own rounding is as large; f16 queries, keys and values enter exactly).  A tile's 128 x 128 exponentials are 1024 cycles of
+// the special-function units; part of them is taken by a polynomial on the FMA units instead.
 // Positions past a unit's last visible one are not loaded beyond their box; V rows there are cleared in shared memory, since a
 // weight of zero times a stray NaN is a NaN.
 // Every wait on an mbarrier is bounded; on a timeout the fault word is set and the CTA ends with nothing in flight.
@@ -38,8 +40,15 @@
 
 namespace fnxk {
 
+#ifndef SA_COST_V
+#define SA_COST_V 640
+#endif
+#ifndef SA_POLY_V
+#define SA_POLY_V 12
+#endif
 constexpr int SA_ROWS = 128, SA_KT = 128, SA_THREADS = 384, SA_SOFT = 256, SA_STRIP = 4096;
-constexpr int SA_COST = 256;    // what a unit's beginning and end cost, in positions
+constexpr int SA_POLY = SA_POLY_V;     // of a thread's 32 pairs of exponentials a tile, those by polynomial
+constexpr int SA_COST = SA_COST_V;    // what a unit's beginning and end cost, in positions
 constexpr int SA_LEAST = 256;   // work a pair gets at least, in positions
 template <int HD> struct SaShape {
     static constexpr int QBYTES = SA_ROWS * HD * 2;
@@ -62,7 +71,9 @@ struct SqAttn {
     int tok;      // tokens of a CTA's rows: 128 / qpk
     int box;      // cache rows a copy brings: a power of two that divides a page's rows
     int pairs;    // the scan's pairs of CTAs
-    float* part;  // [2 pairs][2][128][HD] parts of units, then (ref, z) [2 pairs][2][128][2]
+    float4* part; // parts of units, as the threads hold them: [2 pairs][2][4 quarters of the rows][HD / 4][32 rows]
+    float2* mz;   // their (ref, z): [2 pairs][2][128]
+    int4* cuts;   // [pairs][2] what there is to join at the end of a pair's run
     unsigned* fault;
 };
 
@@ -166,16 +177,35 @@ struct SqPlan {
     int pairs;
     __device__ __forceinline__ long long begin(int g) const { return each * g + (unsigned) (total - each * pairs) * (unsigned) g / (unsigned) pairs; }
 };
-__device__ __forceinline__ SqPlan sq_plan(const SqAttn& a) {   // called by a converged warp
-    const int lane = threadIdx.x & 31;
-    long long w = 0;
-    for (int s = lane; s < a.sq.nseq; s += 32) {
-        int r0, len, pos0;
-        sq_seq(a, s, r0, len, pos0);
-        w += sq_work(a, len, pos0);
-    }
+// a lane's sequence of 32 neighbouring ones: its rows and the work up to and with it
+struct SqLane {
+    int r0, len, pos0;
+    long long mine, upto;
+    __device__ __forceinline__ void get(const SqAttn& a, int s) {   // called by a converged warp
+        r0 = len = pos0 = 0;
+        if (s < a.sq.nseq) sq_seq(a, s, r0, len, pos0);
+        mine = upto = sq_work(a, len, pos0);
+        if (a.sq.nseq == 1) {   // (lane 0's, all the same)
+            upto = sq_shfl(upto, 0);
+            return;
+        }
 #pragma unroll
-    for (int o = 16; o; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long y = __shfl_up_sync(0xffffffffu, upto, o);
+            if ((int) (threadIdx.x & 31) >= o) upto += y;
+        }
+    }
+};
+// called by a converged warp; `lanes`: the first 32 sequences
+__device__ __forceinline__ SqPlan sq_plan(const SqAttn& a, SqLane& lanes) {
+    const int lane = threadIdx.x & 31;
+    lanes.get(a, lane);
+    long long w = sq_shfl(lanes.upto, 31);
+    for (int s0 = 32; s0 < a.sq.nseq; s0 += 32) {
+        SqLane more;
+        more.get(a, s0 + lane);
+        w += sq_shfl(more.upto, 31);
+    }
     SqPlan p;
     p.total = w;
     p.pairs = (int) min((long long) a.pairs, w ? max(1ll, w / SA_LEAST) : 0ll);   // a run is never shorter than a tile
@@ -183,28 +213,21 @@ __device__ __forceinline__ SqPlan sq_plan(const SqAttn& a) {   // called by a co
     return p;
 }
 // the unit that work item `at` (below the plan's total) belongs to; `at` is left relative to the unit.  Called by a converged warp
-__device__ __forceinline__ SqUnit sq_locate(const SqAttn& a, long long& at) {
+__device__ __forceinline__ SqUnit sq_locate(const SqAttn& a, const SqLane& lanes, long long& at) {
     const int lane = threadIdx.x & 31;
     SqUnit u;
-    for (int s0 = 0;; s0 += 32) {   // the sequence
-        const int s = s0 + lane;
-        int r0 = 0, len = 0, pos0 = 0;
-        if (s < a.sq.nseq) sq_seq(a, s, r0, len, pos0);
-        const long long mine = sq_work(a, len, pos0);
-        long long w = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long y = __shfl_up_sync(0xffffffffu, w, o);
-            if (lane >= o) w += y;
-        }
-        const unsigned past = __ballot_sync(0xffffffffu, w > at);
+    SqLane x = lanes;
+    for (int s0 = 0;;) {   // the sequence
+        const unsigned past = __ballot_sync(0xffffffffu, x.upto > at);
         if (past || s0 + 32 >= a.sq.nseq) {
             const int l = past ? __ffs(past) - 1 : 0;
-            at -= sq_shfl(w - mine, l);
-            u.s = s0 + l, u.r0 = __shfl_sync(0xffffffffu, r0, l), u.len = __shfl_sync(0xffffffffu, len, l), u.pos0 = __shfl_sync(0xffffffffu, pos0, l);
+            at -= sq_shfl(x.upto - x.mine, l);
+            u.s = s0 + l, u.r0 = __shfl_sync(0xffffffffu, x.r0, l), u.len = __shfl_sync(0xffffffffu, x.len, l), u.pos0 = __shfl_sync(0xffffffffu, x.pos0, l);
             break;
         }
-        at -= sq_shfl(w, 31);
+        at -= sq_shfl(x.upto, 31);
+        s0 += 32;
+        x.get(a, s0 + lane);
     }
     int lo = 0, hi = (u.len + 2 * a.tok - 1) / (2 * a.tok);   // the block: the last that does not begin past `at`
     while (hi - lo > 1) {
@@ -275,6 +298,25 @@ __device__ __forceinline__ unsigned sq_tree_bits(const unsigned* anc, int words,
 }
 __device__ __forceinline__ unsigned sq_first(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
 
+// What there is to join where the run of pair g ends: the unit that is cut there, unless an earlier run's end has cut it before;
+// (parts, the first part's place, first packed row, tokens), (head, 0, 0, 0).  Called by a converged warp
+__device__ __forceinline__ void sq_cut(const SqAttn& a, const SqPlan& plan, const SqLane& lanes, int g, int4& x, int& head) {
+    x = make_int4(0, 0, 0, 0), head = 0;
+    if (g + 1 >= plan.pairs) return;
+    const long long cut = plan.begin(g + 1);
+    long long at = cut;
+    const SqUnit u = sq_locate(a, lanes, at);
+    const long long begin = cut - at;
+    // the tile of the unit that the run of pair p begins with
+    auto tile = [&](int p) { return plan.begin(p) <= begin ? 0 : sq_tile(plan.begin(p) - begin); };
+    if (!sq_tile(at) || tile(g)) return;
+    int parts = 2;
+    while (g + parts < plan.pairs && plan.begin(g + parts) < begin + u.end + SA_COST) ++parts;
+    // pair g's part is its run's first where the run does not begin in a unit before; the later pairs' runs begin inside the unit
+    x = make_int4(parts, 2 * g + (plan.begin(g) >= begin ? 0 : 1), u.r0 + u.tok0, min(u.len - u.tok0, 2 * a.tok));
+    head = u.head;
+}
+
 // Waits for a phase of `bar`, at most `spins` polls of up to 16 us (asleep: warps that poll without a break keep the barriers'
 // unit from the one that issues the MMAs); a wait that ran out is reported, and later ones of the thread do not linger
 constexpr int SA_SPINS = 1 << 16;
@@ -287,6 +329,37 @@ __device__ __forceinline__ bool sa_wait(unsigned long long* bar, unsigned parity
                      : "memory");
     if (!ok) spins = 1, atomicOr(fault, 8u);
     return ok != 0;
+}
+// whether the phase is over
+__device__ __forceinline__ bool sa_test(unsigned long long* bar, unsigned parity) {
+    unsigned ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(ok)
+                 : "r"(um_s32(bar)), "r"(parity)
+                 : "memory");
+    return ok != 0;
+}
+// 2^x of two values on the FMA units: x = n + f, n the nearest integer (by adding and taking away 1.5 2^23, whose low bits then hold
+// n), a polynomial of degree 5 for 2^f on [-1/2, 1/2] (fitted to the relative error: 2.4e-7 with its roundings in 32 bits),
+// n added to the exponent.  Below -126: 2^-126 or so instead of zero, which f16 rounds to zero and no sum notices
+__device__ __forceinline__ float2 sa_ex2_poly(float2 x) {
+    const float magic = 12582912.f;
+    x.x = fmaxf(x.x, -126.f), x.y = fmaxf(x.y, -126.f);
+    const float2 t = add2(x, make_float2(magic, magic)), n = add2(t, make_float2(-magic, -magic));
+    const float2 f = fma2(n, make_float2(-1.f, -1.f), x);
+    float2 p = fma2(f, make_float2(1.3276456157e-3f, 1.3276456157e-3f), make_float2(9.6755409613e-3f, 9.6755409613e-3f));
+    p = fma2(p, f, make_float2(5.5507134646e-2f, 5.5507134646e-2f));
+    p = fma2(p, f, make_float2(2.4022120237e-1f, 2.4022120237e-1f));
+    p = fma2(p, f, make_float2(6.9314694405e-1f, 6.9314694405e-1f));
+    p = fma2(p, f, make_float2(1.0000001192f, 1.0000001192f));
+    return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)), __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
+}
+// a pair of gated values: y / (1 + e^-g), one reciprocal for both (the gates cut at -40, where no f16 value has anything left)
+__device__ __forceinline__ void sa_gate(float& y0, float& y1, float g0, float g1) {
+    const float a = 1.0f + ex2_ftz(-1.44269504f * (g0 < -40.f ? -40.f : g0)), b = 1.0f + ex2_ftz(-1.44269504f * (g1 < -40.f ? -40.f : g1));
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(a * b));
+    y0 *= r * b, y1 *= r * a;
 }
 // the same by one lane for its warp (all lanes get the answer)
 __device__ __forceinline__ bool sa_wait_warp(unsigned long long* bar, unsigned parity, int& spins, unsigned* fault) {
@@ -306,8 +379,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(SA_THREADS, 1) k_att
     // memory.  empty, q_empty, s_full, o_full: MMAs are done, told to both
     unsigned long long *full = bars, *empty = full + S::SLOTS, *ready = empty + S::SLOTS, *q_full = ready + S::SLOTS, *q_ready = q_full + 1, *q_empty = q_full + 2,
                        *s_full = q_full + 3, *s_free = q_full + 4, *o_free = q_full + 5, *idle = q_full + 6, *p_full = q_full + 7, *o_full = q_full + 9;
-    volatile int* run_at = reinterpret_cast<int*>(q_full + 12);
     volatile unsigned *tmem_at = reinterpret_cast<unsigned*>(q_full + 11), *work_at = tmem_at + 1;
+    volatile int* run_at = reinterpret_cast<int*>(q_full + 12);
     const int tid = threadIdx.x, warp = (int) um_uniform(tid >> 5), lane = tid & 31, rank = blockIdx.x & 1, g = blockIdx.x >> 1;
     if (tid == 0) {
         for (int i = 0; i < S::SLOTS; ++i) sa_init(&full[i], 1), sa_init(&empty[i], 1), sa_init(&ready[i], 2);
@@ -325,34 +398,43 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(SA_THREADS, 1) k_att
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(um_s32((const void*) tmem_at)), "r"(512));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
     }
-    pdl_wait();
-    pdl_go();
-    if (warp == 3) {   // the pair's run of work
-        const SqPlan plan = sq_plan(a);
-        const bool any = g < plan.pairs;
-        SqRun r = {};
-        bool some = false;
-        if (any) {
-            const long long lo = plan.begin(g);
-            long long at = lo;
-            r.u = sq_locate(a, at);
-            r.left = plan.begin(g + 1) - lo + at;
-            r.first = 1;
-            some = r.measure(sq_tile(at));
-            if (!some) r.left = 0;
-        }
-        if (lane == 0) {
-            r.put(run_at);
-            *work_at = some;
-        }
-    }
     sa_before();
     sa_cluster();   // barriers and tensor memory of both CTAs are there
     sa_after();
     const unsigned tm = um_uniform(*tmem_at);
     const int qpk = a.nq / a.nkv;
     int spins = SA_SPINS;
-    const bool work = um_uniform(*work_at) != 0;
+    pdl_wait();   // all of the above while the kernel before still runs
+    pdl_go();
+    if (warp == 3) {   // the pair's run of work, and what there is to join at its end
+        SqLane lanes;
+        const SqPlan plan = sq_plan(a, lanes);
+        SqRun r = {};
+        bool some = g < plan.pairs;
+        if (some) {
+            const long long lo = plan.begin(g);
+            long long at = lo;
+            r.u = sq_locate(a, lanes, at);
+            r.left = plan.begin(g + 1) - lo + at;
+            r.first = 1;
+            some = r.measure(sq_tile(at));
+        }
+        if (lane == 0) {
+            r.put(run_at);
+            *work_at = some;
+        }
+        __syncwarp();
+        asm volatile("bar.arrive 2, %0;" ::"n"(SA_THREADS) : "memory");   // the others go on while the record is made
+        if (rank == 0) {
+            int4 x;
+            int head;
+            sq_cut(a, plan, lanes, g, x, head);
+            if (lane == 0) a.cuts[2 * g] = x, a.cuts[2 * g + 1] = make_int4(head, 0, 0, 0);
+        }
+    } else {
+        asm volatile("bar.sync 2, %0;" ::"n"(SA_THREADS) : "memory");
+    }
+    const bool work = warp != 3 && um_uniform(*work_at) != 0;
     auto leave = [&]() {
         sa_before();
         asm volatile("bar.sync 0, %0;" ::"n"(SA_THREADS) : "memory");
@@ -364,12 +446,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(SA_THREADS, 1) k_att
     if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (warp == 0) {
-        // ---- copies.  Load number c of the ring takes slot c % SLOTS; tile i's K load comes before tile i - 1's V load.  A slot
+        // ---- copies.  Load number c of the ring takes slot c % SLOTS; tile i's K load comes before tile i - 2's V load.  A slot
         // holds groups of 64 rows, each as column blocks of 64 dims (8 KB, swizzled)
         int c = 0, nseg = 0, kv0 = 0;
-        bool alive = true;
         SqRun r;
         r.get(run_at);
+        bool alive = true;
         // lane j looks after box j of a tile: the table's entry, asked for a tile ahead, and with it where the box lies
         auto entry = [&](int tile) {
             const int p = tile * SA_KT + lane * a.box;
@@ -412,7 +494,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(SA_THREADS, 1) k_att
         for (bool more = work; more && alive; more = r.next(a)) {
             if (!r.n) continue;
             kv0 = !a.sq.pt && a.sq.kv0 ? a.sq.kv0[r.u.s] : 0;
-            int e = entry(r.t0), y0, z0, y1 = 0, z1 = 0;
+            const int end = r.t0 + r.n;
+            int e = entry(r.t0), y0, z0, y1 = 0, z1 = 0, y2 = 0, z2 = 0;
             if (nseg) alive = sa_wait_warp(q_empty, (unsigned) (nseg - 1) & 1u, spins, a.fault);   // the scores before are done
             if (!alive) break;
             if (um_elect()) {
@@ -429,14 +512,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(SA_THREADS, 1) k_att
             place(r.t0, e, y0, z0);
             e = entry(r.t0 + 1);
             load_k(r.t0, y0, z0);
-            for (int t = r.t0; t < r.t0 + r.n && alive; ++t) {
-                if (t + 1 < r.t0 + r.n) {
-                    place(t + 1, e, y1, z1);
-                    e = entry(t + 2);
-                    load_k(t + 1, y1, z1);
+            if (r.n > 1) {
+                place(r.t0 + 1, e, y1, z1);
+                e = entry(r.t0 + 2);
+                load_k(r.t0 + 1, y1, z1);
+            }
+            for (int t = r.t0; t < end && alive; ++t) {
+                if (t + 2 < end) {
+                    place(t + 2, e, y2, z2);
+                    e = entry(t + 3);
+                    load_k(t + 2, y2, z2);
                 }
                 load_v(t, y0, z0);
-                y0 = y1, z0 = z1;
+                y0 = y1, z0 = z1, y1 = y2, z1 = z2;
             }
         }
         // nothing is in flight when the block ends: the last loads have landed (a load over another waited for that one's use)
@@ -449,9 +537,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(SA_THREADS, 1) k_att
     } else if (warp == 2) {
         // ---- what has landed here, told to the first CTA in the order of the loads; V rows past the newest position cleared first
         int c = 0, nseg = 0;
-        bool alive = true;
         SqRun r;
         r.get(run_at);
+        bool alive = true;
         auto landed = [&](int clear, int upto) {
             const int slot = c % S::SLOTS;
             alive = alive && sa_wait_warp(&full[slot], (unsigned) (c / S::SLOTS) & 1u, spins, a.fault);
@@ -476,15 +564,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(SA_THREADS, 1) k_att
             if (lane == 0) sa_tell(q_ready);
             ++nseg;
             landed(0, 0);
+            if (r.n > 1) landed(0, 0);
             for (int t = r.t0; t < r.t0 + r.n && alive; ++t) {
-                if (t + 1 < r.t0 + r.n) landed(0, 0);
+                if (t + 2 < r.t0 + r.n) landed(0, 0);
                 const int have = min(SA_KT, r.u.kv_len - t * SA_KT);
                 landed(have, (have + 15) / 16 * 16);   // of the last step of 16 positions
             }
         }
     } else if (warp == 1 && rank == 0) {
         // ---- the pair's MMAs, one lane's work from wait to commit
-        int c = 0, j = 0, nseg = 0;   // slots used in the order of their loads; tiles; segments
+        int c = 0, j = 0, nseg = 0;   // slots used in the order of their loads (the elected lane's); tiles; segments
         bool alive = true;            // the elected lane's
         SqRun r;
         r.get(run_at);
@@ -496,62 +585,59 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(SA_THREADS, 1) k_att
         };
         // short loops: an MMA takes the tensor core 64 or 128 cycles, and a long body would have to be fetched again every time, the
         // softmax warps' code having gone over it
-        auto scores = [&](bool last) {
+        auto scores = [&](bool last) {   // (the elected lane)
             const int slot = c % S::SLOTS;
-            if (um_elect()) {
-                wait(&ready[slot], (unsigned) (c / S::SLOTS) & 1u);
-                if (alive) {
-                    unsigned long long dq = um_desc(um_s32(Q)), dk = um_desc(um_s32(ring) + slot * S::SLOT);
-#pragma unroll 1
-                    for (int b = 0; b < HD / 64; ++b, dq += SA_ROWS * 128 >> 4, dk += 8192 >> 4)
-#pragma unroll
-                        for (int ks = 0; ks < 4; ++ks) sa_mma(tm + S::COL_S, dq + (ks * 32 >> 4), dk + (ks * 32 >> 4), idesc_s, (unsigned) (b | ks));
-                    sa_commit(&empty[slot]);
-                    sa_commit(s_full);
-                    if (last) sa_commit(q_empty);
-                }
-            }
+            wait(&ready[slot], (unsigned) (c / S::SLOTS) & 1u);
             ++c;
-            __syncwarp();
+            if (!alive) return;
+            unsigned long long dq = um_desc(um_s32(Q)), dk = um_desc(um_s32(ring) + slot * S::SLOT);
+#pragma unroll 1
+            for (int b = 0; b < HD / 64; ++b, dq += SA_ROWS * 128 >> 4, dk += 8192 >> 4)
+#pragma unroll
+                for (int ks = 0; ks < 4; ++ks) sa_mma(tm + S::COL_S, dq + (ks * 32 >> 4), dk + (ks * 32 >> 4), idesc_s, (unsigned) (b | ks));
+            sa_commit(&empty[slot]);
+            sa_commit(s_full);
+            if (last) sa_commit(q_empty);
         };
         auto output = [&](int t) {
             const int slot = c % S::SLOTS, steps = (min(r.u.kv_len - t * SA_KT, SA_KT) + 15) / 16;   // of 16 positions that exist
-            if (um_elect()) {
-                wait(&ready[slot], (unsigned) (c / S::SLOTS) & 1u);
-                if (alive) {
-                    unsigned long long dv = um_desc_x(um_s32(ring) + slot * S::SLOT, 8192, 1024, 2);
-                    unsigned dp = tm + S::COL_P + (j & 1) * (SA_KT / 2), more = (unsigned) (t - r.t0);
-                    int ks = 0;
-#pragma unroll 1
-                    for (; ks + 4 <= steps; ks += 4, dv += HD / 128 * 8192 >> 4, dp += 32, more = 1u)   // a group of 64 positions
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) sa_mma_ts(tm, dp + i * 8, dv + (i * 2048 >> 4), idesc_o, more | (unsigned) i);
-#pragma unroll 1
-                    for (; ks < steps; ++ks, dv += 2048 >> 4, dp += 8, more = 1u) sa_mma_ts(tm, dp, dv, idesc_o, more);
-                    sa_commit(&empty[slot]);
-                    sa_commit(&o_full[j & 1]);
-                }
-            }
+            wait(&ready[slot], (unsigned) (c / S::SLOTS) & 1u);
             ++c;
-            __syncwarp();
-        };
-        auto when = [&](unsigned long long* bar, unsigned parity) {   // the elected lane's wait
-            if (um_elect()) wait(bar, parity);
-            __syncwarp();
+            if (!alive) return;
+            unsigned long long dv = um_desc_x(um_s32(ring) + slot * S::SLOT, 8192, 1024, 2);
+            unsigned dp = tm + S::COL_P + (j & 1) * (SA_KT / 2), more = (unsigned) (t - r.t0);
+            int ks = 0;
+#pragma unroll 1
+            for (; ks + 4 <= steps; ks += 4, dv += HD / 128 * 8192 >> 4, dp += 32, more = 1u)   // a group of 64 positions
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sa_mma_ts(tm, dp + i * 8, dv + (i * 2048 >> 4), idesc_o, more | (unsigned) i);
+#pragma unroll 1
+            for (; ks < steps; ++ks, dv += 2048 >> 4, dp += 8, more = 1u) sa_mma_ts(tm, dp, dv, idesc_o, more);
+            sa_commit(&empty[slot]);
+            sa_commit(&o_full[j & 1]);
         };
         for (bool more = work; more; more = r.next(a)) {
             if (!r.n) continue;
-            when(q_ready, (unsigned) nseg & 1u);
-            if (j) when(s_free, (unsigned) (j - 1) & 1u);
-            scores(r.n == 1);
-            for (int t = r.t0; t < r.t0 + r.n; ++t, ++j) {
-                if (t + 1 < r.t0 + r.n) {
-                    when(s_free, (unsigned) j & 1u);   // S(t) is in registers
-                    scores(t + 2 == r.t0 + r.n);
+            const int end = r.t0 + r.n;
+            if (um_elect()) {
+                wait(q_ready, (unsigned) nseg & 1u);
+                if (j) wait(s_free, (unsigned) (j - 1) & 1u);
+                scores(r.n == 1);
+                if (r.n > 1) {
+                    wait(s_free, (unsigned) j & 1u);   // the first tile's scores are in registers
+                    scores(r.n == 2);
                 }
-                when(&p_full[j & 1], (unsigned) (j >> 1) & 1u);
-                if (t == r.t0 && nseg) when(o_free, (unsigned) (nseg - 1) & 1u);   // the rows before are out of O
-                output(t);
+            }
+            __syncwarp();
+            for (int t = r.t0; t < end; ++t, ++j) {
+                if (um_elect()) {
+                    if (t + 2 < end) wait(s_free, (unsigned) (j + 1) & 1u);   // S(t + 1) is in registers, and so P(t) is written
+                    wait(&p_full[j & 1], (unsigned) (j >> 1) & 1u);
+                    if (t + 2 < end) scores(t + 3 == end);
+                    if (t == r.t0 && nseg) wait(o_free, (unsigned) (nseg - 1) & 1u);   // the rows before are out of O
+                    output(t);
+                }
+                __syncwarp();
             }
             ++nseg;
         }
@@ -639,18 +725,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(SA_THREADS, 1) k_att
                     }
                 }
                 const float less = ref == -INFINITY ? 0.f : -ref;
+                const bool p_free = j < 2 || sa_test(&o_full[j & 1], (unsigned) ((j >> 1) - 1) & 1u);   // the P tile's last reader is done
                 unsigned pk[32];
                 float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
                 for (int k = 0; k < 32; ++k) {
                     float2 e = fma2(make_float2(x[2 * k], x[2 * k + 1]), make_float2(scale, scale), make_float2(less, less));
-                    e.x = ex2_ftz(e.x), e.y = ex2_ftz(e.y);
+                    if (k * SA_POLY / 32 != (k + 1) * SA_POLY / 32) e = sa_ex2_poly(e);
+                    else e.x = ex2_ftz(e.x), e.y = ex2_ftz(e.y);
                     sum = add2(sum, e);
                     const __half2 h = __floats2half2_rn(e.x, e.y);
                     pk[k] = *reinterpret_cast<const unsigned*>(&h);
                 }
                 z += sum.x + sum.y;
-                if (j > 1) wait(&o_full[j & 1], (unsigned) ((j >> 1) - 1) & 1u);   // the P tile's last reader is done
+                if (!__all_sync(0xffffffffu, p_free)) wait(&o_full[j & 1], (unsigned) ((j >> 1) - 1) & 1u);
+                else sa_after();
                 sa_st32(tl + S::COL_P + (j & 1) * (SA_KT / 2) + half * 32, pk);
                 sa_wait_st();
                 sa_before();
@@ -663,141 +752,133 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(SA_THREADS, 1) k_att
             asm volatile("bar.sync 1, %0;" ::"n"(SA_SOFT) : "memory");
             z += xm[(half ^ 1) * SA_ROWS + m];
             asm volatile("bar.sync 1, %0;" ::"n"(SA_SOFT) : "memory");   // (a segment without tiles would write there again)
-            const float inv = r.cut ? 1.0f : z > 0.f ? 1.0f / z : 0.f;
-            const size_t slot = ((size_t) (2 * g + (r.first ? 0 : 1)) * 2 + rank) * SA_ROWS;   // of the parts, this CTA's first row
-            // lane l's part of row 4 k + l / 8 of this warp's: columns 4 (l % 8) .. + 3 of every 32
-            const int sub = lane >> 3, col = 4 * (lane & 7), rows = min(a.tok, u.len - tok0) * qpk - (warp & 3) * 32;   // rows of the warp that are real
-            auto place = [&](int k, int& t, int& h) {
-                const int mm = (warp & 3) * 32 + 4 * k + sub;
-                t = mm * inv_qpk >> 16, h = u.head * qpk + mm - t * qpk;
-                return 4 * k + sub < rows;
-            };
-            constexpr int CHUNKS = HD / 64;   // of 32 columns, this half's
-            float4 gate[8];
-            auto ask = [&](int ch) {
-                if (r.cut || !a.qg) return;
+            const bool none = ref == -INFINITY;   // the row saw nothing
+            const float inv = none ? 0.f : 1.0f / z;
+            const size_t slot = (size_t) (2 * g + (r.first ? 0 : 1)) * 2 + rank;   // of the parts
+            float4* part = a.part + ((slot * 4 + (warp & 3)) * (HD / 4) + half * (HD / 8)) * 32 + lane;
+            if (r.cut && real && half == 0) a.mz[slot * SA_ROWS + m] = make_float2(ref, z);
+            // lane l's part of row 4 k + l / 8 of this warp's: columns 4 (l % 8) .. + 3 of every 32; where those rows lie
+            const int sub = lane >> 3, col = half * (HD / 2) + 4 * (lane & 7), rows = min(a.tok, u.len - tok0) * qpk - (warp & 3) * 32;   // rows of the warp that are real
+            uint16_t* out = a.out + (size_t) first_row * a.out_stride + (size_t) u.head * qpk * HD + col;
+            const float* gates = a.qg + ((size_t) first_row * a.nq + u.head * qpk) * 2 * HD + HD + col;
+            int out_at[8], gate_at[8];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    int t, h;
-                    if (place(k, t, h))
-                        gate[k] = *reinterpret_cast<const float4*>(a.qg + ((size_t) (first_row + t) * a.nq + h) * 2 * HD + HD + half * (HD / 2) + ch * 32 + col);
-                }
+            for (int k = 0; k < 8; ++k) {
+                const int mm = (warp & 3) * 32 + 4 * k + sub, t = mm * inv_qpk >> 16, h = mm - t * qpk;
+                out_at[k] = 4 * k + sub < rows ? t * a.out_stride + h * HD : -1, gate_at[k] = (t * a.nq + h) * 2 * HD;
+            }
+            constexpr int STRIPS = HD / 64;   // of 32 columns, this half's
+            float4 gate[8];
+            const bool gated = !r.cut && a.qg;
+            auto ask = [&](int k, int st) {   // a strip ahead
+                if (gated && st < STRIPS && out_at[k] >= 0) gate[k] = *reinterpret_cast<const float4*>(gates + gate_at[k] + st * 32);
             };
+#pragma unroll
+            for (int k = 0; k < 8; ++k) ask(k, 0);
             if (r.n) wait(&o_full[(j - 1) & 1], (unsigned) ((j - 1) >> 1) & 1u);
 #pragma unroll 1
-            for (int ch = 0; ch < CHUNKS; ++ch) {
-                const int cb = half * (HD / 2) + ch * 32;
-                ask(ch);
+            for (int st = 0; st < STRIPS; ++st) {
                 unsigned o[32];
                 if (r.n) {
-                    sa_ld32(o, tl + cb);
+                    sa_ld32(o, tl + half * (HD / 2) + st * 32);
                     sa_wait_ld();
-                    if (ch == CHUNKS - 1) {   // O is in registers
+                    if (st == STRIPS - 1) {   // O is in registers
                         sa_before();
                         __syncwarp();
                         if (lane == 0) sa_tell(o_free);
                     }
                 }
+                if (__any_sync(0xffffffffu, none || !r.n))   // rows that saw nothing
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    float4 y = make_float4(__uint_as_float(o[4 * k]) * inv, __uint_as_float(o[4 * k + 1]) * inv, __uint_as_float(o[4 * k + 2]) * inv,
-                                           __uint_as_float(o[4 * k + 3]) * inv);
-                    if (!r.n || (!r.cut && !(z > 0.f))) y = make_float4(0.f, 0.f, 0.f, 0.f);
-                    *reinterpret_cast<float4*>(strip + lane * 128 + ((k ^ (lane & 7)) << 4)) = y;
+                    for (int k = 0; k < 32; ++k) o[k] = none || !r.n ? 0u : o[k];
+                if (r.cut) {
+                    if (real)
+#pragma unroll
+                        for (int k = 0; k < 8; ++k)
+                            part[(st * 8 + k) * 32] =
+                                make_float4(__uint_as_float(o[4 * k]), __uint_as_float(o[4 * k + 1]), __uint_as_float(o[4 * k + 2]), __uint_as_float(o[4 * k + 3]));
+                    continue;
                 }
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    *reinterpret_cast<float4*>(strip + lane * 128 + ((k ^ (lane & 7)) << 4)) =
+                        make_float4(__uint_as_float(o[4 * k]) * inv, __uint_as_float(o[4 * k + 1]) * inv, __uint_as_float(o[4 * k + 2]) * inv,
+                                    __uint_as_float(o[4 * k + 3]) * inv);
                 __syncwarp();
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
                     const int l = 4 * k + sub;
                     float4 y = *reinterpret_cast<const float4*>(strip + l * 128 + (((lane & 7) ^ (l & 7)) << 4));
-                    int t, h;
-                    if (!place(k, t, h)) continue;
-                    if (r.cut) {
-                        *reinterpret_cast<float4*>(a.part + (slot + (warp & 3) * 32 + l) * HD + cb + col) = y;
-                        continue;
-                    }
-                    if (a.qg) {
-                        const float4 q = gate[k];
-                        y.x = __fdividef(y.x, 1.0f + __expf(-q.x)), y.y = __fdividef(y.y, 1.0f + __expf(-q.y));
-                        y.z = __fdividef(y.z, 1.0f + __expf(-q.z)), y.w = __fdividef(y.w, 1.0f + __expf(-q.w));
-                    }
-                    *reinterpret_cast<uint2*>(a.out + (size_t) (first_row + t) * a.out_stride + (size_t) h * HD + cb + col) =
-                        make_uint2((unsigned) f2h(y.x) | ((unsigned) f2h(y.y) << 16), (unsigned) f2h(y.z) | ((unsigned) f2h(y.w) << 16));
+                    if (gated) sa_gate(y.x, y.y, gate[k].x, gate[k].y), sa_gate(y.z, y.w, gate[k].z, gate[k].w);
+                    ask(k, st + 1);
+                    if (out_at[k] >= 0)
+                        *reinterpret_cast<uint2*>(out + out_at[k] + st * 32) =
+                            make_uint2((unsigned) f2h(y.x) | ((unsigned) f2h(y.y) << 16), (unsigned) f2h(y.z) | ((unsigned) f2h(y.w) << 16));
                 }
                 __syncwarp();
             }
-            if (r.cut && real && half == 0)
-                *reinterpret_cast<float2*>(a.part + (size_t) 4 * a.pairs * SA_ROWS * HD + (slot + m) * 2) = make_float2(ref, z);
         }
         leave();
     }
 }
 
-// The parts of a unit that was cut, joined: block (boundary between pairs g and g + 1, eight rows), where that boundary is the
-// first inside its unit; a warp a row.
+// The parts of units that were cut, joined: where a pair's run ends, a block takes 32 rows of the unit that it cut, a warp eight of
+// their columns at a time, a lane a row, as the parts lie; eight parts' loads are in flight together.
+constexpr int SJ_PARTS = 8;
 template <int HD> __global__ void __launch_bounds__(256) k_attn_seqs_join(const __grid_constant__ SqAttn a) {
-    constexpr int E = HD / 32;
-    const int g = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = blockIdx.y / (SA_ROWS / 8), m = blockIdx.y % (SA_ROWS / 8) * 8 + warp;
+    const int g = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rank = blockIdx.y >> 2, quarter = blockIdx.y & 3;   // CTA of the pair, quarter of its rows
     pdl_wait();
     pdl_go();
-    const SqPlan plan = sq_plan(a);
-    if (g + 1 >= plan.pairs) return;
-    const long long cut = plan.begin(g + 1);
-    long long at = cut;
-    const SqUnit u = sq_locate(a, at);
-    const int qpk = a.nq / a.nkv, tok0 = u.tok0 + rank * a.tok;
-    if (!sq_tile(at) || m >= min(a.tok, u.len - tok0) * qpk) return;   // no cut here; no such row
-    const long long begin = cut - at;
-    // the tile of the unit that the run of pair p begins with
-    auto tile = [&](int p) { return plan.begin(p) <= begin ? 0 : sq_tile(plan.begin(p) - begin); };
-    if (tile(g)) return;   // not the unit's first cut
-    int parts = 2;
-    while (g + parts < plan.pairs && plan.begin(g + parts) < begin + u.end + SA_COST) ++parts;
-    // pair g's part is its run's first where the run does not begin in a unit before; the later pairs' runs begin inside the unit
-    const size_t slot0 = 2 * g + (plan.begin(g) >= begin ? 0 : 1);
-    auto slot = [&](int p) { return ((p ? (size_t) 2 * (g + p) : slot0) * 2 + rank) * SA_ROWS + m; };
-    const float* mz = a.part + (size_t) 4 * a.pairs * SA_ROWS * HD;
-    float top = -INFINITY;
-    for (int p = lane; p < parts; p += 32) top = fmaxf(top, mz[slot(p) * 2]);
+    const int4 x = a.cuts[2 * g];
+    const int qpk = a.nq / a.nkv, m = quarter * 32 + lane, rows = min(a.tok, x.w - rank * a.tok) * qpk, n = x.x;
+    if (!n || m >= rows) return;
+    const int head = a.cuts[2 * g + 1].x * qpk + m % qpk;
+    const size_t row = (size_t) x.z + rank * a.tok + m / qpk;
+    auto slot = [&](int p) { return ((size_t) (p ? 2 * (g + p) : x.y)) * 2 + rank; };
+#pragma unroll 1
+    for (int c = warp + 8 * blockIdx.z; c < HD / 8; c += 8 * gridDim.z) {
+        const float* gate = a.qg ? a.qg + (row * a.nq + head) * 2 * HD + HD + c * 8 : nullptr;
+        float4 t0 = make_float4(0.f, 0.f, 0.f, 0.f), t1 = t0;
+        if (gate) t0 = *reinterpret_cast<const float4*>(gate), t1 = *reinterpret_cast<const float4*>(gate + 4);
+        float top = -INFINITY, z = 0.f, acc[8];
 #pragma unroll
-    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    float z = 0.f, acc[E];
+        for (int k = 0; k < 8; ++k) acc[k] = 0.f;
+#pragma unroll 1
+        for (int p0 = 0; p0 < n; p0 += SJ_PARTS) {
+            float2 q[SJ_PARTS];
+            float4 v[SJ_PARTS][2];
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = 0.f;
-    for (int p0 = 0; p0 < parts; p0 += 32) {
-        float w = 0.f;
-        if (p0 + lane < parts) {
-            const float2 x = *reinterpret_cast<const float2*>(mz + slot(p0 + lane) * 2);
-            w = x.x == -INFINITY ? 0.f : ex2_ftz(x.x - top);   // -inf: the row sees nothing there
-            z += w * x.y;
-        }
-        const int n = min(32, parts - p0);
-#pragma unroll 4
-        for (int p = 0; p < n; ++p) {
-            const float f = __shfl_sync(0xffffffffu, w, p);
-            const float* src = a.part + slot(p0 + p) * HD + lane * E;
+            for (int i = 0; i < SJ_PARTS; ++i) {
+                q[i] = make_float2(-INFINITY, 0.f), v[i][0] = v[i][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (p0 + i >= n) continue;
+                q[i] = a.mz[slot(p0 + i) * SA_ROWS + m];
+                const float4* src = a.part + ((slot(p0 + i) * 4 + quarter) * (HD / 4) + c * 2) * 32 + lane;
+                v[i][0] = src[0], v[i][1] = src[32];
+            }
+            float most = top;
 #pragma unroll
-            for (int e = 0; e < E; e += 4) {
-                const float4 v = *reinterpret_cast<const float4*>(src + e);
-                acc[e] = fmaf(v.x, f, acc[e]), acc[e + 1] = fmaf(v.y, f, acc[e + 1]), acc[e + 2] = fmaf(v.z, f, acc[e + 2]), acc[e + 3] = fmaf(v.w, f, acc[e + 3]);
+            for (int i = 0; i < SJ_PARTS; ++i) most = fmaxf(most, q[i].x);
+            if (most == -INFINITY) continue;   // the row sees nothing there
+            const float f0 = top == -INFINITY ? 0.f : ex2_ftz(top - most);
+            top = most, z *= f0;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) acc[k] *= f0;
+#pragma unroll
+            for (int i = 0; i < SJ_PARTS; ++i) {
+                const float f = q[i].x == -INFINITY ? 0.f : ex2_ftz(q[i].x - top);
+                z = fmaf(f, q[i].y, z);
+                acc[0] = fmaf(f, v[i][0].x, acc[0]), acc[1] = fmaf(f, v[i][0].y, acc[1]), acc[2] = fmaf(f, v[i][0].z, acc[2]), acc[3] = fmaf(f, v[i][0].w, acc[3]);
+                acc[4] = fmaf(f, v[i][1].x, acc[4]), acc[5] = fmaf(f, v[i][1].y, acc[5]), acc[6] = fmaf(f, v[i][1].z, acc[6]), acc[7] = fmaf(f, v[i][1].w, acc[7]);
             }
         }
-    }
+        const float inv = z > 0.f ? 1.0f / z : 0.f;
 #pragma unroll
-    for (int o = 16; o; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
-    const float inv = z > 0.f ? 1.0f / z : 0.f;
-    const int row = u.r0 + tok0 + m / qpk, h = u.head * qpk + m % qpk;
-    const float* gate = a.qg ? a.qg + ((size_t) row * a.nq + h) * 2 * HD + HD + lane * E : nullptr;
-    uint16_t* out = a.out + (size_t) row * a.out_stride + (size_t) h * HD + lane * E;
+        for (int k = 0; k < 8; ++k) acc[k] *= inv;
+        if (gate) sa_gate(acc[0], acc[1], t0.x, t0.y), sa_gate(acc[2], acc[3], t0.z, t0.w), sa_gate(acc[4], acc[5], t1.x, t1.y), sa_gate(acc[6], acc[7], t1.z, t1.w);
+        unsigned u[4];
 #pragma unroll
-    for (int e = 0; e < E; e += 4) {
-        float4 t = make_float4(0.f, 0.f, 0.f, 0.f), y = make_float4(acc[e] * inv, acc[e + 1] * inv, acc[e + 2] * inv, acc[e + 3] * inv);
-        if (gate) {
-            t = *reinterpret_cast<const float4*>(gate + e);
-            y.x = __fdividef(y.x, 1.0f + __expf(-t.x)), y.y = __fdividef(y.y, 1.0f + __expf(-t.y)), y.z = __fdividef(y.z, 1.0f + __expf(-t.z)),
-            y.w = __fdividef(y.w, 1.0f + __expf(-t.w));
-        }
-        *reinterpret_cast<uint2*>(out + e) = make_uint2((unsigned) f2h(y.x) | ((unsigned) f2h(y.y) << 16), (unsigned) f2h(y.z) | ((unsigned) f2h(y.w) << 16));
+        for (int e = 0; e < 4; ++e) u[e] = (unsigned) f2h(acc[2 * e]) | ((unsigned) f2h(acc[2 * e + 1]) << 16);
+        *reinterpret_cast<uint4*>(a.out + row * a.out_stride + (size_t) head * HD + c * 8) = make_uint4(u[0], u[1], u[2], u[3]);
     }
 }
 
@@ -819,7 +900,7 @@ template <int HD> static int sq_launch(const SqMaps& maps, const SqAttn& a, cons
     launch(0, k_attn_seqs<HD>, dim3(2 * a.pairs), SA_THREADS, SaShape<HD>::SMEM, st, maps, a);
     if (launch_ok(what)) return 1;
     if (a.pairs == 1) return 0;
-    launch(0, k_attn_seqs_join<HD>, dim3(a.pairs - 1, 2 * SA_ROWS / 8), 256, 0, st, a);
+    launch(0, k_attn_seqs_join<HD>, dim3(a.pairs - 1, 8, HD / 128), 256, 0, st, a);
     return launch_ok(what);
 }
 
@@ -856,7 +937,9 @@ static int attn_seqs(const uint16_t* q16, int q_stride, const float* qg, const u
     // no more pairs than there can be work for
     const long long units = sq_units(sq, tok, nkv), most = sq->max_pos ? units * (sq->max_pos + SA_COST) : 1ll << 60;
     const int pairs = (int) std::max(1ll, std::min((long long) sq_processors() / 2, (most + SA_LEAST - 1) / SA_LEAST));
-    const SqAttn a{qg, g, *sq, anc, out, out_stride, nq, nkv, words, tok, box, pairs, (float*) scratch, fault};
+    float4* part = (float4*) scratch;
+    float2* mz = reinterpret_cast<float2*>(part + (size_t) 4 * pairs * SA_ROWS * (hd / 4));
+    const SqAttn a{qg, g, *sq, anc, out, out_stride, nq, nkv, words, tok, box, pairs, part, mz, reinterpret_cast<int4*>(mz + (size_t) 4 * pairs * SA_ROWS), fault};
     return hd == 256 ? sq_launch<256>(maps, a, what, strm(st)) : sq_launch<128>(maps, a, what, strm(st));
 }
 
@@ -868,7 +951,8 @@ extern "C" {
 
 size_t fnx_attn_seqs_scratch_bytes(const FnxSeqs* sq, int nq, int nkv, int hd) {
     if (!sq || nq < 1 || nkv < 1 || hd < 1) return 0;
-    return (size_t) 4 * std::max(1, sq_processors() / 2) * SA_ROWS * (hd + 2) * 4;
+    const size_t pairs = (size_t) std::max(1, sq_processors() / 2);
+    return pairs * (4 * SA_ROWS * (hd + 2) * 4 + 2 * sizeof(int4));
 }
 
 int fnx_attn_prompt(const uint16_t* q16, int q_stride, const float* qg, const uint16_t* kc, const uint16_t* vc, FnxKvPages g, const FnxSeqs* sq,
