@@ -706,7 +706,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(SA_THREADS, 1) k_att
                 xm[half * SA_ROWS + m] = mx;
                 asm volatile("bar.sync 1, %0;" ::"n"(SA_SOFT) : "memory");
                 mx = fmaxf(mx, xm[(half ^ 1) * SA_ROWS + m]) * scale;
-                const bool up = mx > ref + 8.0f || (ref == -INFINITY && mx != -INFINITY);
+                const bool up = real && (mx > ref + 8.0f || (ref == -INFINITY && mx != -INFINITY));   // (other rows hold what was there before)
                 if (__any_sync(0xffffffffu, up)) {
                     const float f = !up ? 1.0f : ref == -INFINITY ? 0.f : ex2_ftz(ref - mx);
                     if (up) ref = mx;
@@ -823,63 +823,63 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(SA_THREADS, 1) k_att
 }
 
 // The parts of units that were cut, joined: where a pair's run ends, a block takes 32 rows of the unit that it cut, a warp eight of
-// their columns at a time, a lane a row, as the parts lie; eight parts' loads are in flight together.
-constexpr int SJ_PARTS = 8;
-template <int HD> __global__ void __launch_bounds__(256) k_attn_seqs_join(const __grid_constant__ SqAttn a) {
+// their columns, a lane a row, as the parts lie; four parts' loads are in flight together.
+constexpr int SJ_PARTS = 4;
+template <int HD> __global__ void __launch_bounds__(256, 3) k_attn_seqs_join(const __grid_constant__ SqAttn a) {
     const int g = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rank = blockIdx.y >> 2, quarter = blockIdx.y & 3;   // CTA of the pair, quarter of its rows
     pdl_wait();
     pdl_go();
     const int4 x = a.cuts[2 * g];
     const int qpk = a.nq / a.nkv, m = quarter * 32 + lane, rows = min(a.tok, x.w - rank * a.tok) * qpk, n = x.x;
     if (!n || m >= rows) return;
-    const int head = a.cuts[2 * g + 1].x * qpk + m % qpk;
+    const int head = a.cuts[2 * g + 1].x * qpk + m % qpk, c = warp + 8 * blockIdx.z;   // c: which eight columns
     const size_t row = (size_t) x.z + rank * a.tok + m / qpk;
-    auto slot = [&](int p) { return ((size_t) (p ? 2 * (g + p) : x.y)) * 2 + rank; };
+    const float* gate = a.qg ? a.qg + (row * a.nq + head) * 2 * HD + HD + c * 8 : nullptr;
+    if (gate) l2_ask(gate);
+    auto slot = [&](int p) { return (p ? 2 * (g + p) : x.y) * 2 + rank; };
+    const float4* part = a.part + (quarter * (HD / 4) + c * 2) * 32 + lane;
+    float top = -INFINITY, z = 0.f, acc[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) acc[k] = 0.f;
 #pragma unroll 1
-    for (int c = warp + 8 * blockIdx.z; c < HD / 8; c += 8 * gridDim.z) {
-        const float* gate = a.qg ? a.qg + (row * a.nq + head) * 2 * HD + HD + c * 8 : nullptr;
-        float4 t0 = make_float4(0.f, 0.f, 0.f, 0.f), t1 = t0;
-        if (gate) t0 = *reinterpret_cast<const float4*>(gate), t1 = *reinterpret_cast<const float4*>(gate + 4);
-        float top = -INFINITY, z = 0.f, acc[8];
+    for (int p0 = 0; p0 < n; p0 += SJ_PARTS) {
+        float2 q[SJ_PARTS];
+        float4 v[SJ_PARTS][2];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) acc[k] = 0.f;
-#pragma unroll 1
-        for (int p0 = 0; p0 < n; p0 += SJ_PARTS) {
-            float2 q[SJ_PARTS];
-            float4 v[SJ_PARTS][2];
-#pragma unroll
-            for (int i = 0; i < SJ_PARTS; ++i) {
-                q[i] = make_float2(-INFINITY, 0.f), v[i][0] = v[i][1] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (p0 + i >= n) continue;
-                q[i] = a.mz[slot(p0 + i) * SA_ROWS + m];
-                const float4* src = a.part + ((slot(p0 + i) * 4 + quarter) * (HD / 4) + c * 2) * 32 + lane;
-                v[i][0] = src[0], v[i][1] = src[32];
-            }
-            float most = top;
-#pragma unroll
-            for (int i = 0; i < SJ_PARTS; ++i) most = fmaxf(most, q[i].x);
-            if (most == -INFINITY) continue;   // the row sees nothing there
-            const float f0 = top == -INFINITY ? 0.f : ex2_ftz(top - most);
-            top = most, z *= f0;
-#pragma unroll
-            for (int k = 0; k < 8; ++k) acc[k] *= f0;
-#pragma unroll
-            for (int i = 0; i < SJ_PARTS; ++i) {
-                const float f = q[i].x == -INFINITY ? 0.f : ex2_ftz(q[i].x - top);
-                z = fmaf(f, q[i].y, z);
-                acc[0] = fmaf(f, v[i][0].x, acc[0]), acc[1] = fmaf(f, v[i][0].y, acc[1]), acc[2] = fmaf(f, v[i][0].z, acc[2]), acc[3] = fmaf(f, v[i][0].w, acc[3]);
-                acc[4] = fmaf(f, v[i][1].x, acc[4]), acc[5] = fmaf(f, v[i][1].y, acc[5]), acc[6] = fmaf(f, v[i][1].z, acc[6]), acc[7] = fmaf(f, v[i][1].w, acc[7]);
-            }
+        for (int i = 0; i < SJ_PARTS; ++i) {
+            q[i] = make_float2(-INFINITY, 0.f), v[i][0] = v[i][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (p0 + i >= n) continue;
+            const int at = slot(p0 + i);
+            q[i] = a.mz[at * SA_ROWS + m];
+            v[i][0] = part[at * (SA_ROWS * HD / 4)], v[i][1] = part[at * (SA_ROWS * HD / 4) + 32];
         }
-        const float inv = z > 0.f ? 1.0f / z : 0.f;
+        float most = top;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) acc[k] *= inv;
-        if (gate) sa_gate(acc[0], acc[1], t0.x, t0.y), sa_gate(acc[2], acc[3], t0.z, t0.w), sa_gate(acc[4], acc[5], t1.x, t1.y), sa_gate(acc[6], acc[7], t1.z, t1.w);
-        unsigned u[4];
+        for (int i = 0; i < SJ_PARTS; ++i) most = fmaxf(most, q[i].x);
+        if (most == -INFINITY) continue;   // the row sees nothing there
+        const float f0 = top == -INFINITY ? 0.f : ex2_ftz(top - most);
+        top = most, z *= f0;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) u[e] = (unsigned) f2h(acc[2 * e]) | ((unsigned) f2h(acc[2 * e + 1]) << 16);
-        *reinterpret_cast<uint4*>(a.out + row * a.out_stride + (size_t) head * HD + c * 8) = make_uint4(u[0], u[1], u[2], u[3]);
+        for (int k = 0; k < 8; ++k) acc[k] *= f0;
+#pragma unroll
+        for (int i = 0; i < SJ_PARTS; ++i) {
+            const float f = q[i].x == -INFINITY ? 0.f : ex2_ftz(q[i].x - top);
+            z = fmaf(f, q[i].y, z);
+            acc[0] = fmaf(f, v[i][0].x, acc[0]), acc[1] = fmaf(f, v[i][0].y, acc[1]), acc[2] = fmaf(f, v[i][0].z, acc[2]), acc[3] = fmaf(f, v[i][0].w, acc[3]);
+            acc[4] = fmaf(f, v[i][1].x, acc[4]), acc[5] = fmaf(f, v[i][1].y, acc[5]), acc[6] = fmaf(f, v[i][1].z, acc[6]), acc[7] = fmaf(f, v[i][1].w, acc[7]);
+        }
     }
+    const float inv = z > 0.f ? 1.0f / z : 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) acc[k] *= inv;
+    if (gate) {
+        const float4 t0 = *reinterpret_cast<const float4*>(gate), t1 = *reinterpret_cast<const float4*>(gate + 4);
+        sa_gate(acc[0], acc[1], t0.x, t0.y), sa_gate(acc[2], acc[3], t0.z, t0.w), sa_gate(acc[4], acc[5], t1.x, t1.y), sa_gate(acc[6], acc[7], t1.z, t1.w);
+    }
+    unsigned u[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) u[e] = (unsigned) f2h(acc[2 * e]) | ((unsigned) f2h(acc[2 * e + 1]) << 16);
+    *reinterpret_cast<uint4*>(a.out + row * a.out_stride + (size_t) head * HD + c * 8) = make_uint4(u[0], u[1], u[2], u[3]);
 }
 
 static long long sq_units(const FnxSeqs* sq, int tok, int nkv) {   // at most
@@ -900,7 +900,7 @@ template <int HD> static int sq_launch(const SqMaps& maps, const SqAttn& a, cons
     launch(0, k_attn_seqs<HD>, dim3(2 * a.pairs), SA_THREADS, SaShape<HD>::SMEM, st, maps, a);
     if (launch_ok(what)) return 1;
     if (a.pairs == 1) return 0;
-    launch(0, k_attn_seqs_join<HD>, dim3(a.pairs - 1, 8, HD / 128), 256, 0, st, a);
+    launch(0, k_attn_seqs_join<HD>, dim3(a.pairs - 1, 8, HD / 64), 256, 0, st, a);
     return launch_ok(what);
 }
 
