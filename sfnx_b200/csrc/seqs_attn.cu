@@ -40,15 +40,13 @@
 
 namespace fnxk {
 
-#ifndef SA_COST_V
-#define SA_COST_V 640
-#endif
-#ifndef SA_POLY_V
-#define SA_POLY_V 12
-#endif
 constexpr int SA_ROWS = 128, SA_KT = 128, SA_THREADS = 384, SA_SOFT = 256, SA_STRIP = 4096;
-constexpr int SA_POLY = SA_POLY_V;     // of a thread's 32 pairs of exponentials a tile, those by polynomial
-constexpr int SA_COST = SA_COST_V;    // what a unit's beginning and end cost, in positions
+// Of a thread's 32 pairs of exponentials a tile, those by polynomial: 1000 rows after 31 000 positions 612 us with 0, 594 with 8, 612 with
+// 12, 620 with 16
+constexpr int SA_POLY = 8;
+// What a unit's beginning and end cost, in positions (the dealing of the work): a prompt of 8192 tokens, whose first units are short,
+// 782 us with 512, 655 with 768, 649 with 1024; the packed short prompts 37.5, 35.3, 40.8
+constexpr int SA_COST = 768;
 constexpr int SA_LEAST = 256;   // work a pair gets at least, in positions
 template <int HD> struct SaShape {
     static constexpr int QBYTES = SA_ROWS * HD * 2;
