@@ -1,10 +1,11 @@
 // Log probabilities of given tokens, the entropy of their distribution and the likeliest alternatives, in one pass over the
 // logits (no counterpart in the reference, which returns tokens only).
 //
-// With a reference r, z = sum e^(x - r) and s = sum (x - r) e^(x - r):  lse = r + log z,  H = log z - s / z, and a token's log
-// probability is x - lse.  The reference is raised - z' = f z, s' = f (s + (r - r') z), f = e^(r - r') - only when a value exceeds
-// it by more than 8, so a thread rescales once or twice a row and e^(x - r) stays below e^8.  The centred s keeps H free of the
-// cancellation that sum p x - lse has for large logits.  A NaN or +inf makes z a NaN, which is how the row is found out.
+// With t = x log2 e - R for a reference R, z = sum 2^t and s = sum t 2^t:  lse = (R + log2 z) ln 2,  H = (log2 z - s / z) ln 2, and a
+// token's log probability is x - lse (R is a 32-bit number and nothing is rounded between it and the sums, so R ln 2 is taken
+// in double).  The reference is raised - z' = f z, s' = f (s + (R - R') z), f = 2^(R - R') - only when a value exceeds it by more
+// than 8, so a thread rescales once or twice a row and 2^t stays below 2^8.  The centred s keeps H free of the cancellation
+// that sum p x - lse has for large logits.  A NaN or +inf makes z a NaN, which is how the row is found out.
 // The k best: a bound that k values of the row's first batch reach or exceed (the k-th largest or so of the threads'
 // maxima, found by bisection), and of the rest of the row every warp lists what exceeds it, about k / 4096 of the values,
 // without a word to the other warps.  A list that is full (rising logits) is cut to its own k best, which raises that
@@ -12,15 +13,20 @@
 // larger ones.  Entries are 64-bit composites (the value's order-preserving key, the index's complement), no two equal, so ties go
 // to the lower index whatever order they come in.
 // A row goes to one block when there are many, else to as many as the GPU holds at once; the row's last block joins the parts.
+// A pass is bound by DRAM when there are many rows: a thread copies its own values into shared memory three batches ahead
+// (cp.async; nobody else reads them, so no barrier belongs to it), 96 KB in flight a multiprocessor; with one batch ahead in
+// registers 2000 rows took 342 us.  A value costs about seven instructions, most of them two values at a time.
 #include <algorithm>
 
 #include "common.cuh"
 #include "exact_math.cuh"
+#include "moe_internal.cuh"
 
 namespace fnxk {
 
 constexpr int LP_THREADS = 512, LP_WARPS = LP_THREADS / 32, LP_PER = 8, LP_BATCH = LP_THREADS * LP_PER, LP_LIST = 256;
 constexpr int LP_CAP = LP_WARPS * LP_LIST;   // entries of all lists
+constexpr int LP_STAGES = 4;            // batches in the ring
 constexpr int LP_BLOCKS = 2 * 148;   // blocks the GPU holds at once; rows that go to several blocks are fewer
 
 struct LpPart {   // a block's part of a row
@@ -50,8 +56,8 @@ __device__ __forceinline__ void lp_join(float& r, float& z, float& s, float r2, 
         z += z2, s += s2;
         return;
     }
-    const float d1 = fmaxf(r - rn, -200.f), d2 = fmaxf(r2 - rn, -200.f);   // e^-200 is zero: a part of nothing (-inf) drops out
-    const float f1 = __expf(d1), f2 = __expf(d2);
+    const float d1 = fmaxf(r - rn, -200.f), d2 = fmaxf(r2 - rn, -200.f);   // 2^-200 is zero: a part of nothing (-inf) drops out
+    const float f1 = ex2_ftz(d1), f2 = ex2_ftz(d2);
     s = f1 * (s + d1 * z) + f2 * (s2 + d2 * z2);
     z = f1 * z + f2 * z2;
     r = rn;
@@ -101,8 +107,25 @@ struct LpShared {
     float lse;
 };
 
-// the bound that at least k of the threads' maxima reach (0: fewer than k have any)
+// A bound that at least k of the threads' maxima reach (0: where fewer than k have any, or warps in the first case).  Few: the k-th largest of the
+// warps' maxima; else bisection over the threads' by one warp
 __device__ __forceinline__ unsigned long long lp_block_bound(LpShared& sh, unsigned long long mine, int k) {
+    const int lane = threadIdx.x & 31;
+    if (k <= LP_WARPS) {
+#pragma unroll
+        for (int o = 16; o; o >>= 1) {
+            const unsigned long long x = __shfl_xor_sync(0xffffffffu, mine, o);
+            mine = x > mine ? x : mine;
+        }
+        if (lane == 0) sh.best[threadIdx.x >> 5] = mine;
+        __syncthreads();
+        const unsigned long long own = sh.best[lane % LP_WARPS];
+        int above = 0;
+#pragma unroll
+        for (int i = 0; i < LP_WARPS; ++i) above += sh.best[i] > own;   // (entries are distinct, but for the zeros)
+        const unsigned who = __ballot_sync(0xffffffffu, above == k - 1);
+        return who ? sh.best[(__ffs(who) - 1) % LP_WARPS] : 0ull;
+    }
     sh.best[threadIdx.x] = mine;
     __syncthreads();
     if (threadIdx.x < 32) {
@@ -123,7 +146,8 @@ template <int N, typename F> __device__ __forceinline__ void lp_best(LpShared& s
 #pragma unroll
     for (int i = 0; i < N; ++i) most = e[i] > most ? e[i] : most;
     if (tid == 0) sh.n = 0u;
-    unsigned long long b = lp_block_bound(sh, most, k);
+    const unsigned long long b = lp_block_bound(sh, most, k);
+    __syncthreads();
     // k + 2 + k / 8 threads at most have entries above the bound, and fewer than k have any where there is none
     unsigned long long* all = &sh.list[0][0];   // (the lists are in registers)
 #pragma unroll
@@ -148,51 +172,63 @@ __global__ void __launch_bounds__(LP_THREADS, 2) k_logprobs(const LpArgs a) {
     const int nbatch = (end + LP_BATCH - 1) / LP_BATCH, per = (nbatch + a.nsplit - 1) / a.nsplit;
     const int lo = (int) min((long long) split * per * LP_BATCH, (long long) end), hi = (int) min((long long) lo + (long long) per * LP_BATCH, (long long) end);
     const float* base = x - shift;
-    auto load = [&](int i0, float* v) {
+    extern __shared__ __align__(16) unsigned char lp_ring[];   // [LP_STAGES][2][LP_THREADS] runs of four
+    auto at = [&](int stage, int g) { return lp_ring + ((size_t) (stage * 2 + g) * LP_THREADS + tid) * 16; };
+    auto load = [&](int i0, int stage) {
+        if (i0 < hi)
 #pragma unroll
-        for (int g = 0; g < 2; ++g) {
-            const int p = i0 + g * (LP_BATCH / 2) + tid * 4;
-            if (p >= shift && p + 4 <= hi) {
-                const float4 f = __ldcs(reinterpret_cast<const float4*>(base + p));
-                v[4 * g] = f.x, v[4 * g + 1] = f.y, v[4 * g + 2] = f.z, v[4 * g + 3] = f.w;
-            } else {
+            for (int g = 0; g < 2; ++g) {
+                const int p = i0 + g * (LP_BATCH / 2) + tid * 4;
+                if (p >= shift && p + 4 <= hi) {
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((unsigned) __cvta_generic_to_shared(at(stage, g))), "l"(base + p) : "memory");
+                } else {
+                    float v[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[4 * g + e] = p + e >= shift && p + e < hi ? base[p + e] : -INFINITY;
+                    for (int e = 0; e < 4; ++e) v[e] = p + e >= shift && p + e < hi ? base[p + e] : -INFINITY;
+                    *reinterpret_cast<float4*>(at(stage, g)) = make_float4(v[0], v[1], v[2], v[3]);
+                }
             }
-        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
     };
     auto index = [&](int i0, int j) { return i0 + (j >> 2) * (LP_BATCH / 2) + tid * 4 + (j & 3); };
     pdl_wait();
     pdl_go();
-    float r = -INFINITY, bound_v = -INFINITY;
+    const float L2E = 1.44269504f;
+    float r = -INFINITY, bound_v = -INFINITY;                              // r: the reference, in units of log2
     float2 z2 = make_float2(0.f, 0.f), s2 = make_float2(0.f, 0.f);   // the sums of the even and the odd values
     unsigned long long bound = 0ull;   // an entry has to be above it
     int cnt = 0;                       // this warp's list
     unsigned long long* list = sh.list[warp];
-    float next[LP_PER];
-    load(lo, next);
-    for (int i0 = lo; i0 < hi; i0 += LP_BATCH) {
-        float v[LP_PER];
 #pragma unroll
-        for (int j = 0; j < LP_PER; ++j) v[j] = next[j];
-        if (i0 + LP_BATCH < hi) load(i0 + LP_BATCH, next);
+    for (int i = 0; i < LP_STAGES - 1; ++i) load(lo + i * LP_BATCH, i);
+    int stage = 0;
+    for (int i0 = lo; i0 < hi; i0 += LP_BATCH) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(LP_STAGES - 2) : "memory");
+        float v[LP_PER];
+        {
+            const float4 f = *reinterpret_cast<const float4*>(at(stage, 0)), g = *reinterpret_cast<const float4*>(at(stage, 1));
+            v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w, v[4] = g.x, v[5] = g.y, v[6] = g.z, v[7] = g.w;
+        }
+        load(i0 + (LP_STAGES - 1) * LP_BATCH, (stage + LP_STAGES - 1) % LP_STAGES);
+        stage = (stage + 1) % LP_STAGES;
         float mx = v[0];
 #pragma unroll
         for (int j = 1; j < LP_PER; ++j) mx = fmaxf(mx, v[j]);
-        if (mx > r + 8.f || (r == -INFINITY && mx > -INFINITY)) {
-            const float d = fmaxf(r - mx, -200.f), f = __expf(d);
+        const float top = mx * L2E;
+        if (top > r + 8.f || (r == -INFINITY && mx > -INFINITY)) {
+            const float d = fmaxf(r - top, -200.f), f = ex2_ftz(d);
             s2.x = f * (s2.x + d * z2.x), s2.y = f * (s2.y + d * z2.y);
             z2.x *= f, z2.y *= f;
-            r = mx;
+            r = top;
         }
         const float less = r == -INFINITY ? 0.f : -r;
 #pragma unroll
         for (int j = 0; j < LP_PER; j += 2) {
-            float2 d = add2(make_float2(v[j], v[j + 1]), make_float2(less, less)), e = mul2(d, make_float2(1.44269504f, 1.44269504f));
-            e.x = ex2_ftz(e.x), e.y = ex2_ftz(e.y);
-            d.x = fmaxf(d.x, -200.f), d.y = fmaxf(d.y, -200.f);
+            float2 t = fma2(make_float2(v[j], v[j + 1]), make_float2(L2E, L2E), make_float2(less, less));
+            const float2 e = make_float2(ex2_ftz(t.x), ex2_ftz(t.y));
+            t.x = fmaxf(t.x, -200.f), t.y = fmaxf(t.y, -200.f);
             z2 = add2(z2, e);
-            s2 = fma2(e, d, s2);
+            s2 = fma2(e, t, s2);
         }
         if (!a.k) continue;
         if (i0 == lo) {
@@ -297,10 +333,10 @@ __global__ void __launch_bounds__(LP_THREADS, 2) k_logprobs(const LpArgs a) {
     if (tid == 0) {
         const bool bad = z != z, none = r == -INFINITY && !bad;
         if (bad || none) atomicOr(a.err, 16u);
-        const float lz = logf(z);
-        sh.lse = bad ? NAN : none ? -INFINITY : r + lz;
+        const double ln2 = 0.6931471805599453, lz = log2((double) z);
+        sh.lse = bad ? NAN : none ? -INFINITY : (float) (((double) r + lz) * ln2);
         a.lse[row] = sh.lse;
-        if (a.ent) a.ent[row] = bad ? NAN : none ? 0.f : fmaxf(lz - s / z, 0.f);
+        if (a.ent) a.ent[row] = bad ? NAN : none ? 0.f : fmaxf((float) ((lz - (double) s / z) * ln2), 0.f);
     }
     __syncthreads();
     const float lse = sh.lse;
@@ -355,7 +391,9 @@ int fnx_logprobs(const float* logits, size_t stride, int n, int T, int v0, const
     // the counters have their place whatever the call's sizes, so that one scratch serves calls of different ones
     a.part = reinterpret_cast<LpPart*>((char*) scratch + LP_BLOCKS * 4);
     a.cand = reinterpret_cast<unsigned long long*>(a.part + (size_t) T * ns);
-    launch(0, k_logprobs, dim3((unsigned) T * ns), LP_THREADS, 0, strm(st), a);
+    constexpr size_t ring = (size_t) LP_STAGES * LP_BATCH * 4;
+    if (smem_optin(k_logprobs, ring, "logprobs")) return 1;
+    launch(0, k_logprobs, dim3((unsigned) T * ns), LP_THREADS, ring, strm(st), a);
     return launch_ok("logprobs");
 }
 }
