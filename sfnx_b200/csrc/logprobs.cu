@@ -24,18 +24,19 @@
 
 namespace fnxk {
 
-constexpr int LP_THREADS = 512, LP_WARPS = LP_THREADS / 32, LP_PER = 8, LP_BATCH = LP_THREADS * LP_PER, LP_LIST = 256;
+constexpr int LP_THREADS = 384, LP_WARPS = LP_THREADS / 32, LP_PER = 8, LP_BATCH = LP_THREADS * LP_PER, LP_LIST = 256;
 constexpr int LP_CAP = LP_WARPS * LP_LIST;   // entries of all lists
 constexpr int LP_STAGES = 4;            // batches in the ring
+constexpr int LP_TIGHTEN = 6;           // batches after which the bound is made anew
 constexpr int LP_BLOCKS = 2 * 148;   // blocks the GPU holds at once; rows that go to several blocks are fewer
 
-struct LpPart {   // a block's part of a row
+struct LpPart {   // the sums over a block's part of a row
     float r, z, s, pad;
 };
 struct LpArgs {
     const float* logits;
     size_t stride;
-    int n, v0, k, ntok, nsplit;
+    int rows, n, v0, k, ntok, nsplit;
     const int* tok;
     float *lse, *ent, *lp, *top_lp;
     int* top_i;
@@ -107,8 +108,8 @@ struct LpShared {
     float lse;
 };
 
-// A bound that at least k of the threads' maxima reach (0: where fewer than k have any, or warps in the first case).  Few: the k-th largest of the
-// warps' maxima; else bisection over the threads' by one warp
+// A bound that at least k of the threads' maxima reach (0 where fewer have any).  Few: the k-th largest of the warps' maxima (0 where
+// fewer warps have any); else bisection over the threads' by one warp
 __device__ __forceinline__ unsigned long long lp_block_bound(LpShared& sh, unsigned long long mine, int k) {
     const int lane = threadIdx.x & 31;
     if (k <= LP_WARPS) {
@@ -124,7 +125,9 @@ __device__ __forceinline__ unsigned long long lp_block_bound(LpShared& sh, unsig
 #pragma unroll
         for (int i = 0; i < LP_WARPS; ++i) above += sh.best[i] > own;   // (entries are distinct, but for the zeros)
         const unsigned who = __ballot_sync(0xffffffffu, above == k - 1);
-        return who ? sh.best[(__ffs(who) - 1) % LP_WARPS] : 0ull;
+        const unsigned long long b = who ? sh.best[(__ffs(who) - 1) % LP_WARPS] : 0ull;
+        __syncthreads();   // the next call writes there
+        return b;
     }
     sh.best[threadIdx.x] = mine;
     __syncthreads();
@@ -147,7 +150,6 @@ template <int N, typename F> __device__ __forceinline__ void lp_best(LpShared& s
     for (int i = 0; i < N; ++i) most = e[i] > most ? e[i] : most;
     if (tid == 0) sh.n = 0u;
     const unsigned long long b = lp_block_bound(sh, most, k);
-    __syncthreads();
     // k + 2 + k / 8 threads at most have entries above the bound, and fewer than k have any where there is none
     unsigned long long* all = &sh.list[0][0];   // (the lists are in registers)
 #pragma unroll
@@ -163,198 +165,233 @@ template <int N, typename F> __device__ __forceinline__ void lp_best(LpShared& s
     }
 }
 
+struct LpItem {   // a block's part of a row
+    const float* base;   // positions are counted from the 16-byte boundary at or before the row's first logit
+    int row, split, shift, lo, hi;
+};
+__device__ __forceinline__ LpItem lp_item(const LpArgs& a, long long w) {
+    LpItem t;
+    t.row = (int) (w / a.nsplit), t.split = (int) (w % a.nsplit);
+    const float* x = a.logits + (size_t) t.row * a.stride;
+    t.shift = (int) (((uintptr_t) x >> 2) & 3u), t.base = x - t.shift;
+    const int end = a.n + t.shift, batches = (end + LP_BATCH - 1) / LP_BATCH, per = (batches + a.nsplit - 1) / a.nsplit;
+    t.lo = (int) min((long long) t.split * per * LP_BATCH, (long long) end), t.hi = (int) min((long long) t.lo + (long long) per * LP_BATCH, (long long) end);
+    return t;
+}
+
 __global__ void __launch_bounds__(LP_THREADS, 2) k_logprobs(const LpArgs a) {
     __shared__ LpShared sh;
-    const int row = blockIdx.x / a.nsplit, split = blockIdx.x % a.nsplit, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const float* x = a.logits + (size_t) row * a.stride;
-    // positions are counted from the 16-byte boundary at or before the row's first logit: a thread has two runs of four a batch
-    const int shift = (int) (((uintptr_t) x >> 2) & 3u), end = a.n + shift;
-    const int nbatch = (end + LP_BATCH - 1) / LP_BATCH, per = (nbatch + a.nsplit - 1) / a.nsplit;
-    const int lo = (int) min((long long) split * per * LP_BATCH, (long long) end), hi = (int) min((long long) lo + (long long) per * LP_BATCH, (long long) end);
-    const float* base = x - shift;
     extern __shared__ __align__(16) unsigned char lp_ring[];   // [LP_STAGES][2][LP_THREADS] runs of four
-    auto at = [&](int stage, int g) { return lp_ring + ((size_t) (stage * 2 + g) * LP_THREADS + tid) * 16; };
-    auto load = [&](int i0, int stage) {
-        if (i0 < hi)
-#pragma unroll
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    unsigned long long* list = sh.list[warp];
+    const unsigned ring = (unsigned) __cvta_generic_to_shared(lp_ring) + tid * 16;   // this thread's slots, a stage's two LP_THREADS * 16 bytes apart
+    constexpr unsigned RUN = LP_THREADS * 16;
+    auto load = [&](const LpItem& t, int i0, unsigned slot) {   // a thread has two runs of four a batch
+        if (i0 >= t.lo + 4 && i0 + LP_BATCH <= t.hi) {   // whole runs all
+            const float* src = t.base + i0 + tid * 4;
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(slot), "l"(src) : "memory");
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(slot + RUN), "l"(src + LP_BATCH / 2) : "memory");
+        } else if (i0 < t.hi) {
+#pragma unroll 1
             for (int g = 0; g < 2; ++g) {
                 const int p = i0 + g * (LP_BATCH / 2) + tid * 4;
-                if (p >= shift && p + 4 <= hi) {
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((unsigned) __cvta_generic_to_shared(at(stage, g))), "l"(base + p) : "memory");
+                if (p >= t.shift && p + 4 <= t.hi) {
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(slot + g * RUN), "l"(t.base + p) : "memory");
                 } else {
                     float v[4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] = p + e >= shift && p + e < hi ? base[p + e] : -INFINITY;
-                    *reinterpret_cast<float4*>(at(stage, g)) = make_float4(v[0], v[1], v[2], v[3]);
+                    for (int e = 0; e < 4; ++e) v[e] = p + e >= t.shift && p + e < t.hi ? t.base[p + e] : -INFINITY;
+                    asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(slot + g * RUN), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]) : "memory");
                 }
             }
+        }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
+    auto slot = [&](int stage) { return ring + (unsigned) stage * (2 * RUN); };
     auto index = [&](int i0, int j) { return i0 + (j >> 2) * (LP_BATCH / 2) + tid * 4 + (j & 3); };
     pdl_wait();
     pdl_go();
     const float L2E = 1.44269504f;
-    float r = -INFINITY, bound_v = -INFINITY;                              // r: the reference, in units of log2
-    float2 z2 = make_float2(0.f, 0.f), s2 = make_float2(0.f, 0.f);   // the sums of the even and the odd values
-    unsigned long long bound = 0ull;   // an entry has to be above it
-    int cnt = 0;                       // this warp's list
-    unsigned long long* list = sh.list[warp];
-#pragma unroll
-    for (int i = 0; i < LP_STAGES - 1; ++i) load(lo + i * LP_BATCH, i);
+    const long long items = (long long) a.rows * a.nsplit;
+    LpItem next = lp_item(a, blockIdx.x);
     int stage = 0;
-    for (int i0 = lo; i0 < hi; i0 += LP_BATCH) {
-        asm volatile("cp.async.wait_group %0;" ::"n"(LP_STAGES - 2) : "memory");
-        float v[LP_PER];
-        {
-            const float4 f = *reinterpret_cast<const float4*>(at(stage, 0)), g = *reinterpret_cast<const float4*>(at(stage, 1));
-            v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w, v[4] = g.x, v[5] = g.y, v[6] = g.z, v[7] = g.w;
-        }
-        load(i0 + (LP_STAGES - 1) * LP_BATCH, (stage + LP_STAGES - 1) % LP_STAGES);
-        stage = (stage + 1) % LP_STAGES;
-        float mx = v[0];
 #pragma unroll
-        for (int j = 1; j < LP_PER; ++j) mx = fmaxf(mx, v[j]);
-        const float top = mx * L2E;
-        if (top > r + 8.f || (r == -INFINITY && mx > -INFINITY)) {
-            const float d = fmaxf(r - top, -200.f), f = ex2_ftz(d);
-            s2.x = f * (s2.x + d * z2.x), s2.y = f * (s2.y + d * z2.y);
-            z2.x *= f, z2.y *= f;
-            r = top;
-        }
-        const float less = r == -INFINITY ? 0.f : -r;
+    for (int i = 0; i < LP_STAGES - 1; ++i) load(next, next.lo + i * LP_BATCH, slot(i));
+    for (long long w = blockIdx.x; w < items; w += gridDim.x) {
+        const LpItem t = next;
+        float r = -INFINITY, bound_v = -INFINITY;                        // r: the reference, in units of log2
+        float2 z2 = make_float2(0.f, 0.f), s2 = make_float2(0.f, 0.f);   // the sums of the even and the odd values
+        unsigned long long bound = 0ull;                                 // an entry has to be above it
+        int cnt = 0;                                                     // this warp's list
+        for (int i0 = t.lo; i0 < t.hi; i0 += LP_BATCH) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(LP_STAGES - 2) : "memory");
+            float v[LP_PER];
+            asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]) : "r"(slot(stage)) : "memory");
+            asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]) : "r"(slot(stage) + RUN) : "memory");
+            load(t, i0 + (LP_STAGES - 1) * LP_BATCH, slot((stage + LP_STAGES - 1) % LP_STAGES));
+            stage = (stage + 1) % LP_STAGES;
+            float mx = v[0];
 #pragma unroll
-        for (int j = 0; j < LP_PER; j += 2) {
-            float2 t = fma2(make_float2(v[j], v[j + 1]), make_float2(L2E, L2E), make_float2(less, less));
-            const float2 e = make_float2(ex2_ftz(t.x), ex2_ftz(t.y));
-            t.x = fmaxf(t.x, -200.f), t.y = fmaxf(t.y, -200.f);
-            z2 = add2(z2, e);
-            s2 = fma2(e, t, s2);
-        }
-        if (!a.k) continue;
-        if (i0 == lo) {
-            unsigned long long most = 0ull;
+            for (int j = 1; j < LP_PER; ++j) mx = fmaxf(mx, v[j]);
+            const float top = mx * L2E;
+            if (top > r + 8.f || (r == -INFINITY && mx > -INFINITY)) {
+                const float d = fmaxf(r - top, -200.f), f = ex2_ftz(d);
+                s2.x = f * (s2.x + d * z2.x), s2.y = f * (s2.y + d * z2.y);
+                z2.x *= f, z2.y *= f;
+                r = top;
+            }
+            const float less = r == -INFINITY ? 0.f : -r;
+#pragma unroll
+            for (int j = 0; j < LP_PER; j += 2) {
+                float2 q = fma2(make_float2(v[j], v[j + 1]), make_float2(L2E, L2E), make_float2(less, less));
+                const float2 e = make_float2(ex2_ftz(q.x), ex2_ftz(q.y));
+                q.x = fmaxf(q.x, -200.f), q.y = fmaxf(q.y, -200.f);
+                z2 = add2(z2, e);
+                s2 = fma2(e, q, s2);
+            }
+            if (!a.k) continue;
+            if (i0 == t.lo) {
+                unsigned long long most = 0ull;
+#pragma unroll
+                for (int j = 0; j < LP_PER; ++j) {
+                    const int p = index(i0, j);
+                    const unsigned long long c = p >= t.shift && p < t.hi && v[j] == v[j] ? lp_composite(v[j], (unsigned) (p - t.shift)) : 0ull;
+                    most = c > most ? c : most;
+                }
+                bound = lp_block_bound(sh, most, a.k);
+                bound_v = bound ? fkey_inv((unsigned) (bound >> 32)) : -INFINITY;
+                bound -= bound != 0ull;   // the bound itself may enter
+            }
+            // some way on, the bound of everything so far: fewer values pass it from there on
+            if (i0 == t.lo + LP_TIGHTEN * LP_BATCH) {
+                unsigned long long most = 0ull;
+                __syncwarp();
+                for (int i = lane; i < cnt; i += 32) most = list[i] > most ? list[i] : most;
+                const unsigned long long b = lp_block_bound(sh, most, a.k);
+                if (b > bound + 1ull) bound = b - 1ull, bound_v = fkey_inv((unsigned) (b >> 32));
+            }
+            if (!__any_sync(0xffffffffu, mx >= bound_v)) continue;
+            unsigned any = 0u;
+#pragma unroll
+            for (int j = 0; j < LP_PER; ++j) any |= v[j] >= bound_v ? 1u << j : 0u;
+            any = __reduce_or_sync(0xffffffffu, any);
 #pragma unroll
             for (int j = 0; j < LP_PER; ++j) {
+                if (!(any >> j & 1u)) continue;
                 const int p = index(i0, j);
-                const unsigned long long c = p >= shift && p < hi && v[j] == v[j] ? lp_composite(v[j], (unsigned) (p - shift)) : 0ull;
-                most = c > most ? c : most;
-            }
-            bound = lp_block_bound(sh, most, a.k);
-            bound_v = bound ? fkey_inv((unsigned) (bound >> 32)) : -INFINITY;
-            bound -= bound != 0ull;   // the bound itself may enter
-        }
-        if (!__any_sync(0xffffffffu, mx >= bound_v)) continue;
-        unsigned any = 0u;
+                bool in = v[j] >= bound_v && p >= t.shift && p < t.hi;
+                if (cnt + 32 > LP_LIST) {   // full: its best k stay
+                    unsigned long long e[LP_LIST / 32];
+                    __syncwarp();
 #pragma unroll
-        for (int j = 0; j < LP_PER; ++j) any |= v[j] >= bound_v ? 1u << j : 0u;
-        any = __reduce_or_sync(0xffffffffu, any);
+                    for (int i = 0; i < LP_LIST / 32; ++i) e[i] = i * 32 + lane < cnt ? list[i * 32 + lane] : 0ull;
+                    const unsigned long long b = lp_bound(e, a.k, 0);
+                    __syncwarp();
+                    cnt = 0;
 #pragma unroll
-        for (int j = 0; j < LP_PER; ++j) {
-            if (!(any >> j & 1u)) continue;
-            const int p = index(i0, j);
-            bool in = v[j] >= bound_v && p >= shift && p < hi;
-            if (cnt + 32 > LP_LIST) {   // full: its best k stay
-                unsigned long long e[LP_LIST / 32];
-                __syncwarp();
-#pragma unroll
-                for (int i = 0; i < LP_LIST / 32; ++i) e[i] = i * 32 + lane < cnt ? list[i * 32 + lane] : 0ull;
-                const unsigned long long b = lp_bound(e, a.k, 0);
-                __syncwarp();
-                cnt = 0;
-#pragma unroll
-                for (int i = 0; i < LP_LIST / 32; ++i) {
-                    const bool keep = e[i] >= b;
-                    const unsigned kept = __ballot_sync(0xffffffffu, keep);
-                    if (keep) list[cnt + __popc(kept & ((1u << lane) - 1u))] = e[i];
-                    cnt += __popc(kept);
+                    for (int i = 0; i < LP_LIST / 32; ++i) {
+                        const bool keep = e[i] >= b;
+                        const unsigned kept = __ballot_sync(0xffffffffu, keep);
+                        if (keep) list[cnt + __popc(kept & ((1u << lane) - 1u))] = e[i];
+                        cnt += __popc(kept);
+                    }
+                    bound = b, bound_v = fkey_inv((unsigned) (b >> 32));
                 }
-                bound = b, bound_v = fkey_inv((unsigned) (b >> 32));
+                const unsigned long long c = lp_composite(v[j], (unsigned) (p - t.shift));
+                in = in && c > bound;
+                const unsigned who = __ballot_sync(0xffffffffu, in);
+                if (in) list[cnt + __popc(who & ((1u << lane) - 1u))] = c;
+                cnt += __popc(who);
             }
-            const unsigned long long c = lp_composite(v[j], (unsigned) (p - shift));
-            in = in && c > bound;
-            const unsigned who = __ballot_sync(0xffffffffu, in);
-            if (in) list[cnt + __popc(who & ((1u << lane) - 1u))] = c;
-            cnt += __popc(who);
         }
-    }
-    // ---- the block's statistics
-    float z = z2.x + z2.y, s = s2.x + s2.y;
+        if (w + gridDim.x < items) {   // the next row's first batches are on their way while this one is finished
+            next = lp_item(a, w + gridDim.x);
 #pragma unroll
-    for (int o = 16; o; o >>= 1) {
-        const float ro = __shfl_xor_sync(0xffffffffu, r, o), zo = __shfl_xor_sync(0xffffffffu, z, o), so = __shfl_xor_sync(0xffffffffu, s, o);
-        lp_join(r, z, s, ro, zo, so);
-    }
-    if (lane == 0) sh.r[warp] = r, sh.z[warp] = z, sh.s[warp] = s;
-    unsigned long long e[LP_LIST / 32];
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < LP_LIST / 32; ++i) e[i] = i * 32 + lane < cnt ? list[i * 32 + lane] : 0ull;
-    __syncthreads();
-    const bool many = a.nsplit > 1;
-    LpPart* parts = a.part + (size_t) row * a.nsplit;
-    unsigned long long* cands = a.cand + (size_t) row * a.nsplit * a.k;
-    if (warp == 0) {
-        r = lane < LP_WARPS ? sh.r[lane] : -INFINITY, z = lane < LP_WARPS ? sh.z[lane] : 0.f, s = lane < LP_WARPS ? sh.s[lane] : 0.f;
-#pragma unroll
-        for (int o = LP_WARPS / 2; o; o >>= 1) {
-            const float r2 = __shfl_xor_sync(0xffffffffu, r, o), z2 = __shfl_xor_sync(0xffffffffu, z, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
-            lp_join(r, z, s, r2, z2, s2);
+            for (int i = 0; i < LP_STAGES - 1; ++i) load(next, next.lo + i * LP_BATCH, slot((stage + i) % LP_STAGES));
         }
-        if (many && lane == 0) parts[split] = LpPart{r, z, s, 0.f};
-    }
-    if (many) {   // the row's last block joins the parts
-        if (a.k) {
-            for (int i = tid; i < a.k; i += LP_THREADS) cands[(size_t) split * a.k + i] = 0ull;
-            __syncthreads();
-            lp_best(sh, e, a.k, [&](int at, unsigned long long c) { cands[(size_t) split * a.k + at] = c; });
+        // ---- the block's statistics
+        float z = z2.x + z2.y, s = s2.x + s2.y;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) {
+            const float ro = __shfl_xor_sync(0xffffffffu, r, o), zo = __shfl_xor_sync(0xffffffffu, z, o), so = __shfl_xor_sync(0xffffffffu, s, o);
+            lp_join(r, z, s, ro, zo, so);
         }
-        __threadfence();
+        if (lane == 0) sh.r[warp] = r, sh.z[warp] = z, sh.s[warp] = s;
+        unsigned long long e[LP_LIST / 32];
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < LP_LIST / 32; ++i) e[i] = i * 32 + lane < cnt ? list[i * 32 + lane] : 0ull;
         __syncthreads();
-        if (tid == 0) sh.last = atomicAdd(&a.count[row], 1u) == (unsigned) a.nsplit - 1u;
-        __syncthreads();
-        if (!sh.last) return;
-        __threadfence();
+        LpPart* parts = a.part + (size_t) t.row * a.nsplit;
+        unsigned long long* cands = a.cand + (size_t) t.row * a.nsplit * a.k;
         if (warp == 0) {
-            r = -INFINITY, z = 0.f, s = 0.f;
-            for (int i = lane; i < a.nsplit; i += 32) {
-                const LpPart p = parts[i];
-                lp_join(r, z, s, p.r, p.z, p.s);
-            }
+            r = lane < LP_WARPS ? sh.r[lane] : -INFINITY, z = lane < LP_WARPS ? sh.z[lane] : 0.f, s = lane < LP_WARPS ? sh.s[lane] : 0.f;
 #pragma unroll
             for (int o = 16; o; o >>= 1) {
-                const float r2 = __shfl_xor_sync(0xffffffffu, r, o), z2 = __shfl_xor_sync(0xffffffffu, z, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
-                lp_join(r, z, s, r2, z2, s2);
+                const float ro = __shfl_xor_sync(0xffffffffu, r, o), zo = __shfl_xor_sync(0xffffffffu, z, o), so = __shfl_xor_sync(0xffffffffu, s, o);
+                lp_join(r, z, s, ro, zo, so);
             }
         }
+        bool mine = true;   // whether the row's results are this block's to write
+        if (a.nsplit > 1) {   // the row's last block joins the parts
+            if (tid == 0) parts[t.split] = LpPart{r, z, s, 0.f};
+            if (a.k) {
+                for (int i = tid; i < a.k; i += LP_THREADS) cands[(size_t) t.split * a.k + i] = 0ull;
+                __syncthreads();
+                lp_best(sh, e, a.k, [&](int place, unsigned long long c) { cands[(size_t) t.split * a.k + place] = c; });
+            }
+            __threadfence();
+            __syncthreads();
+            if (tid == 0) sh.last = atomicAdd(&a.count[t.row], 1u) == (unsigned) a.nsplit - 1u;
+            __syncthreads();
+            mine = sh.last != 0u;
+            if (mine) {
+                __threadfence();
+                if (warp == 0) {
+                    r = -INFINITY, z = 0.f, s = 0.f;
+                    for (int i = lane; i < a.nsplit; i += 32) {
+                        const LpPart p = parts[i];
+                        lp_join(r, z, s, p.r, p.z, p.s);
+                    }
 #pragma unroll
-        for (int i = 0; i < LP_LIST / 32; ++i) e[i] = i * LP_THREADS + tid < a.nsplit * a.k ? cands[i * LP_THREADS + tid] : 0ull;
-        if (tid == 0) a.count[row] = 0u;
+                    for (int o = 16; o; o >>= 1) {
+                        const float ro = __shfl_xor_sync(0xffffffffu, r, o), zo = __shfl_xor_sync(0xffffffffu, z, o), so = __shfl_xor_sync(0xffffffffu, s, o);
+                        lp_join(r, z, s, ro, zo, so);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < LP_LIST / 32; ++i) e[i] = i * LP_THREADS + tid < a.nsplit * a.k ? cands[i * LP_THREADS + tid] : 0ull;
+                if (tid == 0) a.count[t.row] = 0u;
+            }
+        }
+        if (mine) {
+            if (tid == 0) {
+                const bool bad = z != z, none = r == -INFINITY && !bad;
+                if (bad || none) atomicOr(a.err, 16u);
+                const double ln2 = 0.6931471805599453, lz = log2((double) z);
+                sh.lse = bad ? NAN : none ? -INFINITY : (float) (((double) r + lz) * ln2);
+                a.lse[t.row] = sh.lse;
+                if (a.ent) a.ent[t.row] = bad ? NAN : none ? 0.f : fmaxf((float) ((lz - (double) s / z) * ln2), 0.f);
+            }
+            __syncthreads();
+            const float lse = sh.lse;
+            const bool bad = lse != lse, none = lse == -INFINITY;
+            for (int j = tid; j < a.ntok; j += LP_THREADS) {
+                const long long i = (long long) a.tok[(size_t) t.row * a.ntok + j] - a.v0;
+                const bool in = i >= 0 && i < a.n;
+                a.lp[(size_t) t.row * a.ntok + j] = !in ? -INFINITY : bad ? NAN : none ? -INFINITY : t.base[t.shift + i] - lse;
+            }
+            if (a.k && bad) {   // no order to speak of
+                for (int j = tid; j < a.k; j += LP_THREADS) a.top_i[(size_t) t.row * a.k + j] = -1, a.top_lp[(size_t) t.row * a.k + j] = NAN;
+            } else if (a.k) {
+                lp_best(sh, e, a.k, [&](int place, unsigned long long c) {
+                    a.top_i[(size_t) t.row * a.k + place] = a.v0 + (int) (0xffffffffu - (unsigned) (c & 0xffffffffu));
+                    a.top_lp[(size_t) t.row * a.k + place] = none ? -INFINITY : fkey_inv((unsigned) (c >> 32)) - lse;
+                });
+            }
+        }
+        __syncthreads();   // the lists are the next row's
     }
-    if (tid == 0) {
-        const bool bad = z != z, none = r == -INFINITY && !bad;
-        if (bad || none) atomicOr(a.err, 16u);
-        const double ln2 = 0.6931471805599453, lz = log2((double) z);
-        sh.lse = bad ? NAN : none ? -INFINITY : (float) (((double) r + lz) * ln2);
-        a.lse[row] = sh.lse;
-        if (a.ent) a.ent[row] = bad ? NAN : none ? 0.f : fmaxf((float) ((lz - (double) s / z) * ln2), 0.f);
-    }
-    __syncthreads();
-    const float lse = sh.lse;
-    const bool bad = lse != lse, none = lse == -INFINITY;
-    for (int j = tid; j < a.ntok; j += LP_THREADS) {
-        const long long t = (long long) a.tok[(size_t) row * a.ntok + j] - a.v0;
-        const bool in = t >= 0 && t < a.n;
-        a.lp[(size_t) row * a.ntok + j] = !in ? -INFINITY : bad ? NAN : none ? -INFINITY : x[t] - lse;
-    }
-    if (!a.k) return;
-    if (bad) {   // no order to speak of
-        for (int j = tid; j < a.k; j += LP_THREADS) a.top_i[(size_t) row * a.k + j] = -1, a.top_lp[(size_t) row * a.k + j] = NAN;
-        return;
-    }
-    lp_best(sh, e, a.k, [&](int at, unsigned long long c) {
-        a.top_i[(size_t) row * a.k + at] = a.v0 + (int) (0xffffffffu - (unsigned) (c & 0xffffffffu));
-        a.top_lp[(size_t) row * a.k + at] = none ? -INFINITY : fkey_inv((unsigned) (c >> 32)) - lse;
-    });
 }
 
 // blocks a row: as many as the GPU holds at once, each with a batch of the row at least; their k best have room in one block
@@ -386,14 +423,13 @@ int fnx_logprobs(const float* logits, size_t stride, int n, int T, int v0, const
     FNX_REQUIRE(logits && lse && scratch && err && (!k || (top_lp && top_i)), "logprobs: a null buffer");
     FNX_REQUIRE((uintptr_t) scratch % 16 == 0, "logprobs: scratch not 16-byte aligned");
     const int ns = lp_splits(n, T, k);
-    FNX_REQUIRE((long long) T * ns < (1ll << 31), "logprobs: %d rows", T);
-    LpArgs a{logits, stride, n, v0, k, ntok, ns, tok, lse, entropy, lp, top_lp, top_i, (unsigned*) scratch, nullptr, nullptr, err};
+    LpArgs a{logits, stride, T, n, v0, k, ntok, ns, tok, lse, entropy, lp, top_lp, top_i, (unsigned*) scratch, nullptr, nullptr, err};
     // the counters have their place whatever the call's sizes, so that one scratch serves calls of different ones
     a.part = reinterpret_cast<LpPart*>((char*) scratch + LP_BLOCKS * 4);
     a.cand = reinterpret_cast<unsigned long long*>(a.part + (size_t) T * ns);
     constexpr size_t ring = (size_t) LP_STAGES * LP_BATCH * 4;
     if (smem_optin(k_logprobs, ring, "logprobs")) return 1;
-    launch(0, k_logprobs, dim3((unsigned) T * ns), LP_THREADS, ring, strm(st), a);
+    launch(0, k_logprobs, dim3((unsigned) std::min<long long>((long long) T * ns, LP_BLOCKS)), LP_THREADS, ring, strm(st), a);
     return launch_ok("logprobs");
 }
 }
