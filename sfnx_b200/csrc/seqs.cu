@@ -41,8 +41,9 @@ __global__ void __launch_bounds__(TM_THREADS) k_tree_masks(const int* __restrict
 
 // ---------------------------------------------------------------- append
 // A block per row, a warp per head at a time (four heads' loads in flight): a lane holds E neighbouring elements of its head.  The
-// angles' sines and cosines (double precision) are made once a row for all heads.  Bound by DRAM: a row's queries and K/V are
-// read in f32 and written in f16.
+// angles' sines and cosines (double precision) are made once a row for all heads.  A row's queries and K/V are read in f32 and
+// written in f16 (40 us of copying at 5301 rows of 24 + 2 * 4 heads of 256); a block's own chain of dependent loads and the angles
+// bound it before DRAM does, so the loads come first and four blocks lie on a processor: 64.5 us (4.1 TB/s), with three 71.7.
 struct SaArgs {
     const float *qg, *k, *v, *qn, *kn;
     uint16_t *kc, *vc, *q16;
@@ -76,21 +77,43 @@ template <int E> __device__ __forceinline__ void sa_store(uint16_t* p, const SaV
     else *reinterpret_cast<uint2*>(p) = make_uint2(u[0], u[1]);
 }
 
+// The sum of 32 neighbouring values (E a lane) as the xor-tree over a warp forms it, offsets 16 .. 1: at each of the first steps a
+// lane keeps the half of its values that its partner does not, so nobody adds what another adds.  Every lane gets the sum.
+template <int E> __device__ __forceinline__ float sa_tree(const float* q, int lane) {
+    if constexpr (E == 8) {   // offset 16: lane ^ 2, 8: lane ^ 1, 4 .. 1: within a lane at first
+        const bool hi = lane & 2, odd = lane & 1;
+        float a[4], b[2];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) a[i] = fadd(hi ? q[4 + i] : q[i], __shfl_xor_sync(0xffffffffu, hi ? q[i] : q[4 + i], 2));
+#pragma unroll
+        for (int i = 0; i < 2; ++i) b[i] = fadd(odd ? a[2 + i] : a[i], __shfl_xor_sync(0xffffffffu, odd ? a[i] : a[2 + i], 1));
+        // b[i]: elements 4 hi + 2 odd + i of offsets 4 and less
+        float c = fadd(hi ? b[1] : b[0], __shfl_xor_sync(0xffffffffu, hi ? b[0] : b[1], 2));   // offset 4; element 2 odd + hi
+        c = fadd(c, __shfl_xor_sync(0xffffffffu, c, 1));                                         // offset 2
+        return fadd(c, __shfl_xor_sync(0xffffffffu, c, 2));                                      // offset 1
+    } else {   // offset 16: lane ^ 4, 8: lane ^ 2, 4: lane ^ 1
+        const bool hi = lane & 4, mid = lane & 2;
+        float a[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) a[i] = fadd(hi ? q[2 + i] : q[i], __shfl_xor_sync(0xffffffffu, hi ? q[i] : q[2 + i], 4));
+        float c = fadd(mid ? a[1] : a[0], __shfl_xor_sync(0xffffffffu, mid ? a[0] : a[1], 2));   // offset 8; element 2 hi + mid
+        c = fadd(c, __shfl_xor_sync(0xffffffffu, c, 1));                                         // offset 4
+        c = fadd(c, __shfl_xor_sync(0xffffffffu, c, 4));                                         // offset 2
+        return fadd(c, __shfl_xor_sync(0xffffffffu, c, 2));                                      // offset 1
+    }
+}
+
 template <int HD>
-__global__ void __launch_bounds__(SA_THREADS, 3) k_seqs_append(const __grid_constant__ SaArgs a) {
+__global__ void __launch_bounds__(SA_THREADS, 4) k_seqs_append(const __grid_constant__ SaArgs a) {
     constexpr int E = HD / 32;
-    __shared__ __align__(16) float sn[64], cs[64];
+    __shared__ __align__(16) float sn[64], cs[64], wt[2][HD];
     __shared__ float rot[SA_WARPS][128];
     const int t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nh = a.nq + 2 * a.nkv;
     pdl_wait();
     pdl_go();
-    const int s = sq_find(a.sq.row0, a.sq.nseq, t);
-    if (s < 0) return;   // behind the last sequence (the whole block agrees)
     const size_t row_elems = (size_t) a.nkv * HD;
-    auto source = [&](int h) {
-        return (h < a.nq ? a.qg + ((size_t) t * a.nq + h) * 2 * HD : h < a.nq + a.nkv ? a.k + (size_t) t * row_elems + (size_t) (h - a.nq) * HD
-                                                                                        : a.v + (size_t) t * row_elems + (size_t) (h - a.nq - a.nkv) * HD) + lane * E;
-    };
+    const float *rq = a.qg + (size_t) t * a.nq * 2 * HD + lane * E, *rk = a.k + (size_t) t * row_elems + lane * E, *rv = a.v + (size_t) t * row_elems + lane * E;
+    auto source = [&](int h) { return h < a.nq ? rq + h * 2 * HD : h < a.nq + a.nkv ? rk + (h - a.nq) * HD : rv + (h - a.nq - a.nkv) * HD; };
     SaVec<E> x[SA_HEADS];
     auto ask = [&](int h0) {
 #pragma unroll
@@ -98,55 +121,61 @@ __global__ void __launch_bounds__(SA_THREADS, 3) k_seqs_append(const __grid_cons
             if (h0 + b * SA_WARPS < nh) x[b] = sa_load<E>(source(h0 + b * SA_WARPS));
     };
     ask(warp);   // on their way while the row's place and angles are worked out
+    const int s = sq_find(a.sq.row0, a.sq.nseq, t);
+    if (s < 0) return;   // behind the last sequence (the whole block agrees)
     const int i0 = t - a.sq.row0[s], p0 = a.sq.pos0[s];
     const int turn = max(0, p0) + (a.depth ? max(0, a.depth[t]) : i0);
     if (threadIdx.x < a.nrot / 2) {
         const float theta = fmul((float) turn, a.freq[threadIdx.x]);
         ex_sincos((double) theta, &sn[threadIdx.x], &cs[threadIdx.x]);
     }
+    for (int i = threadIdx.x; i < HD; i += SA_THREADS) wt[0][i] = a.qn[i], wt[1][i] = a.kn[i];
     const long long cell = sq_cell(a.sq, a.g, s, p0 < 0 || i0 > INT_MAX - p0 ? -1 : p0 + i0);
     if (threadIdx.x == 0 && cell < 0) atomicOr(a.err, SQ_ERR_ROOM);
     const size_t at = cell < 0 ? 0 : sq_at(a.sq, a.g, cell, row_elems);
     __syncthreads();
-    // element i < nrot pairs with i -+ half: y = c x + d x', d negative for the lower one.  Whole lanes apart (half a multiple of
-    // E) the partner comes by a shuffle, else through shared memory
+    // element i < nrot pairs with i -+ half: the lower one becomes x c - x' s, the upper one x c + x' s, the first product rounded before the
+    // fused second.  Whole lanes apart (half a multiple of E) the partner comes by a shuffle, else through shared memory
     const int half = a.nrot / 2, apart = half % E ? 0 : half / E;
     const bool turned = lane * E < a.nrot, lower = lane * E < half;
     for (int h0 = warp; h0 < nh; h0 += SA_HEADS * SA_WARPS) {
         if (h0 != warp) ask(h0);
+        // ---- the heads' square sums, one root for all: lane b takes head b's
+        float mine = 1.f;
+#pragma unroll
+        for (int b = 0; b < SA_HEADS; ++b) {
+            if (h0 + b * SA_WARPS >= a.nq + a.nkv) continue;
+            float q[E];
+#pragma unroll
+            for (int e = 0; e < E; ++e) q[e] = fmul(x[b].x[e], x[b].x[e]);
+            const float group = sa_tree<E>(q, lane);
+            float tot = 0.f;
+#pragma unroll
+            for (int g = 0; g < E; ++g) tot = fadd(tot, __shfl_sync(0xffffffffu, group, g * (32 / E)));
+            mine = lane == b ? tot : mine;
+        }
+        mine = ex_rsqrt(fadd(fmul(mine, 1.0f / (float) HD), a.eps));   // (HD is a power of two: the quotient's bits)
 #pragma unroll
         for (int b = 0; b < SA_HEADS; ++b) {
             const int h = h0 + b * SA_WARPS;
             if (h >= nh) break;
             if (h < a.nq + a.nkv) {
-                // squares of 32 neighbouring elements summed as the xor-tree over a warp does (offsets 16 .. 1), the groups ascending
-                float q[E];
+                const float r = __shfl_sync(0xffffffffu, mine, b);
+                const SaVec<E> w = sa_load<E>(&wt[h < a.nq ? 0 : 1][lane * E]);
 #pragma unroll
-                for (int e = 0; e < E; ++e) q[e] = fmul(x[b].x[e], x[b].x[e]);
-#pragma unroll
-                for (int o = 16; o >= E; o >>= 1)
-#pragma unroll
-                    for (int e = 0; e < E; ++e) q[e] = fadd(q[e], __shfl_xor_sync(0xffffffffu, q[e], o / E));
-#pragma unroll
-                for (int o = E / 2; o; o >>= 1)
-#pragma unroll
-                    for (int e = 0; e < o; ++e) q[e] = fadd(q[e], q[e + o]);
-                float tot = 0.f;
-#pragma unroll
-                for (int g = 0; g < E; ++g) tot = fadd(tot, __shfl_sync(0xffffffffu, q[0], g * (32 / E)));
-                const float r = ex_rsqrt(fadd(fmul(tot, 1.0f / (float) HD), a.eps));   // (HD is a power of two: the quotient's bits)
-                const SaVec<E> wt = sa_load<E>((h < a.nq ? a.qn : a.kn) + lane * E);
-#pragma unroll
-                for (int e = 0; e < E; ++e) x[b].x[e] = fmul(fmul(x[b].x[e], r), wt.x[e]);
+                for (int e = 0; e < E; ++e) x[b].x[e] = fmul(fmul(x[b].x[e], r), w.x[e]);
                 if (apart) {
                     float other[E];
 #pragma unroll
                     for (int e = 0; e < E; ++e) other[e] = __shfl_sync(0xffffffffu, x[b].x[e], lower ? lane + apart : lane - apart);
                     if (turned) {
-                        const SaVec<E> c = sa_load<E>(&cs[lane * E - (lower ? 0 : half)]), d = sa_load<E>(&sn[lane * E - (lower ? 0 : half)]);
+                        const int i = lane * E - (lower ? 0 : half);
+                        const SaVec<E> c = sa_load<E>(lower ? &cs[i] : &sn[i]), d = sa_load<E>(lower ? &sn[i] : &cs[i]);
 #pragma unroll
-                        for (int e = 0; e < E; ++e)
-                            x[b].x[e] = lower ? ffma(-other[e], d.x[e], fmul(x[b].x[e], c.x[e])) : ffma(x[b].x[e], c.x[e], fmul(other[e], d.x[e]));
+                        for (int e = 0; e < E; ++e) {
+                            const float y = x[b].x[e];
+                            x[b].x[e] = ffma(lower ? -other[e] : y, d.x[e], fmul(lower ? y : other[e], c.x[e]));
+                        }
                     }
                 } else {
                     if (turned)
@@ -164,8 +193,8 @@ __global__ void __launch_bounds__(SA_THREADS, 3) k_seqs_append(const __grid_cons
             }
             if (h < a.nq) sa_store<E>(a.q16 + ((size_t) t * a.nq + h) * HD + lane * E, x[b]);
             else if (h < a.nq + a.nkv) {
-                if (cell >= 0) sa_store<E>(a.kc + at + (size_t) (h - a.nq) * HD + lane * E, x[b]);
-            } else if (cell >= 0) sa_store<E>(a.vc + at + (size_t) (h - a.nq - a.nkv) * HD + lane * E, x[b]);
+                if (cell >= 0) sa_store<E>(a.kc + at + (h - a.nq) * HD + lane * E, x[b]);
+            } else if (cell >= 0) sa_store<E>(a.vc + at + (h - a.nq - a.nkv) * HD + lane * E, x[b]);
         }
     }
 }
