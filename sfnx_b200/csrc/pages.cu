@@ -4,40 +4,43 @@
 // State is what the header says: a reference count a page, a table and a length a sequence.  Every result is a function of
 // that state alone: reference counts are sums of integers, free pages are handed out lowest first in the sequences' order,
 // and which holder of a shared page keeps it is the lowest, so no order of atomics shows.
-// The tables are a few thousand words: fork and reserve are bound by the latency of a handful of dependent steps and launches,
-// the row copies by DRAM.
+// The tables are a few thousand words: what these calls cost is the latency of a handful of dependent loads and launches, so
+// loads go out before their use is known and divisions are 32 bits wide; the row copies are DRAM's.
 #include <algorithm>
 #include <climits>
 
 #include "common.cuh"
-#include "exact_math.cuh"
+#include "moe_internal.cuh"
 
 namespace fnxk {
 
 constexpr int PG_SEQS = 4096, PG_THREADS = 1024, PG_WARPS = PG_THREADS / 32, PG_PER = PG_SEQS / PG_THREADS;
 constexpr unsigned PG_ERR_ROOM = 32u, PG_ERR_VALUE = 64u;
 
-// the scratch's words: a header (jobs of the copy), then per page: holders of a tail page in this call, the complement of the
-// lowest of them (both zero between calls), the free list; per sequence: copy jobs (from, to, rows), the verdict, the old length;
-// the old tables
+// the scratch's words: a header (jobs of the copy; blocks of a fork that have the lengths, zero between calls), then per page:
+// holders of a tail page in this call, the complement of the lowest of them (both zero between calls), the free list; per
+// sequence: copy jobs (from, to, rows), the verdict
 struct PgScratch {
-    int *njobs, *holders, *lowest, *free_list, *jobs, *verdict, *old_len, *old_pt;
+    int *njobs, *holders, *lowest, *free_list, *jobs, *verdict;
+    unsigned* seen;
 };
 __host__ __device__ inline PgScratch pg_scratch(const FnxPagePool& p, void* scratch) {
     int* w = (int*) scratch;
     PgScratch s;
-    s.njobs = w, w += 4;
+    s.njobs = w, s.seen = (unsigned*) w + 1, w += 4;
     s.holders = w, w += p.npages;
     s.lowest = w, w += p.npages;
     s.free_list = w, w += p.npages;
     s.jobs = w, w += 3 * (size_t) p.nseq;
-    s.verdict = w, w += p.nseq;
-    s.old_len = w, w += p.nseq;
-    s.old_pt = w;
+    s.verdict = w;
     return s;
 }
-__device__ __forceinline__ int pg_held(const FnxPagePool& p, int len) {   // pages that len positions need, at most the table's
-    return min((int) (((long long) max(len, 0) + p.rows - 1) / p.rows), p.pt_stride);
+__device__ __forceinline__ unsigned pg_pages(const FnxPagePool& p, unsigned len) {   // pages that len < 2^32 positions need
+    const unsigned rows = (unsigned) p.rows, q = len / rows;
+    return q + (q * rows != len);
+}
+__device__ __forceinline__ int pg_held(const FnxPagePool& p, int len) {   // at most the table's
+    return min((int) pg_pages(p, (unsigned) max(len, 0)), p.pt_stride);
 }
 __device__ __forceinline__ bool pg_valid(const FnxPagePool& p, int page) { return page >= 0 && page < p.npages; }
 
@@ -52,37 +55,50 @@ __host__ inline PgRows pg_rows(const FnxPagePool& p, const FnxKvPages& g, int nk
 }
 
 // ---------------------------------------------------------------- fork
-__global__ void __launch_bounds__(256) k_pages_save(const FnxPagePool p, void* scratch) {
+// A sequence's new table is another's old one, column by column: block i has 2^shift columns of all sequences in shared memory
+// before it writes one.  The lengths are one column for all blocks, so the last block to have read them writes them.
+__global__ void __launch_bounds__(256) k_pages_fork(const FnxPagePool p, const int* __restrict__ from, const int* __restrict__ lim, int shift, void* scratch,
+                                                    unsigned* err) {
+    extern __shared__ int pf_sm[];
+    __shared__ bool last;
     const PgScratch w = pg_scratch(p, scratch);
+    int *src = pf_sm, *held = src + p.nseq, *now_held = held + p.nseq, *now_len = now_held + p.nseq, *was = now_len + p.nseq;
+    const int j0 = (int) blockIdx.x << shift, n = p.nseq << shift, mask = (1 << shift) - 1;
     pdl_wait();
     pdl_go();
-    const long long n = (long long) p.nseq * p.pt_stride;
-    for (long long i = (long long) blockIdx.x * 256 + threadIdx.x; i < n; i += (long long) gridDim.x * 256) w.old_pt[i] = p.pt[i];
-    for (int s = blockIdx.x * 256 + threadIdx.x; s < p.nseq; s += gridDim.x * 256) w.old_len[s] = p.len[s];
-}
-__global__ void __launch_bounds__(256) k_pages_fork(const FnxPagePool p, const int* __restrict__ from, const int* __restrict__ lim, void* scratch, unsigned* err) {
-    const PgScratch w = pg_scratch(p, scratch);
-    pdl_wait();
-    pdl_go();
-    const long long n = (long long) p.nseq * p.pt_stride;
-    for (long long i = (long long) blockIdx.x * 256 + threadIdx.x; i < n; i += (long long) gridDim.x * 256) {
-        const int s = (int) (i / p.pt_stride), j = (int) (i % p.pt_stride);
-        int src = from[s];
-        if (src >= p.nseq) {
-            if (j == 0) atomicOr(err, PG_ERR_VALUE);
-            src = s;
-        }
-        int len = src < 0 ? 0 : max(w.old_len[src], 0);
-        if (lim) len = min(len, max(lim[s], 0));
-        const int was = j < pg_held(p, w.old_len[s]) ? w.old_pt[i] : -1;
-        const int now = j < pg_held(p, len) ? w.old_pt[(long long) src * p.pt_stride + j] : -1;
-        if (was != now) {
-            if (pg_valid(p, now)) atomicAdd(&p.ref[now], 1);
-            if (pg_valid(p, was)) atomicSub(&p.ref[was], 1);
-        }
-        p.pt[i] = now;
-        if (j == 0) p.len[s] = len;
+    for (int i = threadIdx.x; i < n; i += 256) {
+        const int j = j0 + (i & mask);
+        was[i] = j < p.pt_stride ? p.pt[(size_t) (i >> shift) * p.pt_stride + j] : -1;
     }
+    for (int s = threadIdx.x; s < p.nseq; s += 256) {
+        int f = from[s];
+        if (f >= p.nseq) {
+            if (blockIdx.x == 0) atomicOr(err, PG_ERR_VALUE);
+            f = s;
+        }
+        int len = f < 0 ? 0 : max(p.len[f], 0);
+        if (lim) len = min(len, max(lim[s], 0));
+        src[s] = f, held[s] = pg_held(p, p.len[s]), now_held[s] = pg_held(p, len), now_len[s] = len;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        __threadfence();
+        last = atomicAdd(w.seen, 1u) == gridDim.x - 1;
+    }
+    for (int i = threadIdx.x; i < n; i += 256) {
+        const int s = i >> shift, c = i & mask, j = j0 + c;
+        if (j >= p.pt_stride) continue;
+        const int before = j < held[s] ? was[i] : -1, now = j < now_held[s] ? was[(src[s] << shift) + c] : -1;
+        if (before != now) {
+            if (pg_valid(p, now)) atomicAdd(&p.ref[now], 1);
+            if (pg_valid(p, before)) atomicSub(&p.ref[before], 1);
+        }
+        if (was[i] != now) p.pt[(size_t) s * p.pt_stride + j] = now;
+    }
+    __syncthreads();
+    if (!last) return;
+    for (int s = threadIdx.x; s < p.nseq; s += 256) p.len[s] = now_len[s];
+    if (threadIdx.x == 0) *w.seen = 0u;
 }
 
 // ---------------------------------------------------------------- reserve
@@ -107,30 +123,52 @@ __device__ __forceinline__ void pg_scan2(long long& a, long long& b, long long& 
     a += pa - a0, b += pb - b0;
 }
 
+constexpr int PG_NEAR = 2048;   // places of the list of pages handed out that lie in shared memory
 __global__ void __launch_bounds__(PG_THREADS) k_pages_reserve(const FnxPagePool p, const int* __restrict__ add, int* pos0, int* row0, void* scratch, unsigned* err) {
     const PgScratch w = pg_scratch(p, scratch);
     __shared__ long long sh[PG_WARPS][2];
-    __shared__ int first[PG_SEQS], wcount[PG_WARPS];   // a sequence's first place in the list of pages handed out
+    __shared__ int first[PG_SEQS], near[PG_NEAR], wcount[PG_WARPS];   // first: a sequence's first place in the list of pages handed out
+    __shared__ unsigned fresh[PG_SEQS];                                // where its new pages begin in its table, times two, + 1: after a copy
     __shared__ unsigned njobs_s;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, per = (p.nseq + PG_THREADS - 1) / PG_THREADS;
     if (tid == 0) njobs_s = 0u;
     pdl_wait();
     pdl_go();
-    // ---- what each sequence holds and wants; thread i has PG_PER neighbouring sequences
-    int len[PG_PER], more[PG_PER], tail[PG_PER], want[PG_PER];
+    auto free_bits = [&](int q0, unsigned* is) {   // a warp has 128 neighbouring pages of 4 * PG_THREADS
+        int ref[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int q = q0 + warp * 128 + k * 32 + lane;
+            ref[k] = q < p.npages ? p.ref[q] : 1;
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) is[k] = __ballot_sync(0xffffffffu, ref[k] == 0);
+    };
+    unsigned is[4];
+    free_bits(0, is);
+    // ---- what each sequence holds and wants; thread i has `per` neighbouring sequences
+    int len[PG_PER], more[PG_PER], tail[PG_PER], want[PG_PER], refs[PG_PER];
     bool bad = false, room = true;
 #pragma unroll
     for (int k = 0; k < PG_PER; ++k) {
-        const int s = tid * PG_PER + k;
-        len[k] = more[k] = want[k] = 0, tail[k] = -1;
-        if (s >= p.nseq) continue;
+        const int s = tid * per + k;
+        len[k] = more[k] = want[k] = refs[k] = 0, tail[k] = -1;
+        if (k >= per || s >= p.nseq) continue;
         len[k] = max(p.len[s], 0), more[k] = add[s];
+    }
+#pragma unroll
+    for (int k = 0; k < PG_PER; ++k) {
+        const int s = tid * per + k;
+        if (k >= per || s >= p.nseq) continue;
         if (more[k] < 0) bad = true;
-        else if (((long long) len[k] + more[k] + p.rows - 1) / p.rows > p.pt_stride) room = false;
-        else if (more[k] > 0 && len[k] % p.rows) {
+        else if (pg_pages(p, (unsigned) len[k] + (unsigned) more[k]) > (unsigned) p.pt_stride) room = false;
+        else if (more[k] > 0 && (unsigned) len[k] % (unsigned) p.rows) {
             tail[k] = p.pt[(size_t) s * p.pt_stride + len[k] / p.rows];
             if (!pg_valid(p, tail[k])) room = false, tail[k] = -1;
-            else atomicAdd(&w.holders[tail[k]], 1), atomicMax(&w.lowest[tail[k]], INT_MAX - s);
+            else {
+                atomicAdd(&w.holders[tail[k]], 1), atomicMax(&w.lowest[tail[k]], INT_MAX - s);
+                refs[k] = p.ref[tail[k]];
+            }
         }
     }
     __threadfence_block();
@@ -139,10 +177,10 @@ __global__ void __launch_bounds__(PG_THREADS) k_pages_reserve(const FnxPagePool 
     long long a = 0, b = 0, pages, rows;
 #pragma unroll
     for (int k = 0; k < PG_PER; ++k) {
-        const int s = tid * PG_PER + k;
-        copy[k] = tail[k] >= 0 && (p.ref[tail[k]] > __ldcg(&w.holders[tail[k]]) || __ldcg(&w.lowest[tail[k]]) != INT_MAX - s);
-        if (s < p.nseq && more[k] >= 0 && room)
-            want[k] = (int) (((long long) len[k] + more[k] + p.rows - 1) / p.rows - ((long long) len[k] + p.rows - 1) / p.rows) + (copy[k] ? 1 : 0);
+        const int s = tid * per + k;
+        copy[k] = tail[k] >= 0 && (refs[k] > __ldcg(&w.holders[tail[k]]) || __ldcg(&w.lowest[tail[k]]) != INT_MAX - s);
+        if (k < per && s < p.nseq && more[k] >= 0 && room)
+            want[k] = (int) (pg_pages(p, (unsigned) len[k] + (unsigned) more[k]) - pg_pages(p, (unsigned) len[k])) + (copy[k] ? 1 : 0);
         a += want[k], b += more[k] > 0 ? more[k] : 0;
     }
     __syncthreads();   // everyone has looked at the holders
@@ -155,27 +193,20 @@ __global__ void __launch_bounds__(PG_THREADS) k_pages_reserve(const FnxPagePool 
     // ---- the lowest free pages, as many as are wanted
     int got = 0;
     if (room && !bad)
-        for (int q0 = 0; q0 < p.npages && got < pages; q0 += 4 * PG_THREADS) {   // a warp has 128 neighbouring pages
-            unsigned is[4];
+        for (int q0 = 0; q0 < p.npages && got < pages; q0 += 4 * PG_THREADS) {
+            if (q0) free_bits(q0, is);
             int mine = 0, before[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int q = q0 + warp * 128 + k * 32 + lane;
-                is[k] = __ballot_sync(0xffffffffu, q < p.npages && p.ref[q] == 0);
-                before[k] = mine;
-                mine += __popc(is[k]);
-            }
+            for (int k = 0; k < 4; ++k) before[k] = mine, mine += __popc(is[k]);
             if (lane == 0) wcount[warp] = mine;
             __syncthreads();
-            int below = got;
-            for (int i = 0; i < PG_WARPS; ++i) {
-                if (i < warp) below += wcount[i];
-                got += wcount[i];
-            }
+            const int others = wcount[lane];   // (PG_WARPS = 32)
+            int below = got + __reduce_add_sync(0xffffffffu, lane < warp ? others : 0);
+            got += __reduce_add_sync(0xffffffffu, others);
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const int at = below + before[k] + __popc(is[k] & ((1u << lane) - 1u));
-                if ((is[k] >> lane & 1u) && at < pages) w.free_list[at] = q0 + warp * 128 + k * 32 + lane;
+                if ((is[k] >> lane & 1u) && at < pages) (at < PG_NEAR ? near[at] : w.free_list[at]) = q0 + warp * 128 + k * 32 + lane;
             }
             __syncthreads();
         }
@@ -183,8 +214,8 @@ __global__ void __launch_bounds__(PG_THREADS) k_pages_reserve(const FnxPagePool 
     if (!ok) {   // nothing changes
 #pragma unroll
         for (int k = 0; k < PG_PER; ++k) {
-            const int s = tid * PG_PER + k;
-            if (s < p.nseq) pos0[s] = len[k], row0[s] = 0;
+            const int s = tid * per + k;
+            if (k < per && s < p.nseq) pos0[s] = len[k], row0[s] = 0;
         }
         if (tid == 0) {
             row0[p.nseq] = 0, *w.njobs = 0;
@@ -192,31 +223,27 @@ __global__ void __launch_bounds__(PG_THREADS) k_pages_reserve(const FnxPagePool 
         }
         return;
     }
+    auto handed = [&](int i) { return i < PG_NEAR ? near[i] : w.free_list[i]; };
+    // ---- the lengths and the copies, then the new entries: place i of the list belongs to the last sequence that begins at or before it
 #pragma unroll
     for (int k = 0; k < PG_PER; ++k) {
-        const int s = tid * PG_PER + k;
-        first[s] = s < p.nseq ? (int) a : (int) pages;
-        if (s < p.nseq) {
-            pos0[s] = len[k], row0[s] = (int) b;
-            p.len[s] = len[k] + more[k];
+        const int s = tid * per + k;
+        if (k >= per || s >= p.nseq) continue;
+        first[s] = (int) a, fresh[s] = 2u * pg_pages(p, (unsigned) len[k]) + (copy[k] ? 1u : 0u);
+        pos0[s] = len[k], row0[s] = (int) b;
+        p.len[s] = len[k] + more[k];
+        if (copy[k]) {
+            const int page = handed((int) a);
+            p.pt[(size_t) s * p.pt_stride + len[k] / p.rows] = page;
+            p.ref[page] = 1;
+            atomicSub(&p.ref[tail[k]], 1);
+            const unsigned at = atomicAdd(&njobs_s, 1u);
+            w.jobs[3 * at] = tail[k], w.jobs[3 * at + 1] = page, w.jobs[3 * at + 2] = len[k] % p.rows;
         }
         a += want[k], b += more[k];
     }
-    if (tid == 0) row0[p.nseq] = (int) rows;
-    __threadfence_block();
     __syncthreads();
-    // ---- the copies, then the new entries: place i of the list belongs to the last sequence that begins at or before it
-#pragma unroll
-    for (int k = 0; k < PG_PER; ++k) {
-        const int s = tid * PG_PER + k;
-        if (!copy[k]) continue;
-        const int page = w.free_list[first[s]];
-        p.pt[(size_t) s * p.pt_stride + len[k] / p.rows] = page;
-        p.ref[page] = 1;
-        atomicSub(&p.ref[tail[k]], 1);
-        const unsigned at = atomicAdd(&njobs_s, 1u);
-        w.jobs[3 * at] = tail[k], w.jobs[3 * at + 1] = page, w.jobs[3 * at + 2] = len[k] % p.rows;
-    }
+    if (tid == 0) row0[p.nseq] = (int) rows, *w.njobs = (int) njobs_s;
     for (int i = tid; i < (int) pages; i += PG_THREADS) {
         int lo = 0, hi = p.nseq;   // first[lo] <= i
         while (hi - lo > 1) {
@@ -224,15 +251,12 @@ __global__ void __launch_bounds__(PG_THREADS) k_pages_reserve(const FnxPagePool 
             if (first[mid] <= i) lo = mid;
             else hi = mid;
         }
-        const int held = (pos0[lo] + p.rows - 1) / p.rows, total = (lo + 1 < p.nseq ? first[lo + 1] : (int) pages) - first[lo];
-        const int fresh = (int) (((long long) p.len[lo] + p.rows - 1) / p.rows) - held, j = i - first[lo] - (total - fresh);   // total - fresh: 1 with a copy
+        const int j = i - first[lo] - (int) (fresh[lo] & 1u);
         if (j < 0) continue;
-        const int page = w.free_list[i];
-        p.pt[(size_t) lo * p.pt_stride + held + j] = page;
+        const int page = handed(i);
+        p.pt[(size_t) lo * p.pt_stride + (fresh[lo] >> 1) + j] = page;
         p.ref[page] = 1;
     }
-    __syncthreads();
-    if (tid == 0) *w.njobs = (int) njobs_s;
 }
 
 // the rows so far of the pages that reserve copies: block (job, plane, piece of PG_PIECE bytes of a page)
@@ -266,27 +290,62 @@ __global__ void __launch_bounds__(256) k_pages_copy(const FnxPagePool p, void* c
 }
 
 // ---------------------------------------------------------------- keep
-// Block (sequence, plane).  A thread has 16 bytes of a row and walks the path in ascending order, eight rows' loads before
-// their stores: a kept row's old place is never before its new one, and the list ascends, so a store meets only rows whose
-// loads are done.  (Scales of int8 rows the same way, 8 bytes a thread.)
-__global__ void __launch_bounds__(128) k_pages_keep(const FnxPagePool p, const int* __restrict__ pos0, const int* __restrict__ keep, int keep_stride,
+// Block (sequence, plane).  Where each kept row lies goes to shared memory, PK_ROWS at a time; a thread has 16 bytes of a row and
+// walks the path in ascending order, PK_BATCH rows' loads before their stores: a kept row's old place is never before its new
+// one, and the list ascends, so a store meets only rows whose loads are done.  (Scales of int8 rows the same way, 8 bytes a
+// thread.)  The first batch's loads are under way while the pages are still looked at; nothing is stored before that is done.
+constexpr int PK_THREADS = 128, PK_ROWS = PK_THREADS, PK_BATCH = 16;
+struct PkMove {
+    int from, from_row, to, to_row;   // page and row in it; from negative: the row stays, or the list is senseless
+};
+__global__ void __launch_bounds__(PK_THREADS, 3) k_pages_keep(const FnxPagePool p, const int* __restrict__ pos0, const int* __restrict__ keep, int keep_stride,
                                                     const int* __restrict__ nkeep, void* const* __restrict__ planes, const PgRows r, void* scratch, unsigned* err) {
+    __shared__ PkMove moves[PK_ROWS];
     const PgScratch w = pg_scratch(p, scratch);
     pdl_wait();
     pdl_go();
-    const int s = blockIdx.x, n = nkeep[s], tid = threadIdx.x;
+    const int s = blockIdx.x, n = nkeep[s], tid = threadIdx.x, len = p.len[s], at0 = pos0[s];
+    char* base = (char*) planes[blockIdx.y];
     const bool head = blockIdx.y == 0;
     if (n < 0) {
         if (head && tid == 0) w.verdict[s] = -1;
         return;
     }
-    const int len = p.len[s], at0 = pos0[s], have = len - at0;
+    const int have = len - at0;
     const int* list = keep + (size_t) s * keep_stride;
     const int* pt = p.pt + (size_t) s * p.pt_stride;
-    bool bad = at0 < 0 || at0 > len || n > keep_stride || n > have || ((long long) len + p.rows - 1) / p.rows > p.pt_stride;
-    if (!bad) {
-        for (int i = tid; i < n; i += 128) bad = bad || list[i] < (i ? list[i - 1] + 1 : 0) || list[i] >= have;
-        for (int j = at0 / p.rows + tid; j < (len + p.rows - 1) / p.rows; j += 128) {   // the pages that rows are read from and written to
+    bool bad = at0 < 0 || at0 > len || n > keep_stride || n > have || pg_pages(p, (unsigned) max(len, 0)) > (unsigned) p.pt_stride;
+    const bool sound = !bad;   // (the whole block agrees)
+    auto find = [&](int i) {   // kept row i's way; i < n
+        PkMove m{-1, 0, 0, 0};
+        const int e = list[i];
+        if (e < i || e >= have) return m;
+        const unsigned rows = (unsigned) p.rows, f = (unsigned) (at0 + e) / rows, t = (unsigned) (at0 + i) / rows;
+        m.from = pt[f], m.to = pt[t], m.from_row = (int) (at0 + e - f * rows), m.to_row = (int) (at0 + i - t * rows);
+        if (e == i || !pg_valid(p, m.from) || !pg_valid(p, m.to)) m.from = -1;
+        return m;
+    };
+    if (sound && tid < n) moves[tid] = find(tid);
+    __syncthreads();
+    auto ask = [&](auto* v, int k0, int count, size_t start, size_t row_bytes, size_t c) {
+#pragma unroll
+        for (int k = 0; k < PK_BATCH; ++k)
+            if (k0 + k < count && moves[k0 + k].from >= 0)
+                v[k] = *reinterpret_cast<decltype(v)>(base + (size_t) moves[k0 + k].from * r.page_bytes + start + (size_t) moves[k0 + k].from_row * row_bytes + c);
+    };
+    auto put = [&](auto* v, int k0, int count, size_t start, size_t row_bytes, size_t c) {
+#pragma unroll
+        for (int k = 0; k < PK_BATCH; ++k)
+            if (k0 + k < count && moves[k0 + k].from >= 0)
+                *reinterpret_cast<decltype(v)>(base + (size_t) moves[k0 + k].to * r.page_bytes + start + (size_t) moves[k0 + k].to_row * row_bytes + c) = v[k];
+    };
+    uint4 v[PK_BATCH];
+    const bool mine = sound && (size_t) tid * 16 < r.row_bytes;
+    if (mine) ask(v, 0, min(n, PK_ROWS), 0, r.row_bytes, (size_t) tid * 16);
+    if (sound) {
+        for (int i = tid; i < n; i += PK_THREADS) bad = bad || list[i] < (i ? list[i - 1] + 1 : 0) || list[i] >= have;
+        const int end = (int) pg_pages(p, (unsigned) len);
+        for (int j = at0 / p.rows + tid; j < end; j += PK_THREADS) {   // the pages that rows are read from and written to
             const bool ours = pg_valid(p, pt[j]);
             bad = bad || !ours || (n > 0 && j * p.rows < at0 + n && p.ref[pt[j]] != 1);
         }
@@ -297,24 +356,27 @@ __global__ void __launch_bounds__(128) k_pages_keep(const FnxPagePool p, const i
         if (bad) atomicOr(err, PG_ERR_VALUE);
     }
     if (bad) return;
-    char* base = (char*) planes[blockIdx.y];
-    auto move = [&](size_t start, size_t row_bytes, auto unit) {
-        using U = decltype(unit);
-        for (size_t c = (size_t) tid * sizeof(U); c < row_bytes; c += 128 * sizeof(U)) {
-            auto at = [&](int pos) { return base + (size_t) pt[pos / p.rows] * r.page_bytes + start + (size_t) (pos % p.rows) * row_bytes + c; };
-            for (int i0 = 0; i0 < n; i0 += 8) {
-                U v[8];
-#pragma unroll
-                for (int k = 0; k < 8; ++k)
-                    if (i0 + k < n && list[i0 + k] != i0 + k) v[k] = *reinterpret_cast<const U*>(at(at0 + list[i0 + k]));
-#pragma unroll
-                for (int k = 0; k < 8; ++k)
-                    if (i0 + k < n && list[i0 + k] != i0 + k) *reinterpret_cast<U*>(at(at0 + i0 + k)) = v[k];
-            }
+    if (mine) put(v, 0, min(n, PK_ROWS), 0, r.row_bytes, (size_t) tid * 16);
+    for (int i0 = 0; i0 < n; i0 += PK_ROWS) {
+        const int count = min(n - i0, PK_ROWS);
+        if (i0) {
+            __syncthreads();   // everyone is done with the moves before these
+            if (tid < count) moves[tid] = find(i0 + tid);
+            __syncthreads();
         }
-    };
-    move(0, r.row_bytes, uint4{});
-    if (r.scale_at) move(r.scale_at, r.scale_bytes, uint2{});
+        for (size_t c = (size_t) tid * 16; c < r.row_bytes; c += PK_THREADS * 16)
+            for (int k0 = i0 == 0 && c == (size_t) tid * 16 ? PK_BATCH : 0; k0 < count; k0 += PK_BATCH) {
+                ask(v, k0, count, 0, r.row_bytes, c);
+                put(v, k0, count, 0, r.row_bytes, c);
+            }
+        if (r.scale_at)
+            for (size_t c = (size_t) tid * 8; c < r.scale_bytes; c += PK_THREADS * 8)
+                for (int k0 = 0; k0 < count; k0 += PK_BATCH) {
+                    uint2 u[PK_BATCH];
+                    ask(u, k0, count, r.scale_at, r.scale_bytes, c);
+                    put(u, k0, count, r.scale_at, r.scale_bytes, c);
+                }
+    }
 }
 // the lengths and what lies behind them, once every plane's rows are in place
 __global__ void __launch_bounds__(128) k_pages_trim(const FnxPagePool p, void* scratch) {
@@ -357,17 +419,16 @@ extern "C" {
 
 size_t fnx_pages_scratch_bytes(const FnxPagePool* p) {
     if (!p || p->npages < 1 || p->nseq < 1 || p->pt_stride < 1) return 0;
-    return 4 * (4 + 3 * (size_t) p->npages + 5 * (size_t) p->nseq + (size_t) p->nseq * p->pt_stride);
+    return 4 * (4 + 3 * (size_t) p->npages + 4 * (size_t) p->nseq);
 }
 
 int fnx_pages_fork(const FnxPagePool* p, const int* from, const int* lim, void* scratch, unsigned* err, void* st) {
     if (pg_check(p, scratch, err, "pages_fork")) return 1;
     FNX_REQUIRE(from, "pages_fork: a null buffer");
-    const long long n = (long long) p->nseq * p->pt_stride;
-    const unsigned blocks = (unsigned) std::min<long long>(148 * 8, (n + 255) / 256);
-    launch(0, k_pages_save, dim3(blocks), 256, 0, strm(st), *p, scratch);
-    if (launch_ok("pages_fork (tables as they were)")) return 1;
-    launch(0, k_pages_fork, dim3(blocks), 256, 0, strm(st), *p, from, lim, scratch, err);
+    const int shift = p->nseq > 256 ? 3 : 5;   // a sector or four of each table a block; 196 KB of shared memory at most
+    const size_t smem = (size_t) p->nseq * ((1 << shift) + 4) * 4;
+    if (smem > 32 * 1024 && smem_optin(k_pages_fork, (size_t) PG_SEQS * 12 * 4, "pages_fork")) return 1;   // (one size for all calls: they may come from several threads)
+    launch(0, k_pages_fork, dim3((p->pt_stride + (1 << shift) - 1) >> shift), 256, smem, strm(st), *p, from, lim, shift, scratch, err);
     return launch_ok("pages_fork");
 }
 
@@ -375,11 +436,11 @@ int fnx_pages_reserve(const FnxPagePool* p, const int* add, int* pos0, int* row0
                       void* scratch, unsigned* err, void* st) {
     if (pg_check(p, scratch, err, "pages_reserve") || pg_check_planes(p, planes, nplanes, g, nkv, hd, "pages_reserve")) return 1;
     FNX_REQUIRE(add && pos0 && row0, "pages_reserve: a null buffer");
-    launch(0, k_pages_reserve, dim3(1), PG_THREADS, 0, strm(st), *p, add, pos0, row0, scratch, err);
-    if (launch_ok("pages_reserve")) return 1;
     const PgRows r = pg_rows(*p, g, nkv, hd);
     const unsigned pieces = (unsigned) ((p->rows * r.row_bytes + PG_PIECE - 1) / PG_PIECE);
     FNX_REQUIRE(pieces <= 65535, "pages_reserve: a page of %zu bytes", p->rows * r.row_bytes);
+    launch(0, k_pages_reserve, dim3(1), PG_THREADS, 0, strm(st), *p, add, pos0, row0, scratch, err);
+    if (launch_ok("pages_reserve")) return 1;
     launch(0, k_pages_copy, dim3(std::min(p->nseq, 64), nplanes, pieces), 256, 0, strm(st), *p, planes, r, scratch);
     return launch_ok("pages_reserve (copies)");
 }
@@ -389,7 +450,7 @@ int fnx_pages_keep(const FnxPagePool* p, const int* pos0, const int* keep, int k
     if (pg_check(p, scratch, err, "pages_keep") || pg_check_planes(p, planes, nplanes, g, nkv, hd, "pages_keep")) return 1;
     FNX_REQUIRE(pos0 && keep && nkeep && keep_stride >= 1, "pages_keep: a null buffer, or lists of %d", keep_stride);
     const PgRows r = pg_rows(*p, g, nkv, hd);
-    launch(0, k_pages_keep, dim3(p->nseq, nplanes), 128, 0, strm(st), *p, pos0, keep, keep_stride, nkeep, planes, r, scratch, err);
+    launch(0, k_pages_keep, dim3(p->nseq, nplanes), PK_THREADS, 0, strm(st), *p, pos0, keep, keep_stride, nkeep, planes, r, scratch, err);
     if (launch_ok("pages_keep")) return 1;
     launch(0, k_pages_trim, dim3(p->nseq), 128, 0, strm(st), *p, scratch);
     return launch_ok("pages_keep (lengths)");
