@@ -24,6 +24,32 @@ def ancestors(parent, words):
     return bits, depth
 
 
+def formula(q, k, v, seen):
+    """(output, how far an f16 result may be off) in 64 bits, [rows][nq][hd], of q [rows][nq][hd] over k, v [positions][nkv][hd].
+
+    A score is a sum of hd products in 32 bits: off by at most hd 2^-24 sum |q k| / sqrt(hd), call it d; e^x by twice that
+    and 2^-20 for the exponential itself.  A weight is then rounded to f16: 2^-11 of itself, or 2^-25 where it is below
+    2^-14, against a sum z of at least the exact one about the row's maximum.  The sum over the positions in 32 bits adds no
+    more than 2^-20 of the sum of magnitudes (tiles of at most 256 terms, then one addition a tile: under 16 halvings
+    of 2^-24 each for what the tests reach); the gated result is rounded to f16 once."""
+    out, tol = torch.zeros_like(q), torch.zeros_like(q)
+    hd, qpk = q.shape[2], q.shape[1] // k.shape[1]
+    for h in range(q.shape[1]):
+        kh, vh = k[:, h // qpk], v[:, h // qpk]
+        w = q[:, h] @ kh.T / np.sqrt(hd)
+        d = float((q[:, h].abs() @ kh.abs().T).max()) / np.sqrt(hd) * hd * 2.0 ** -24
+        w = w.masked_fill(~seen, -torch.inf)
+        top = w.amax(1, keepdim=True)
+        e = torch.where(seen, torch.exp(w - torch.where(torch.isinf(top), 0.0, top)), 0.0)
+        z = e.sum(1, keepdim=True)
+        p = torch.where(z > 0, e / z, 0.0)
+        o, mag = p @ vh, p @ vh.abs()
+        small = torch.where(z > 0, 2.0 ** -25 * (seen.double() @ vh.abs()) / z, 0.0)
+        out[:, h] = o
+        tol[:, h] = 2.0 ** -11 * o.abs() + (2.0 ** -11 + 2 * d + 2.0 ** -19) * mag + small + 2.0 ** -25
+    return out, tol
+
+
 class Seqs:
     """lens new rows after ctx positions a sequence; page: rows a page (0: one contiguous cache)."""
 
@@ -121,16 +147,9 @@ class Seqs:
         return out
 
     def reference(self, bits=None, gate=True):
-        """(output, how far an f16 result may be off) in 64 bits, [rows][nq][hd].
-
-        A score is a sum of hd products in 32 bits: off by at most hd 2^-24 sum |q k| / sqrt(hd), call it d; e^x by twice that
-        and 2^-20 for the exponential itself.  A weight is then rounded to f16: 2^-11 of itself, or 2^-25 where it is below
-        2^-14, against a sum z of at least the exact one about the row's maximum.  The sum over the positions in 32 bits adds no
-        more than 2^-20 of the sum of magnitudes (tiles of at most 256 terms, then one addition a tile: under 16 halvings
-        of 2^-24 each for what the tests reach); the gated result is rounded to f16 once."""
+        """formula() of every sequence's rows, gated: (output, how far an f16 result may be off), [rows][nq][hd]."""
         out = torch.zeros(self.rows, self.nq, self.hd, dtype=torch.float64, device=DEV)
         tol = torch.zeros_like(out)
-        qpk = self.nq // self.nkv
         for s in range(self.n):
             m, x = self.lens[s], self.ctx[s]
             if not m:
@@ -144,19 +163,7 @@ class Seqs:
             else:
                 b = bits[r]
                 seen[:, x:] = torch.tensor([[bool(i // 32 < b.shape[1] and b[t, i // 32] >> np.uint32(i % 32) & 1) for i in range(m)] for t in range(m)], device=DEV)
-            for h in range(self.nq):
-                k, v = self.k[c, h // qpk].double(), self.v[c, h // qpk].double()
-                w = q[:, h] @ k.T / np.sqrt(self.hd)
-                d = float((q[:, h].abs() @ k.abs().T).max()) / np.sqrt(self.hd) * self.hd * 2.0 ** -24
-                w = w.masked_fill(~seen, -torch.inf)
-                top = w.amax(1, keepdim=True)
-                e = torch.where(seen, torch.exp(w - torch.where(torch.isinf(top), 0.0, top)), 0.0)
-                z = e.sum(1, keepdim=True)
-                p = torch.where(z > 0, e / z, 0.0)
-                o, mag = p @ v, p @ v.abs()
-                small = torch.where(z > 0, 2.0 ** -25 * (seen.double() @ v.abs()) / z, 0.0)
-                out[r, h] = o
-                tol[r, h] = 2.0 ** -11 * o.abs() + (2.0 ** -11 + 2 * d + 2.0 ** -19) * mag + small + 2.0 ** -25
+            out[r], tol[r] = formula(q, self.k[c].double(), self.v[c].double(), seen)
         if gate:
             sig = torch.sigmoid(self.qg[:self.rows, :, self.hd:].double())
             out, tol = out * sig, tol * sig + 2.0 ** -25
