@@ -298,8 +298,8 @@ typedef struct FnxSeqs {
     const int* pt;   /* device [nseq][pt_stride]: its page table (FnxKvPages.pt is not used); null: the cache is contiguous */
     int pt_stride, npages; /* entries a table has; pages the pool has */
     const int* kv0;  /* pt null: device [nseq], the cache row of its position 0 (null: 0), the cache of FnxKvPages.cap rows */
-    int max_pos;     /* no sequence ends past this position after the call (0: the tables' capacity); it decides how many
-                      * blocks share a sequence's positions, not what is computed */
+    int max_pos;     /* no sequence ends past this position after the call (0: unknown); a short call starts fewer blocks for
+                      * it, what is computed does not depend on it */
 } FnxSeqs;
 /* fnx_attn_prep_append for many rows: row t of sequence s, position p = pos0[s] + t - row0[s], is appended at p with the
  * bits that call gives its K and V rows; with `depth` (device [rows]) the row is rotated as position pos0[s] + depth[t]
@@ -319,9 +319,9 @@ int fnx_tree_masks(const int* parent, const FnxSeqs* sq, unsigned* anc, int anc_
  *   fnx_attn_tree:   row t sees the positions before pos0[s] and, of its sequence's rows, those whose bit is set in anc[t].
  * qg not null: the result times sigmoid(gate), gate the second half of each head of qg [rows][nq][2 hd], as fnx_attn_finish.
  * q_stride, out_stride: halves from a row to the next (multiples of 8, at least nq hd).  A row that sees nothing gives
- * zeros.  Table entries that name no page of the pool count as rows of zeros.  scratch: fnx_attn_seqs_scratch_bytes bytes
- * for these sequences (rows, nseq, max_pos, pt_stride), never read before written; calls that overlap need one each.
- * Pages hold a multiple of 8 rows. */
+ * zeros.  Table entries that name no page of the pool count as rows of zeros.  out overlaps none of the inputs.  scratch:
+ * fnx_attn_seqs_scratch_bytes bytes (39 MB at hd 256, whatever the sequences), never read before written; calls that overlap
+ * need one each.  Pages hold a multiple of 8 rows. */
 size_t fnx_attn_seqs_scratch_bytes(const FnxSeqs* sq, int nq, int nkv, int hd);
 int fnx_attn_prompt(const uint16_t* q16, int q_stride, const float* qg, const uint16_t* kc, const uint16_t* vc, FnxKvPages g, const FnxSeqs* sq,
                     uint16_t* out, int out_stride, int nq, int nkv, int hd, void* scratch, void* st);

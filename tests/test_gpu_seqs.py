@@ -174,6 +174,25 @@ def test_tree_masks_that_leave_rows_empty():
     _check(s, out, bits)
 
 
+@pytest.mark.parametrize("tree", [False, True])
+def test_attention_of_a_thousand_sequences(tree):
+    """More sequences than a warp has lanes, most of them empty, some long; runs of work begin and end anywhere among them."""
+    rng = np.random.default_rng(21)
+    lens = [int(rng.integers(1, 9)) if rng.random() < 0.15 else 0 for _ in range(1000)]
+    lens[3], lens[40], lens[999] = 64, 50, 3
+    ctx = [int(rng.integers(0, 40)) if n and rng.random() < 0.9 else 0 for n in lens]
+    ctx[40], ctx[999] = 2500, 700
+    s = S.Seqs(lens, ctx, 8, 2, 128, page=16, seed=21, extra_rows=5)
+    bits = s.tree(2)[1] if tree else None
+    _check(s, s.attend(None if bits is None else torch.from_numpy(bits.view(np.int32)).to(DEV)), bits)
+
+
+@pytest.mark.parametrize("lens,ctx", [([1500], [0]), ([0, 1, 1029, 0, 257, 255, 256], [0, 5, 0, 77, 3, 1, 0]), ([640, 1], [333, 12000])])
+def test_prompt_attention_long_and_ragged(lens, ctx):
+    s = S.Seqs(lens, ctx, 8, 2, 128, seed=31, extra_rows=2)
+    _check(s, s.attend())
+
+
 @pytest.mark.parametrize("scale", [0.0, 40.0])
 @pytest.mark.parametrize("lens,ctx", [([300], [0]), ([3, 1], [4000, 900])])
 def test_prompt_attention_flat_and_sharp_scores(lens, ctx, scale):
