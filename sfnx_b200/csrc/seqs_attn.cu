@@ -41,11 +41,11 @@
 namespace fnxk {
 
 constexpr int SA_ROWS = 128, SA_KT = 128, SA_THREADS = 384, SA_SOFT = 256, SA_STRIP = 4096;
-// Of a thread's 32 pairs of exponentials a tile, those by polynomial: 1000 rows after 31 000 positions 612 us with 0, 594 with 8, 612 with
-// 12, 620 with 16
+// Of a thread's 32 pairs of exponentials a tile, those by polynomial: 1000 rows after 31 000 positions 600 us with 0, 593 with 8, 606
+// with 12
 constexpr int SA_POLY = 8;
 // What a unit's beginning and end cost, in positions (the dealing of the work): a prompt of 8192 tokens, whose first units are short,
-// 782 us with 512, 655 with 768, 649 with 1024; the packed short prompts 37.5, 35.3, 40.8
+// 692 us with 640, 647 with 768, 647 with 896; eight packed short prompts 33.0, 32.8, 33.4
 constexpr int SA_COST = 768;
 constexpr int SA_LEAST = 256;   // work a pair gets at least, in positions
 template <int HD> struct SaShape {
@@ -90,9 +90,11 @@ __device__ __forceinline__ void sa_tell_shared(unsigned long long* bar) {
 __device__ __forceinline__ void sa_tell(unsigned long long* bar) {
     asm volatile("{\n\t.reg .b32 r;\n\tmapa.shared::cluster.u32 r, %0, 0;\n\tmbarrier.arrive.shared::cluster.b64 _, [r];\n\t}" ::"r"(um_s32(bar)) : "memory");
 }
-__device__ __forceinline__ void sa_cluster() {   // both CTAs of the pair, every thread
+// both CTAs of the pair, every thread.  Without a release (1000 cycles): before it come the barriers' own fence and a barrier of the
+// CTA for what that shares, or nothing that the other one reads
+__device__ __forceinline__ void sa_cluster() {
     __syncwarp();
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 __device__ __forceinline__ void sa_tma4d(unsigned dst, const CUtensorMap* map, int x, int y, int z, int w, unsigned long long* bar) {
     asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst), "l"(map),
@@ -397,6 +399,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(SA_THREADS, 1) k_att
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
     }
     sa_before();
+    __syncthreads();
     sa_cluster();   // barriers and tensor memory of both CTAs are there
     sa_after();
     const unsigned tm = um_uniform(*tmem_at);
@@ -639,13 +642,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(SA_THREADS, 1) k_att
             }
             ++nseg;
         }
-        // nothing is under way when the blocks end, also after a wait that ran out
+        // nothing is under way when the blocks end, also after a wait that ran out: neither MMAs nor arrivals from the other CTA
         if (um_elect()) {
             sa_commit(idle);
+            if (j && alive) sa_wait(s_free, (unsigned) (j - 1) & 1u, spins, a.fault), sa_wait(o_free, (unsigned) (nseg - 1) & 1u, spins, a.fault);
             spins = SA_SPINS;
             sa_wait(idle, 0u, spins, a.fault);
         }
         __syncwarp();
+    } else if (warp == 1) {
+        sa_wait_warp(idle, 0u, spins, a.fault);   // the last MMAs' arrivals here
     }
     leave();
     } else {
@@ -659,6 +665,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(SA_THREADS, 1) k_att
         int j = 0;   // tiles
         SqRun r;
         r.get(run_at);
+        auto agree = [&]() { asm volatile("bar.sync 1, %0;" ::"n"(SA_SOFT) : "memory"); };   // the rows' halves
         auto wait = [&](unsigned long long* bar, unsigned parity) {
             if (um_elect()) sa_wait(bar, parity, spins, a.fault);
             __syncwarp();
@@ -668,6 +675,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(SA_THREADS, 1) k_att
             const SqUnit& u = r.u;
             const int tok0 = u.tok0 + rank * a.tok, first_row = u.r0 + tok0;   // this CTA's
             const bool real = token < a.tok && tok0 + token < u.len;
+            // a warp without rows only keeps step; P and O stay as they lie there and reach no other rows.  (Twelve single tokens: 115
+            // us with all warps at work, 108 so; a prompt of 8192 tokens 647 and 635, short ones 32.1 and 32.8)
+            if (tok0 + ((warp & 3) * 32) / qpk >= u.len) {
+                for (int i = 0; i < r.n; ++i, ++j) {
+                    wait(s_full, (unsigned) j & 1u);   // (the scores were issued behind p_full of two tiles before: no phase is met twice)
+                    if (lane == 0) sa_tell(s_free), sa_tell(&p_full[j & 1]);
+                    agree();
+                }
+                agree(); agree();
+                if (r.n) wait(&o_full[(j - 1) & 1], (unsigned) ((j - 1) >> 1) & 1u);
+                if (r.n && lane == 0) sa_tell(o_free);
+                continue;
+            }
             if (a.qg && !r.cut && real)   // the gate will be wanted
                 for (int i = half * (HD / 2); i < (half + 1) * (HD / 2); i += 32)
                     l2_ask(a.qg + ((size_t) (first_row + token) * a.nq + u.head * qpk + hh) * 2 * HD + HD + i);
@@ -702,7 +722,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(SA_THREADS, 1) k_att
                 float mx = fmaxf(fmaxf(mq[0], mq[1]), fmaxf(mq[2], mq[3]));
                 float* xm = xmax + (j & 1) * 2 * SA_ROWS;
                 xm[half * SA_ROWS + m] = mx;
-                asm volatile("bar.sync 1, %0;" ::"n"(SA_SOFT) : "memory");
+                agree();
                 mx = fmaxf(mx, xm[(half ^ 1) * SA_ROWS + m]) * scale;
                 const bool up = real && (mx > ref + 8.0f || (ref == -INFINITY && mx != -INFINITY));   // (other rows hold what was there before)
                 if (__any_sync(0xffffffffu, up)) {
@@ -747,9 +767,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(SA_THREADS, 1) k_att
             // ---- the rows' results: through the warp's strip, so that a line of 32 columns leaves (and its gates come) whole
             float* xm = xmax + (j & 1) * 2 * SA_ROWS;   // the last tile's are in the other half
             xm[half * SA_ROWS + m] = z;
-            asm volatile("bar.sync 1, %0;" ::"n"(SA_SOFT) : "memory");
+            agree();
             z += xm[(half ^ 1) * SA_ROWS + m];
-            asm volatile("bar.sync 1, %0;" ::"n"(SA_SOFT) : "memory");   // (a segment without tiles would write there again)
+            agree();   // (a segment without tiles would write there again)
             const bool none = ref == -INFINITY;   // the row saw nothing
             const float inv = none ? 0.f : 1.0f / z;
             const size_t slot = (size_t) (2 * g + (r.first ? 0 : 1)) * 2 + rank;   // of the parts
@@ -821,12 +841,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(SA_THREADS, 1) k_att
 }
 
 // The parts of units that were cut, joined: where a pair's run ends, a block takes 32 rows of the unit that it cut, a warp eight of
-// their columns, a lane a row, as the parts lie; four parts' loads are in flight together.
-constexpr int SJ_PARTS = 4;
+// their columns, a lane a row, as the parts lie; four parts' loads are in flight together.  With fewer units than runs there are blocks
+// for the units only, which look their run up (a tree of 16 after 3000 positions: 17.3 us with blocks for all runs, 16.6 so).
+constexpr int SJ_PARTS = 4, SJ_PAIRS = 128;
 template <int HD> __global__ void __launch_bounds__(256, 3) k_attn_seqs_join(const __grid_constant__ SqAttn a) {
-    const int g = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rank = blockIdx.y >> 2, quarter = blockIdx.y & 3;   // CTA of the pair, quarter of its rows
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rank = blockIdx.y >> 2, quarter = blockIdx.y & 3;   // CTA of the pair, quarter of its rows
     pdl_wait();
     pdl_go();
+    int g = blockIdx.x;
+    if ((int) gridDim.x < a.pairs - 1) {   // fewer units than runs: the x-th that is cut
+        int count[SJ_PAIRS / 32], which = g;
+        g = a.pairs - 1;   // (nothing is cut at the last run's end)
+#pragma unroll
+        for (int k = 0; k < SJ_PAIRS / 32; ++k) count[k] = k * 32 + lane < a.pairs ? a.cuts[2 * (k * 32 + lane)].x : 0;
+#pragma unroll
+        for (int k = 0; k < SJ_PAIRS / 32; ++k) {
+            const unsigned some = __ballot_sync(0xffffffffu, count[k] != 0);
+            const unsigned it = __ballot_sync(0xffffffffu, count[k] != 0 && __popc(some & ((1u << lane) - 1u)) == which);
+            if (it) g = k * 32 + __ffs(it) - 1;
+            which -= __popc(some);
+        }
+    }
     const int4 x = a.cuts[2 * g];
     const int qpk = a.nq / a.nkv, m = quarter * 32 + lane, rows = min(a.tok, x.w - rank * a.tok) * qpk, n = x.x;
     if (!n || m >= rows) return;
@@ -892,13 +927,15 @@ static int sq_processors() {   // multiprocessors of the current device
     return n[dev];
 }
 
-template <int HD> static int sq_launch(const SqMaps& maps, const SqAttn& a, const char* what, cudaStream_t st) {
+template <int HD> static int sq_launch(const SqMaps& maps, const SqAttn& a, long long units, const char* what, cudaStream_t st) {
     if (cudaFuncSetAttribute(k_attn_seqs<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) SaShape<HD>::SMEM) != cudaSuccess)
         return fail("%s: shared memory opt-in: %s", what, cudaGetErrorString(cudaGetLastError()));
     launch(0, k_attn_seqs<HD>, dim3(2 * a.pairs), SA_THREADS, SaShape<HD>::SMEM, st, maps, a);
     if (launch_ok(what)) return 1;
     if (a.pairs == 1) return 0;
-    launch(0, k_attn_seqs_join<HD>, dim3(a.pairs - 1, 8, HD / 64), 256, 0, st, a);
+    const int qpk = a.nq / a.nkv, most = std::min(a.sq.rows, 2 * a.tok);   // tokens of a unit
+    const int quarters = most > a.tok ? 4 + ((most - a.tok) * qpk + 31) / 32 : (most * qpk + 31) / 32;
+    launch(0, k_attn_seqs_join<HD>, dim3((unsigned) std::min<long long>(a.pairs - 1, units), quarters, HD / 64), 256, 0, st, a);
     return launch_ok(what);
 }
 
@@ -934,11 +971,11 @@ static int attn_seqs(const uint16_t* q16, int q_stride, const float* qg, const u
                 "%s: no tensor map for %d rows %d apart or %d pages of %zu halves", what, sq->rows, q_stride, sq->npages, g.page);
     // no more pairs than there can be work for
     const long long units = sq_units(sq, tok, nkv), most = sq->max_pos ? units * (sq->max_pos + SA_COST) : 1ll << 60;
-    const int pairs = (int) std::max(1ll, std::min((long long) sq_processors() / 2, (most + SA_LEAST - 1) / SA_LEAST));
+    const int pairs = (int) std::max(1ll, std::min((long long) std::min(sq_processors() / 2, SJ_PAIRS), (most + SA_LEAST - 1) / SA_LEAST));
     float4* part = (float4*) scratch;
     float2* mz = reinterpret_cast<float2*>(part + (size_t) 4 * pairs * SA_ROWS * (hd / 4));
     const SqAttn a{qg, g, *sq, anc, out, out_stride, nq, nkv, words, tok, box, pairs, part, mz, reinterpret_cast<int4*>(mz + (size_t) 4 * pairs * SA_ROWS), fault};
-    return hd == 256 ? sq_launch<256>(maps, a, what, strm(st)) : sq_launch<128>(maps, a, what, strm(st));
+    return hd == 256 ? sq_launch<256>(maps, a, units, what, strm(st)) : sq_launch<128>(maps, a, units, what, strm(st));
 }
 
 }  // namespace fnxk
@@ -949,7 +986,7 @@ extern "C" {
 
 size_t fnx_attn_seqs_scratch_bytes(const FnxSeqs* sq, int nq, int nkv, int hd) {
     if (!sq || nq < 1 || nkv < 1 || hd < 1) return 0;
-    const size_t pairs = (size_t) std::max(1, sq_processors() / 2);
+    const size_t pairs = (size_t) std::max(1, std::min(sq_processors() / 2, SJ_PAIRS));
     return pairs * (4 * SA_ROWS * (hd + 2) * 4 + 2 * sizeof(int4));
 }
 
