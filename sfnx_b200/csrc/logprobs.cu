@@ -101,42 +101,33 @@ template <int N> __device__ __forceinline__ unsigned long long lp_bound(const un
 
 struct LpShared {
     unsigned long long list[LP_WARPS][LP_LIST];
-    unsigned long long best[LP_THREADS];   // the threads' maxima; then the entries that are placed
+    alignas(16) unsigned long long best[LP_THREADS >> 2];   // groups' maxima
     float r[LP_WARPS], z[LP_WARPS], s[LP_WARPS];
     unsigned long long bound;
     unsigned n, last;
     float lse;
 };
 
-// A bound that at least k of the threads' maxima reach (0 where fewer have any).  Few: the k-th largest of the warps' maxima (0 where
-// fewer warps have any); else bisection over the threads' by one warp
+// A bound that at least k of the threads' entries reach (0 where there are too few): the k-th largest of the maxima of groups of
+// threads, 12 groups, 48 or 96.  Their ranks are counted, which has no steps that wait for one another: a bisection over all
+// threads' maxima took 1 us longer.
 __device__ __forceinline__ unsigned long long lp_block_bound(LpShared& sh, unsigned long long mine, int k) {
-    const int lane = threadIdx.x & 31;
-    if (k <= LP_WARPS) {
-#pragma unroll
-        for (int o = 16; o; o >>= 1) {
-            const unsigned long long x = __shfl_xor_sync(0xffffffffu, mine, o);
-            mine = x > mine ? x : mine;
-        }
-        if (lane == 0) sh.best[threadIdx.x >> 5] = mine;
-        __syncthreads();
-        const unsigned long long own = sh.best[lane % LP_WARPS];
-        int above = 0;
-#pragma unroll
-        for (int i = 0; i < LP_WARPS; ++i) above += sh.best[i] > own;   // (entries are distinct, but for the zeros)
-        const unsigned who = __ballot_sync(0xffffffffu, above == k - 1);
-        const unsigned long long b = who ? sh.best[(__ffs(who) - 1) % LP_WARPS] : 0ull;
-        __syncthreads();   // the next call writes there
-        return b;
+    const int tid = threadIdx.x, shift = k <= LP_WARPS ? 5 : k <= 40 ? 3 : 2, groups = LP_THREADS >> shift;
+    for (int o = 1; o < 1 << shift; o <<= 1) {
+        const unsigned long long x = __shfl_xor_sync(0xffffffffu, mine, o);
+        mine = x > mine ? x : mine;
     }
-    sh.best[threadIdx.x] = mine;
+    if (!(tid & ((1 << shift) - 1))) sh.best[tid >> shift] = mine;
     __syncthreads();
-    if (threadIdx.x < 32) {
-        unsigned long long e[LP_WARPS];
-#pragma unroll
-        for (int i = 0; i < LP_WARPS; ++i) e[i] = sh.best[i * 32 + threadIdx.x];
-        const unsigned long long b = lp_bound(e, k, 2 + k / 8);
-        if (threadIdx.x == 0) sh.bound = b;
+    if (tid < groups) {
+        const unsigned long long own = sh.best[tid];
+        int above = 0;
+#pragma unroll 4
+        for (int i = 0; i < groups; i += 2) {
+            const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(&sh.best[i]);
+            above += x.x > own, above += x.y > own;
+        }
+        if (above == k - 1 || (!own && above < k)) sh.bound = own;   // (entries are distinct, but for the zeros)
     }
     __syncthreads();
     return sh.bound;
@@ -150,7 +141,6 @@ template <int N, typename F> __device__ __forceinline__ void lp_best(LpShared& s
     for (int i = 0; i < N; ++i) most = e[i] > most ? e[i] : most;
     if (tid == 0) sh.n = 0u;
     const unsigned long long b = lp_block_bound(sh, most, k);
-    // k + 2 + k / 8 threads at most have entries above the bound, and fewer than k have any where there is none
     unsigned long long* all = &sh.list[0][0];   // (the lists are in registers)
 #pragma unroll
     for (int i = 0; i < N; ++i)
@@ -169,9 +159,9 @@ struct LpItem {   // a block's part of a row
     const float* base;   // positions are counted from the 16-byte boundary at or before the row's first logit
     int row, split, shift, lo, hi;
 };
-__device__ __forceinline__ LpItem lp_item(const LpArgs& a, long long w) {
+__device__ __forceinline__ LpItem lp_item(const LpArgs& a, unsigned w) {   // (rows in several parts are few: w is below 2^31)
     LpItem t;
-    t.row = (int) (w / a.nsplit), t.split = (int) (w % a.nsplit);
+    t.row = (int) (w / (unsigned) a.nsplit), t.split = (int) (w - (unsigned) t.row * (unsigned) a.nsplit);
     const float* x = a.logits + (size_t) t.row * a.stride;
     t.shift = (int) (((uintptr_t) x >> 2) & 3u), t.base = x - t.shift;
     const int end = a.n + t.shift, batches = (end + LP_BATCH - 1) / LP_BATCH, per = (batches + a.nsplit - 1) / a.nsplit;
@@ -212,12 +202,12 @@ __global__ void __launch_bounds__(LP_THREADS, 2) k_logprobs(const LpArgs a) {
     pdl_wait();
     pdl_go();
     const float L2E = 1.44269504f;
-    const long long items = (long long) a.rows * a.nsplit;
+    const unsigned items = (unsigned) a.rows * (unsigned) a.nsplit;
     LpItem next = lp_item(a, blockIdx.x);
     int stage = 0;
 #pragma unroll
     for (int i = 0; i < LP_STAGES - 1; ++i) load(next, next.lo + i * LP_BATCH, slot(i));
-    for (long long w = blockIdx.x; w < items; w += gridDim.x) {
+    for (unsigned w = blockIdx.x; w < items; w += gridDim.x) {
         const LpItem t = next;
         float r = -INFINITY, bound_v = -INFINITY;                        // r: the reference, in units of log2
         float2 z2 = make_float2(0.f, 0.f), s2 = make_float2(0.f, 0.f);   // the sums of the even and the odd values
