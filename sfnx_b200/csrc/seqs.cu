@@ -1,10 +1,12 @@
 // The rows of several sequences on their way into the cache: per-head RMS norm, rotary and K/V append for any number of rows
 // (prompts, windows, draft trees), and a draft tree's ancestor masks and depths.  The norm and the rotation are
 // fnx_attn_prep_append's (reference src/kernels.cu:1539-1569), with its order of every sum, so a cache may be filled by either.
+#include <algorithm>
 #include <climits>
 #include <cmath>
 
 #include "exact_math.cuh"
+#include "moe_internal.cuh"
 #include "seqs.cuh"
 
 namespace fnxk {
@@ -40,10 +42,12 @@ __global__ void __launch_bounds__(TM_THREADS) k_tree_masks(const int* __restrict
 }
 
 // ---------------------------------------------------------------- append
-// A block per row, a warp per head at a time (four heads' loads in flight): a lane holds E neighbouring elements of its head.  The
-// angles' sines and cosines (double precision) are made once a row for all heads.  A row's queries and K/V are read in f32 and
-// written in f16 (40 us of copying at 5301 rows of 24 + 2 * 4 heads of 256); a block's own chain of dependent loads and the angles
-// bound it before DRAM does, so the loads come first and four blocks lie on a processor: 64.5 us (4.1 TB/s), with three 71.7.
+// A block has a run of neighbouring rows, a warp four heads of a row at a time.  A row's queries and K/V are read in f32 and written in
+// f16, 40 us of copying at 5301 rows of 24 + 2 * 4 heads of 256; what stands in the way is the chain before a row can be written (its
+// sequence, its page, its angles in double precision) and what a head costs in shuffles.  So the next row's heads are on their way
+// into shared memory while one is worked on, eight rows' places and angles are made at once, a warp a row, and a lane's elements
+// lie as they are read without conflicts: 52.2 us (5.0 TB/s).  With a block a row, the loads in registers, 62.2; with three blocks a
+// multiprocessor 53.0, with three rows' copies under way 57.8.
 struct SaArgs {
     const float *qg, *k, *v, *qn, *kn;
     uint16_t *kc, *vc, *q16;
@@ -55,148 +59,188 @@ struct SaArgs {
     int nq, nkv, nrot;
     float freq[64];   // of pair i, base^(-2 i / nrot), computed by the host's powf
 };
-constexpr int SA_THREADS = 256, SA_WARPS = SA_THREADS / 32, SA_HEADS = 4;
+constexpr int SA_THREADS = 256, SA_WARPS = SA_THREADS / 32, SA_HEADS = 4, SA_BLOCKS = 2;   // (the last: a multiprocessor's)
 
-template <int E> struct SaVec {
-    float x[E];
-};
-template <int E> __device__ __forceinline__ SaVec<E> sa_load(const float* p) {
-    SaVec<E> r;
-#pragma unroll
-    for (int i = 0; i < E; i += 4) {
-        const float4 f = *reinterpret_cast<const float4*>(p + i);
-        r.x[i] = f.x, r.x[i + 1] = f.y, r.x[i + 2] = f.z, r.x[i + 3] = f.w;
-    }
-    return r;
-}
-template <int E> __device__ __forceinline__ void sa_store(uint16_t* p, const SaVec<E>& r) {
-    unsigned u[E / 2];
-#pragma unroll
-    for (int i = 0; i < E; i += 2) u[i / 2] = (unsigned) f2h(r.x[i]) | ((unsigned) f2h(r.x[i + 1]) << 16);
-    if (E == 8) *reinterpret_cast<uint4*>(p) = make_uint4(u[0], u[1], u[E / 2 - 2], u[E / 2 - 1]);
-    else *reinterpret_cast<uint2*>(p) = make_uint2(u[0], u[1]);
-}
-
-// The sum of 32 neighbouring values (E a lane) as the xor-tree over a warp forms it, offsets 16 .. 1: at each of the first steps a
-// lane keeps the half of its values that its partner does not, so nobody adds what another adds.  Every lane gets the sum.
+// A lane has elements 4 lane .. + 3 of a head's first 128, and of its second.  The sums of 32 neighbouring values as the xor-tree over
+// a warp forms them, offsets 16 .. 1: at each step lanes share the work out, so nobody adds what another adds.  Lanes 8 g .. + 7
+// get the sum of the first 128's 32 from 32 g on; with E = 8 only the first four of them, and the last four the second 128's.
 template <int E> __device__ __forceinline__ float sa_tree(const float* q, int lane) {
-    if constexpr (E == 8) {   // offset 16: lane ^ 2, 8: lane ^ 1, 4 .. 1: within a lane at first
-        const bool hi = lane & 2, odd = lane & 1;
+    const bool b2 = lane & 4, b1 = lane & 2, b0 = lane & 1;
+    auto add = [](float own, float give, int mask) { return fadd(own, __shfl_xor_sync(0xffffffffu, give, mask)); };
+    if constexpr (E == 8) {
         float a[4], b[2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) a[i] = fadd(hi ? q[4 + i] : q[i], __shfl_xor_sync(0xffffffffu, hi ? q[i] : q[4 + i], 2));
+        for (int i = 0; i < 4; ++i) a[i] = add(b2 ? q[4 + i] : q[i], b2 ? q[i] : q[4 + i], 4);           // offset 16
 #pragma unroll
-        for (int i = 0; i < 2; ++i) b[i] = fadd(odd ? a[2 + i] : a[i], __shfl_xor_sync(0xffffffffu, odd ? a[i] : a[2 + i], 1));
-        // b[i]: elements 4 hi + 2 odd + i of offsets 4 and less
-        float c = fadd(hi ? b[1] : b[0], __shfl_xor_sync(0xffffffffu, hi ? b[0] : b[1], 2));   // offset 4; element 2 odd + hi
-        c = fadd(c, __shfl_xor_sync(0xffffffffu, c, 1));                                         // offset 2
-        return fadd(c, __shfl_xor_sync(0xffffffffu, c, 2));                                      // offset 1
-    } else {   // offset 16: lane ^ 4, 8: lane ^ 2, 4: lane ^ 1
-        const bool hi = lane & 4, mid = lane & 2;
+        for (int i = 0; i < 2; ++i) b[i] = add(b1 ? a[2 + i] : a[i], b1 ? a[i] : a[2 + i], 2);           // offset 8
+        float c = add(b0 ? b[1] : b[0], b0 ? b[0] : b[1], 1);                                            // offset 4; element 2 b1 + b0
+        c = add(c, c, 2);                                                                                // offset 2
+        return add(c, c, 1);                                                                             // offset 1
+    } else {
         float a[2];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) a[i] = fadd(hi ? q[2 + i] : q[i], __shfl_xor_sync(0xffffffffu, hi ? q[i] : q[2 + i], 4));
-        float c = fadd(mid ? a[1] : a[0], __shfl_xor_sync(0xffffffffu, mid ? a[0] : a[1], 2));   // offset 8; element 2 hi + mid
-        c = fadd(c, __shfl_xor_sync(0xffffffffu, c, 1));                                         // offset 4
-        c = fadd(c, __shfl_xor_sync(0xffffffffu, c, 4));                                         // offset 2
-        return fadd(c, __shfl_xor_sync(0xffffffffu, c, 2));                                      // offset 1
+        for (int i = 0; i < 2; ++i) a[i] = add(b2 ? q[2 + i] : q[i], b2 ? q[i] : q[2 + i], 4);           // offset 16
+        float c = add(b1 ? a[1] : a[0], b1 ? a[0] : a[1], 2);                                            // offset 8; element 2 b2 + b1
+        c = add(c, c, 1);                                                                                // offset 4
+        c = add(c, c, 4);                                                                                // offset 2
+        return add(c, c, 2);                                                                             // offset 1
     }
+}
+__device__ __forceinline__ void sa_get(float* x, const float* p) {
+    const float4 f = *reinterpret_cast<const float4*>(p);
+    x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
 }
 
 template <int HD>
-__global__ void __launch_bounds__(SA_THREADS, 4) k_seqs_append(const __grid_constant__ SaArgs a) {
-    constexpr int E = HD / 32;
-    __shared__ __align__(16) float sn[64], cs[64], wt[2][HD];
-    __shared__ float rot[SA_WARPS][128];
-    const int t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nh = a.nq + 2 * a.nkv;
+__global__ void __launch_bounds__(SA_THREADS, SA_BLOCKS) k_seqs_append(const __grid_constant__ SaArgs a) {
+    constexpr int E = HD / 32, CHUNK = SA_HEADS * SA_WARPS;
+    extern __shared__ __align__(16) unsigned char sa_ring[];   // [2][SA_HEADS][SA_WARPS][HD] floats: a warp's own heads
+    __shared__ __align__(16) float sn[SA_WARPS][64], cs[SA_WARPS][64], wt[2][HD];
+    __shared__ __align__(16) float sums[SA_WARPS][SA_HEADS][E];
+    __shared__ long long place[SA_WARPS];   // of the rows prepared together: where K and V go (-1: nowhere, -2: not even a query)
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nh = a.nq + 2 * a.nkv, chunks = (nh + CHUNK - 1) / CHUNK;
+    const int begin = (int) ((long long) a.sq.rows * blockIdx.x / gridDim.x), end = (int) ((long long) a.sq.rows * (blockIdx.x + 1) / gridDim.x);
+    const unsigned ring = (unsigned) __cvta_generic_to_shared(sa_ring) + warp * HD * 4;
+    const size_t row_elems = (size_t) a.nkv * HD;
+    auto load = [&](int t, int chunk, int stage) {   // a row's heads chunk * CHUNK .., whole lines
+        if (t < end) {
+            const float *rq = a.qg + (size_t) t * a.nq * 2 * HD + lane * 4, *rk = a.k + (size_t) t * row_elems + lane * 4, *rv = a.v + (size_t) t * row_elems + lane * 4;
+#pragma unroll
+            for (int b = 0; b < SA_HEADS; ++b) {
+                const int h = chunk * CHUNK + b * SA_WARPS + warp;
+                if (h >= nh) break;
+                const float* src = h < a.nq ? rq + h * 2 * HD : h < a.nq + a.nkv ? rk + (h - a.nq) * HD : rv + (h - a.nq - a.nkv) * HD;
+#pragma unroll
+                for (int e = 0; e < E / 4; ++e)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(ring + ((stage * SA_HEADS + b) * SA_WARPS * HD + e * 128 + lane * 4) * 4), "l"(src + 128 * e)
+                                 : "memory");
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
     pdl_wait();
     pdl_go();
-    const size_t row_elems = (size_t) a.nkv * HD;
-    const float *rq = a.qg + (size_t) t * a.nq * 2 * HD + lane * E, *rk = a.k + (size_t) t * row_elems + lane * E, *rv = a.v + (size_t) t * row_elems + lane * E;
-    auto source = [&](int h) { return h < a.nq ? rq + h * 2 * HD : h < a.nq + a.nkv ? rk + (h - a.nq) * HD : rv + (h - a.nq - a.nkv) * HD; };
-    SaVec<E> x[SA_HEADS];
-    auto ask = [&](int h0) {
-#pragma unroll
-        for (int b = 0; b < SA_HEADS; ++b)
-            if (h0 + b * SA_WARPS < nh) x[b] = sa_load<E>(source(h0 + b * SA_WARPS));
-    };
-    ask(warp);   // on their way while the row's place and angles are worked out
-    const int s = sq_find(a.sq.row0, a.sq.nseq, t);
-    if (s < 0) return;   // behind the last sequence (the whole block agrees)
-    const int i0 = t - a.sq.row0[s], p0 = a.sq.pos0[s];
-    const int turn = max(0, p0) + (a.depth ? max(0, a.depth[t]) : i0);
-    if (threadIdx.x < a.nrot / 2) {
-        const float theta = fmul((float) turn, a.freq[threadIdx.x]);
-        ex_sincos((double) theta, &sn[threadIdx.x], &cs[threadIdx.x]);
-    }
+    load(begin, 0, 0);   // on its way while the rows' places and angles are worked out
     for (int i = threadIdx.x; i < HD; i += SA_THREADS) wt[0][i] = a.qn[i], wt[1][i] = a.kn[i];
-    const long long cell = sq_cell(a.sq, a.g, s, p0 < 0 || i0 > INT_MAX - p0 ? -1 : p0 + i0);
-    if (threadIdx.x == 0 && cell < 0) atomicOr(a.err, SQ_ERR_ROOM);
-    const size_t at = cell < 0 ? 0 : sq_at(a.sq, a.g, cell, row_elems);
-    __syncthreads();
     // element i < nrot pairs with i -+ half: the lower one becomes x c - x' s, the upper one x c + x' s, the first product rounded before the
-    // fused second.  Whole lanes apart (half a multiple of E) the partner comes by a shuffle, else through shared memory
-    const int half = a.nrot / 2, apart = half % E ? 0 : half / E;
-    const bool turned = lane * E < a.nrot, lower = lane * E < half;
-    for (int h0 = warp; h0 < nh; h0 += SA_HEADS * SA_WARPS) {
-        if (h0 != warp) ask(h0);
-        // ---- the heads' square sums, one root for all: lane b takes head b's
-        float mine = 1.f;
-#pragma unroll
-        for (int b = 0; b < SA_HEADS; ++b) {
-            if (h0 + b * SA_WARPS >= a.nq + a.nkv) continue;
-            float q[E];
-#pragma unroll
-            for (int e = 0; e < E; ++e) q[e] = fmul(x[b].x[e], x[b].x[e]);
-            const float group = sa_tree<E>(q, lane);
-            float tot = 0.f;
-#pragma unroll
-            for (int g = 0; g < E; ++g) tot = fadd(tot, __shfl_sync(0xffffffffu, group, g * (32 / E)));
-            mine = lane == b ? tot : mine;
+    // fused second.  Whole lanes apart (half a multiple of 4) the partner comes by a shuffle, else through shared memory
+    const int half = a.nrot / 2, apart = half % 4 ? 0 : half / 4;
+    const bool turned = lane * 4 < a.nrot, lower = lane * 4 < half;
+    int stage = 0;
+    for (int t0 = begin; t0 < end; t0 += SA_WARPS) {
+        if (t0 > begin) __syncthreads();   // everyone is done with the angles before these
+        if (t0 + warp < end) {
+            const int t = t0 + warp, s = sq_find(a.sq.row0, a.sq.nseq, t);
+            long long at = -2;
+            if (s >= 0) {
+                const int i0 = t - a.sq.row0[s], p0 = a.sq.pos0[s];
+                const int turn = max(0, p0) + (a.depth ? max(0, a.depth[t]) : i0);
+                for (int i = lane; i < half; i += 32) ex_sincos((double) fmul((float) turn, a.freq[i]), &sn[warp][i], &cs[warp][i]);
+                const long long cell = sq_cell(a.sq, a.g, s, p0 < 0 || i0 > INT_MAX - p0 ? -1 : p0 + i0);
+                if (lane == 0 && cell < 0) atomicOr(a.err, SQ_ERR_ROOM);
+                at = cell < 0 ? -1 : (long long) sq_at(a.sq, a.g, cell, row_elems);
+            }
+            if (lane == 0) place[warp] = at;
         }
-        mine = ex_rsqrt(fadd(fmul(mine, 1.0f / (float) HD), a.eps));   // (HD is a power of two: the quotient's bits)
+        __syncthreads();
+        for (int t = t0; t < min(t0 + SA_WARPS, end); ++t)
+            for (int chunk = 0; chunk < chunks; ++chunk, stage ^= 1) {
+                __syncwarp();
+                load(chunk + 1 < chunks ? t : t + 1, chunk + 1 < chunks ? chunk + 1 : 0, stage ^ 1);   // (what lay there is in registers and used)
+                asm volatile("cp.async.wait_group 1;" ::: "memory");
+                __syncwarp();
+                const long long at = place[t - t0];
+                if (at == -2) continue;   // behind the last sequence
+                const int h0 = chunk * CHUNK + warp;
+                float x[SA_HEADS][E], c[4], d[4];
+                if (turned && apart) {   // the rotation's factors of this lane's elements and of their partners
+                    const int i = lane * 4 - (lower ? 0 : half);
+                    sa_get(c, lower ? &cs[t - t0][i] : &sn[t - t0][i]), sa_get(d, lower ? &sn[t - t0][i] : &cs[t - t0][i]);
+                }
 #pragma unroll
-        for (int b = 0; b < SA_HEADS; ++b) {
-            const int h = h0 + b * SA_WARPS;
-            if (h >= nh) break;
-            if (h < a.nq + a.nkv) {
-                const float r = __shfl_sync(0xffffffffu, mine, b);
-                const SaVec<E> w = sa_load<E>(&wt[h < a.nq ? 0 : 1][lane * E]);
+                for (int b = 0; b < SA_HEADS; ++b)
 #pragma unroll
-                for (int e = 0; e < E; ++e) x[b].x[e] = fmul(fmul(x[b].x[e], r), w.x[e]);
-                if (apart) {
-                    float other[E];
+                    for (int e = 0; e < E; e += 4)
+                        if (h0 + b * SA_WARPS < nh)
+                            asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                                         : "=f"(x[b][e]), "=f"(x[b][e + 1]), "=f"(x[b][e + 2]), "=f"(x[b][e + 3])
+                                         : "r"(ring + ((stage * SA_HEADS + b) * SA_WARPS * HD + e * 32 + lane * 4) * 4)
+                                         : "memory");
+                float* rot = reinterpret_cast<float*>(sa_ring) + (stage * SA_HEADS * SA_WARPS + warp) * HD;   // (these values are in registers)
+                // ---- the heads' square sums, one root for all: lane b takes head b's
 #pragma unroll
-                    for (int e = 0; e < E; ++e) other[e] = __shfl_sync(0xffffffffu, x[b].x[e], lower ? lane + apart : lane - apart);
-                    if (turned) {
-                        const int i = lane * E - (lower ? 0 : half);
-                        const SaVec<E> c = sa_load<E>(lower ? &cs[i] : &sn[i]), d = sa_load<E>(lower ? &sn[i] : &cs[i]);
+                for (int b = 0; b < SA_HEADS; ++b) {
+                    if (h0 + b * SA_WARPS >= a.nq + a.nkv) continue;
+                    float q[E];
 #pragma unroll
-                        for (int e = 0; e < E; ++e) {
-                            const float y = x[b].x[e];
-                            x[b].x[e] = ffma(lower ? -other[e] : y, d.x[e], fmul(lower ? y : other[e], c.x[e]));
+                    for (int e = 0; e < E; ++e) q[e] = fmul(x[b][e], x[b][e]);
+                    const float group = sa_tree<E>(q, lane);
+                    if (lane % (E == 8 ? 4 : 8) == 0) sums[warp][b][E == 8 ? (lane >> 3) + (lane & 4) : lane >> 3] = group;
+                }
+                __syncwarp();
+                float g[E], tot = 0.f;
+#pragma unroll
+                for (int e = 0; e < E; e += 4) sa_get(g + e, &sums[warp][lane % SA_HEADS][e]);
+#pragma unroll
+                for (int e = 0; e < E; ++e) tot = fadd(tot, g[e]);
+                const float mine = ex_rsqrt(fadd(fmul(tot, 1.0f / (float) HD), a.eps));   // (HD is a power of two: the quotient's bits)
+#pragma unroll
+                for (int b = 0; b < SA_HEADS; ++b) {
+                    const int h = h0 + b * SA_WARPS;
+                    if (h >= nh) break;
+                    if (h < a.nq + a.nkv) {
+                        const float r = __shfl_sync(0xffffffffu, mine, b);
+#pragma unroll
+                        for (int e = 0; e < E; e += 4) {
+                            float w[4];
+                            sa_get(w, &wt[h < a.nq ? 0 : 1][e * 32 + lane * 4]);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) x[b][e + i] = fmul(fmul(x[b][e + i], r), w[i]);
+                        }
+                        if (apart) {
+                            float other[4];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) other[e] = __shfl_sync(0xffffffffu, x[b][e], lower ? lane + apart : lane - apart);
+                            if (turned)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    const float y = x[b][e];
+                                    x[b][e] = ffma(lower ? -other[e] : y, d[e], fmul(lower ? y : other[e], c[e]));
+                                }
+                        } else {
+                            __syncwarp();
+                            if (turned)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) rot[lane * 4 + e] = x[b][e];
+                            __syncwarp();
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const int i = lane * 4 + e;
+                                const float *sr = sn[t - t0], *cr = cs[t - t0];
+                                if (i < half) x[b][e] = ffma(-rot[i + half], sr[i], fmul(x[b][e], cr[i]));
+                                else if (i < a.nrot) x[b][e] = ffma(x[b][e], cr[i - half], fmul(rot[i - half], sr[i - half]));
+                            }
+                            __syncwarp();
                         }
                     }
-                } else {
-                    if (turned)
+                    if (h >= a.nq && at < 0) continue;
+                    uint16_t* to = h < a.nq            ? a.q16 + ((size_t) t * a.nq + h) * HD
+                                   : h < a.nq + a.nkv ? a.kc + at + (h - a.nq) * HD
+                                                      : a.vc + at + (h - a.nq - a.nkv) * HD;
 #pragma unroll
-                        for (int e = 0; e < E; ++e) rot[warp][lane * E + e] = x[b].x[e];
-                    __syncwarp();
-#pragma unroll
-                    for (int e = 0; e < E; ++e) {
-                        const int i = lane * E + e;
-                        if (i < half) x[b].x[e] = ffma(-rot[warp][i + half], sn[i], fmul(x[b].x[e], cs[i]));
-                        else if (i < a.nrot) x[b].x[e] = ffma(x[b].x[e], cs[i - half], fmul(rot[warp][i - half], sn[i - half]));
-                    }
-                    __syncwarp();
+                    for (int e = 0; e < E; e += 4)
+                        *reinterpret_cast<uint2*>(to + e * 32 + lane * 4) = make_uint2(sq_pack(x[b][e], x[b][e + 1]), sq_pack(x[b][e + 2], x[b][e + 3]));
                 }
             }
-            if (h < a.nq) sa_store<E>(a.q16 + ((size_t) t * a.nq + h) * HD + lane * E, x[b]);
-            else if (h < a.nq + a.nkv) {
-                if (cell >= 0) sa_store<E>(a.kc + at + (h - a.nq) * HD + lane * E, x[b]);
-            } else if (cell >= 0) sa_store<E>(a.vc + at + (h - a.nq - a.nkv) * HD + lane * E, x[b]);
-        }
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
+template <int HD> static int sa_launch(const SaArgs& a, void* st) {
+    constexpr size_t ring = (size_t) 2 * SA_HEADS * SA_THREADS * HD / 8;
+    if (smem_optin(k_seqs_append<HD>, ring, "attn_seqs_append")) return 1;
+    launch(0, k_seqs_append<HD>, dim3(std::min(a.sq.rows, SA_BLOCKS * 148)), SA_THREADS, ring, strm(st), a);
+    return launch_ok("attn_seqs_append");
 }
 
 }  // namespace fnxk
@@ -223,8 +267,6 @@ int fnx_attn_seqs_append(const float* qg, const float* k, const float* v, const 
     FNX_REQUIRE(rope.nrot % 2 == 0 && rope.nrot >= 2 && rope.nrot <= 128 && rope.nrot <= hd, "attn_seqs_append: rotary width %d", rope.nrot);
     SaArgs a{qg, k, v, q_norm, k_norm, kc, vc, q16, g, *sq, depth, err, eps, nq, nkv, rope.nrot, {}};
     for (int i = 0; i < rope.nrot / 2; ++i) a.freq[i] = powf(rope.base, -2.0f * (float) i / (float) rope.nrot);
-    if (hd == 256) launch(0, k_seqs_append<256>, dim3(sq->rows), SA_THREADS, 0, strm(st), a);
-    else launch(0, k_seqs_append<128>, dim3(sq->rows), SA_THREADS, 0, strm(st), a);
-    return launch_ok("attn_seqs_append");
+    return hd == 256 ? sa_launch<256>(a, st) : sa_launch<128>(a, st);
 }
 }

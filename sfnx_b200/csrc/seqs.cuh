@@ -42,6 +42,11 @@ __device__ __forceinline__ size_t sq_at(const FnxSeqs& sq, const FnxKvPages& g, 
     return sq.pt ? (size_t) (cell / g.rows) * g.page + (size_t) (cell % g.rows) * row_elems : (size_t) cell * row_elems;
 }
 
+__device__ __forceinline__ unsigned sq_pack(float lo, float hi) {   // both rounded to f16 by one instruction
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const unsigned*>(&h);
+}
+
 inline int sq_check(const FnxSeqs* sq, const FnxKvPages& g, int nq, int nkv, int hd, const char* what) {
     FNX_REQUIRE(sq && sq->row0 && sq->pos0, "%s: a null buffer", what);
     FNX_REQUIRE(sq->nseq >= 1 && sq->rows >= 1, "%s: %d rows of %d sequences", what, sq->rows, sq->nseq);

@@ -831,7 +831,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(SA_THREADS, 1) k_att
                     ask(k, st + 1);
                     if (out_at[k] >= 0)
                         *reinterpret_cast<uint2*>(out + out_at[k] + st * 32) =
-                            make_uint2((unsigned) f2h(y.x) | ((unsigned) f2h(y.y) << 16), (unsigned) f2h(y.z) | ((unsigned) f2h(y.w) << 16));
+                            make_uint2(sq_pack(y.x, y.y), sq_pack(y.z, y.w));
                 }
                 __syncwarp();
             }
@@ -911,7 +911,7 @@ template <int HD> __global__ void __launch_bounds__(256, 3) k_attn_seqs_join(con
     }
     unsigned u[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) u[e] = (unsigned) f2h(acc[2 * e]) | ((unsigned) f2h(acc[2 * e + 1]) << 16);
+    for (int e = 0; e < 4; ++e) u[e] = sq_pack(acc[2 * e], acc[2 * e + 1]);
     *reinterpret_cast<uint4*>(a.out + row * a.out_stride + (size_t) head * HD + c * 8) = make_uint4(u[0], u[1], u[2], u[3]);
 }
 
