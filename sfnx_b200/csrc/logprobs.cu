@@ -6,16 +6,17 @@
 // in double).  The reference is raised - z' = f z, s' = f (s + (R - R') z), f = 2^(R - R') - only when a value exceeds it by more
 // than 8, so a thread rescales once or twice a row and 2^t stays below 2^8.  The centred s keeps H free of the cancellation
 // that sum p x - lse has for large logits.  A NaN or +inf makes z a NaN, which is how the row is found out.
-// The k best: a bound that k values of the row's first batch reach or exceed (the k-th largest or so of the threads'
-// maxima, found by bisection), and of the rest of the row every warp lists what exceeds it, about k / 4096 of the values,
-// without a word to the other warps.  A list that is full (rising logits) is cut to its own k best, which raises that
-// warp's bound.  In the end a bound over the lists' entries leaves little more than k, and an entry's place is the number of
-// larger ones.  Entries are 64-bit composites (the value's order-preserving key, the index's complement), no two equal, so ties go
+// The k best: a bound that k values of the row's first batch reach or exceed (the k-th largest of the maxima of groups of
+// threads), made anew from the lists some batches on, and of the rest of the row every warp lists what exceeds it, a few hundredths of a
+// percent of the values, without a word to the other warps.  A list that is full (rising logits) is cut to its own k best, which
+// raises that warp's bound.  In the end a bound over the lists' entries leaves little more than k, and an entry's place is the number
+// of larger ones.  Entries are 64-bit composites (the value's order-preserving key, the index's complement), no two equal, so ties go
 // to the lower index whatever order they come in.
 // A row goes to one block when there are many, else to as many as the GPU holds at once; the row's last block joins the parts.
 // A pass is bound by DRAM when there are many rows: a thread copies its own values into shared memory three batches ahead
-// (cp.async; nobody else reads them, so no barrier belongs to it), 96 KB in flight a multiprocessor; with one batch ahead in
-// registers 2000 rows took 342 us.  A value costs about seven instructions, most of them two values at a time.
+// (cp.async; nobody else reads them, so no barrier belongs to it), 72 KB in flight a multiprocessor.  2000 rows of 151 936 logits with
+// five alternatives: 230 us (5.3 TB/s); with one batch ahead in registers 342.  16 rows with twenty: 14.4 us, latency - three rounds
+// of choosing the best, the blocks' results through memory to the last one.
 #include <algorithm>
 
 #include "common.cuh"
