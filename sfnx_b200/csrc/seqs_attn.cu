@@ -398,6 +398,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(SA_THREADS, 1) k_att
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(um_s32((const void*) tmem_at)), "r"(512));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
     }
+    if (rank && tid >= SA_THREADS - SA_SOFT) {   // Q, for a first unit without rows here
+        for (int i = tid - (SA_THREADS - SA_SOFT); i < S::QBYTES / 16; i += SA_SOFT) reinterpret_cast<uint4*>(Q)[i] = make_uint4(0u, 0u, 0u, 0u);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
     sa_before();
     __syncthreads();
     sa_cluster();   // barriers and tensor memory of both CTAs are there
@@ -450,6 +454,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(SA_THREADS, 1) k_att
         // ---- copies.  Load number c of the ring takes slot c % SLOTS; tile i's K load comes before tile i - 2's V load.  A slot
         // holds groups of 64 rows, each as column blocks of 64 dims (8 KB, swizzled)
         int c = 0, nseg = 0, kv0 = 0;
+        bool zeroed = true;   // Q
         SqRun r;
         r.get(run_at);
         bool alive = true;
@@ -499,14 +504,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(SA_THREADS, 1) k_att
             int e = entry(r.t0), y0, z0, y1 = 0, z1 = 0, y2 = 0, z2 = 0;
             if (nseg) alive = sa_wait_warp(q_empty, (unsigned) (nseg - 1) & 1u, spins, a.fault);   // the scores before are done
             if (!alive) break;
-            if (um_elect()) {
-                const int tok0 = r.u.tok0 + rank * a.tok;
-                if (tok0 < r.u.len) {
+            const int tok0 = r.u.tok0 + rank * a.tok;
+            if (tok0 < r.u.len) {
+                if (um_elect()) {
                     um_expect_tx(q_full, (unsigned) (a.tok * qpk * HD * 2));
                     for (int b = 0; b < HD / 64; ++b) sa_tma3d(um_s32(Q) + b * (SA_ROWS * 128), &maps.q, b * 64, r.u.head * qpk, r.u.r0 + tok0, q_full);
-                } else {
-                    sa_arrive(q_full);   // no rows of this CTA's
                 }
+                zeroed = false;
+            } else {   // no rows of this CTA's: products with zeros take less power than with what lies there
+                if (!zeroed) {
+                    for (int i = lane; i < S::QBYTES / 16; i += 32) reinterpret_cast<uint4*>(Q)[i] = make_uint4(0u, 0u, 0u, 0u);
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    zeroed = true;
+                }
+                if (um_elect()) sa_arrive(q_full);
             }
             __syncwarp();
             ++nseg;
@@ -663,6 +675,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(SA_THREADS, 1) k_att
         const int inv_qpk = (65536 + qpk - 1) / qpk;   // x / qpk = x inv_qpk >> 16 for x < 128
         unsigned char* strip = strips + (warp - 4) * SA_STRIP;
         int j = 0;   // tiles
+        bool zeroed = false;
         SqRun r;
         r.get(run_at);
         auto agree = [&]() { asm volatile("bar.sync 1, %0;" ::"n"(SA_SOFT) : "memory"); };   // the rows' halves
@@ -675,9 +688,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(SA_THREADS, 1) k_att
             const SqUnit& u = r.u;
             const int tok0 = u.tok0 + rank * a.tok, first_row = u.r0 + tok0;   // this CTA's
             const bool real = token < a.tok && tok0 + token < u.len;
-            // a warp without rows only keeps step; P and O stay as they lie there and reach no other rows.  (Twelve single tokens: 115
-            // us with all warps at work, 108 so; a prompt of 8192 tokens 647 and 635, short ones 32.1 and 32.8)
+            // a warp without rows only keeps step, P zero and O what comes of it: they reach no other rows, and the tensor core takes less
+            // power over zeros.  (Twelve single tokens: 115 us with all warps at work, 109 keeping step, 104 with P and Q zero; a prompt of
+            // 8192 tokens 647 and 635, short ones 32.1 and 32.8)
             if (tok0 + ((warp & 3) * 32) / qpk >= u.len) {
+                if (!zeroed) {   // (nothing reads P between two segments)
+                    unsigned zero[32];
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) zero[k] = 0u;
+                    sa_st32(tl + S::COL_P + half * 32, zero), sa_st32(tl + S::COL_P + SA_KT / 2 + half * 32, zero);
+                    sa_wait_st();
+                    sa_before();
+                    zeroed = true;
+                }
                 for (int i = 0; i < r.n; ++i, ++j) {
                     wait(s_full, (unsigned) j & 1u);   // (the scores were issued behind p_full of two tiles before: no phase is met twice)
                     if (lane == 0) sa_tell(s_free), sa_tell(&p_full[j & 1]);
@@ -688,6 +711,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(SA_THREADS, 1) k_att
                 if (r.n && lane == 0) sa_tell(o_free);
                 continue;
             }
+            zeroed = false;
             if (a.qg && !r.cut && real)   // the gate will be wanted
                 for (int i = half * (HD / 2); i < (half + 1) * (HD / 2); i += 32)
                     l2_ask(a.qg + ((size_t) (first_row + token) * a.nq + u.head * qpk + hh) * 2 * HD + HD + i);
