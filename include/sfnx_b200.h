@@ -319,7 +319,9 @@ int fnx_tree_masks(const int* parent, const FnxSeqs* sq, unsigned* anc, int anc_
  *   fnx_attn_tree:   row t sees the positions before pos0[s] and, of its sequence's rows, those whose bit is set in anc[t].
  * qg not null: the result times sigmoid(gate), gate the second half of each head of qg [rows][nq][2 hd], as fnx_attn_finish.
  * q_stride, out_stride: halves from a row to the next (multiples of 8, at least nq hd).  A row that sees nothing gives
- * zeros.  Table entries that name no page of the pool count as rows of zeros.  out overlaps none of the inputs.  scratch:
+ * zeros; a row that sees a score of NaN or +inf gives NaNs.  K rows that a row does not see may hold anything; V rows are finite up to
+ * a sequence's newest one (a weight of zero times a NaN is a NaN), behind it and between the sequences they may hold anything.
+ * Table entries that name no page of the pool count as rows of zeros.  out overlaps none of the inputs.  scratch:
  * fnx_attn_seqs_scratch_bytes bytes (39 MB at hd 256, whatever the sequences), never read before written; calls that overlap
  * need one each.  Pages hold a multiple of 8 rows. */
 size_t fnx_attn_seqs_scratch_bytes(const FnxSeqs* sq, int nq, int nkv, int hd);
@@ -479,7 +481,8 @@ int fnx_top_tokens(float* logits, int n, int T, int v0, const int* pen_tok, cons
 size_t fnx_logprobs_scratch_bytes(int n, int T, int k);
 int fnx_logprobs(const float* logits, size_t stride, int n, int T, int v0, const int* tok, int ntok, int k, float* lse, float* entropy, float* lp,
                  float* top_lp, int* top_i, void* scratch, unsigned* err, void* st);
-/* the slices' results ([nslice][T]..., host) as those of the whole vocabulary (host): fnx_top_merge's counterpart */
+/* the slices' results ([nslice][T]..., host) as those of the whole vocabulary (host): fnx_top_merge's counterpart.  The slices' values
+ * are log probabilities, so alternatives of two slices whose logits differ by less than their rounding may come in either order */
 int fnx_logprobs_merge(const float* lse_s, const float* entropy_s, const float* lp_s, const float* top_lp_s, const int* top_i_s, int nslice, int T,
                        int ntok, int k, float* lse, float* entropy, float* lp, float* top_lp, int* top_i);
 

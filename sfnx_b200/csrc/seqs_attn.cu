@@ -339,9 +339,16 @@ __device__ __forceinline__ bool sa_test(unsigned long long* bar, unsigned parity
                  : "memory");
     return ok != 0;
 }
+// the larger one, a NaN if either is
+__device__ __forceinline__ float sa_max(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
 // 2^x of two values on the FMA units: x = n + f, n the nearest integer (by adding and taking away 1.5 2^23, whose low bits then hold
 // n), a polynomial of degree 5 for 2^f on [-1/2, 1/2] (fitted to the relative error: 2.4e-7 with its roundings in 32 bits),
-// n added to the exponent.  Below -126: 2^-126 or so instead of zero, which f16 rounds to zero and no sum notices
+// n added to the exponent.  Below -126 (and of a NaN, which the row's maximum shows): 2^-126 or so instead of zero, which f16 rounds to
+// zero and no sum notices
 __device__ __forceinline__ float2 sa_ex2_poly(float2 x) {
     const float magic = 12582912.f;
     x.x = fmaxf(x.x, -126.f), x.y = fmaxf(x.y, -126.f);
@@ -357,9 +364,10 @@ __device__ __forceinline__ float2 sa_ex2_poly(float2 x) {
 // a pair of gated values: y / (1 + e^-g), one reciprocal for both (the gates cut at -40, where no f16 value has anything left)
 __device__ __forceinline__ void sa_gate(float& y0, float& y1, float g0, float g1) {
     const float a = 1.0f + ex2_ftz(-1.44269504f * (g0 < -40.f ? -40.f : g0)), b = 1.0f + ex2_ftz(-1.44269504f * (g1 < -40.f ? -40.f : g1));
+    const float am = fmaxf(a, 1.f), bm = fmaxf(b, 1.f);   // (only a NaN differs, and only its own value shall)
     float r;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(a * b));
-    y0 *= r * b, y1 *= r * a;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(am * bm));
+    y0 = fmaf(a, 0.f, y0 * (r * bm)), y1 = fmaf(b, 0.f, y1 * (r * am));
 }
 // the same by one lane for its warp (all lanes get the answer)
 __device__ __forceinline__ bool sa_wait_warp(unsigned long long* bar, unsigned parity, int& spins, unsigned* fault) {
@@ -742,12 +750,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(SA_THREADS, 1) k_att
                 }
                 float mq[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-                for (int k = 4; k < 64; ++k) mq[k & 3] = fmaxf(mq[k & 3], x[k]);
-                float mx = fmaxf(fmaxf(mq[0], mq[1]), fmaxf(mq[2], mq[3]));
+                for (int k = 4; k < 64; ++k) mq[k & 3] = sa_max(mq[k & 3], x[k]);
+                float mx = sa_max(sa_max(mq[0], mq[1]), sa_max(mq[2], mq[3]));
                 float* xm = xmax + (j & 1) * 2 * SA_ROWS;
                 xm[half * SA_ROWS + m] = mx;
                 agree();
-                mx = fmaxf(mx, xm[(half ^ 1) * SA_ROWS + m]) * scale;
+                mx = sa_max(mx, xm[(half ^ 1) * SA_ROWS + m]) * scale;
+                if (!(mx < INFINITY)) z = NAN;   // a score that is no number, or infinite: so is the row
                 const bool up = real && (mx > ref + 8.0f || (ref == -INFINITY && mx != -INFINITY));   // (other rows hold what was there before)
                 if (__any_sync(0xffffffffu, up)) {
                     const float f = !up ? 1.0f : ref == -INFINITY ? 0.f : ex2_ftz(ref - mx);
@@ -794,6 +803,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(SA_THREADS, 1) k_att
             agree();
             z += xm[(half ^ 1) * SA_ROWS + m];
             agree();   // (a segment without tiles would write there again)
+            if (z != z) ref = 0.f;
             const bool none = ref == -INFINITY;   // the row saw nothing
             const float inv = none ? 0.f : 1.0f / z;
             const size_t slot = (size_t) (2 * g + (r.first ? 0 : 1)) * 2 + rank;   // of the parts
@@ -926,7 +936,7 @@ template <int HD> __global__ void __launch_bounds__(256, 3) k_attn_seqs_join(con
             acc[4] = fmaf(f, v[i][1].x, acc[4]), acc[5] = fmaf(f, v[i][1].y, acc[5]), acc[6] = fmaf(f, v[i][1].z, acc[6]), acc[7] = fmaf(f, v[i][1].w, acc[7]);
         }
     }
-    const float inv = z > 0.f ? 1.0f / z : 0.f;
+    const float inv = z == 0.f ? 0.f : 1.0f / z;
 #pragma unroll
     for (int k = 0; k < 8; ++k) acc[k] *= inv;
     if (gate) {

@@ -221,6 +221,42 @@ def test_prompt_attention_entries_outside_the_pool_are_rows_of_zeros():
     _check(s, s.attend())
 
 
+@pytest.mark.parametrize("lens,ctx,at", [([70, 3], [200, 40], range(128, 192)), ([1, 3], [6000, 40], range(5000, 5064)), ([2], [1], range(0, 2)), ([1], [0], range(0, 1))])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_a_score_that_is_no_number_shows_in_the_rows_that_see_it(lens, ctx, at, value):
+    """A NaN or infinity in a key, wherever in a tile it lies: rows that see it and get a NaN or +inf score give NaNs, all others what
+    they gave before (a score of -inf weighs nothing)."""
+    s = S.Seqs(lens, ctx, 8, 2, 128, seed=17)
+    before = s.attend().view(-1, 8, 128)
+    assert torch.isfinite(before).all()
+    q0 = s.q[:s.rows].view(s.rows, 8, 128)[:, :4, 0]
+    pos = torch.tensor([x + t for n, x in zip(lens, ctx) for t in range(n)], device=DEV)
+    for p in at:
+        row = s.rows_of(s.kc)[int(s.cells[0][p]), 0]
+        keep = row.clone()
+        s.rows_of(s.kc)[int(s.cells[0][p]), 0, 0] = value
+        out = s.attend().view(-1, 8, 128)
+        row.copy_(keep)
+        hit = (torch.arange(s.rows, device=DEV) < lens[0])[:, None] & (pos >= p)[:, None] & ((q0 >= 0) if value == float("inf") else torch.ones_like(q0, dtype=torch.bool))
+        assert torch.isnan(out[:, :4][hit]).all(), p
+        if value != value:
+            assert torch.equal(out[:, :4][~hit], before[:, :4][~hit]), p
+        assert torch.isfinite(out[:, :4][~hit]).all() and torch.equal(out[:, 4:], before[:, 4:]), p
+
+
+def test_a_gate_that_is_no_number_shows_in_its_own_element():
+    for lens, ctx in (([5], [60]), ([1], [9000])):
+        s = S.Seqs(lens, ctx, 8, 2, 128, seed=18)
+        before = s.attend()
+        s.qg[0, 3, 128 + 7], s.qg[0, 3, 128 + 20], s.qg[0, 3, 128 + 31] = float("nan"), float("inf"), -float("inf")
+        out, want = s.attend(), before.clone()
+        want[0, 3 * 128 + 7], want[0, 3 * 128 + 31] = float("nan"), 0.0
+        plain = s.attend(gate=False)
+        want[0, 3 * 128 + 20] = plain[0, 3 * 128 + 20]
+        near = (out - want).abs() <= 2.0 ** -10 * want.abs()   # (a sigmoid of a pair's shared reciprocal: the last bit may differ)
+        assert torch.isnan(out[0, 3 * 128 + 7]) and (near | torch.isnan(want)).all()
+
+
 @pytest.mark.parametrize("hint", [0, 1, 50000])
 def test_prompt_attention_whatever_the_hint(hint):
     """max_pos decides how the work is split, never what is computed: too small, unknown, far too large."""
