@@ -191,6 +191,44 @@ def test_reserve_of_many_sequences_and_long_ones(nseq, add, rows):
     assert (p.ref == 0).all() and (p.pt == -1).all() and (p.len == 0).all()
 
 
+@pytest.mark.parametrize("nseq,width", [(256, 37), (257, 13), (4096, 9)])
+def test_forks_among_many_sequences(nseq, width):
+    """Every sequence's source, and where it is cut, anywhere: tables, lengths and counts against the same done one by one."""
+    rng = np.random.default_rng(nseq)
+    rows = 4
+    p = Pool(nseq * width, rows, nseq, width, nplanes=1, nkv=1)
+    p.reserve(rng.integers(0, width * rows + 1, nseq))
+    for step in range(3):
+        pt, ln = p.pt.cpu().numpy(), p.len.cpu().numpy()
+        src, lim = rng.integers(-1, nseq, nseq), rng.integers(0, width * rows + 5, nseq) if step else None
+        p.fork(src, lim)
+        want_len = np.where(src >= 0, ln[src], 0)
+        if lim is not None:
+            want_len = np.minimum(want_len, lim)
+        want = np.where(np.arange(width)[None] < -(-want_len // rows)[:, None], pt[src], -1)
+        assert int(p.err) == 0 and np.array_equal(p.len.cpu().numpy(), want_len) and np.array_equal(p.pt.cpu().numpy(), want)
+        assert np.array_equal(p.ref.cpu().numpy(), np.bincount(want[want >= 0], minlength=p.npages))
+
+
+@pytest.mark.parametrize("q8,nkv", [(False, 2), (True, 2), (False, 9)])
+def test_long_paths_kept(q8, nkv):
+    """Paths of hundreds of rows, rows wider than a block's threads take at once, all rows kept and none."""
+    rng = np.random.default_rng(5)
+    p = Pool(300, 8, 4, 70, nplanes=2, nkv=nkv, hd=256, q8=q8, seed=5)
+    p.reserve([3, 0, 17, 1])
+    want = [[rows for rows in p.write(s, 0, n, rng)] for s, n in enumerate([3, 0, 17, 1])]
+    add = [500, 300, 129, 140]
+    p.reserve(add)
+    for s, n in enumerate(add):
+        have = len(want[s][0])
+        for pl, new in enumerate(p.write(s, have, have + n, rng)):
+            want[s][pl] += new
+    lists = [sorted(rng.choice(500, 333, replace=False).tolist()), list(range(300)), [], list(range(1, 140))]
+    p.keep(lists)
+    base = [3, 0, 17, 1]
+    p.check([[pl[:base[s]] + [pl[base[s] + i] for i in k] for pl in want[s]] for s, k in enumerate(lists)])
+
+
 def test_one_captured_step_replayed():
     """Growth, and the rows behind the first of them given back, captured once: the tables come back to where they were."""
     p = Pool(30, 8, 3, 8)

@@ -303,6 +303,34 @@ def test_prompt_attention_captured_then_replayed_on_other_lengths():
     torch.cuda.synchronize()
 
 
+@pytest.mark.parametrize("page,lens,ctx", [(0, [1], [0]), (0, [2, 1], [0, 3]), (8, [1], [0]), (8, [3], [5]), (256, [1], [2])])
+@pytest.mark.parametrize("nq,nkv,hd", [(1, 1, 128), (16, 1, 256), (22, 2, 128)])
+def test_caches_and_calls_smaller_than_a_tile(page, lens, ctx, nq, nkv, hd):
+    """Pools of a page or two and contiguous caches of a few rows, shorter than any box that is copied out of them; no row behind
+    the last sequence."""
+    s = S.Seqs(lens, ctx, nq, nkv, hd, page=page, seed=page + nq)
+    _check(s, s.attend())
+    _, bits, _ = s.tree(1)
+    _check(s, s.attend(torch.from_numpy(bits.view(np.int32)).to(DEV)), bits)
+
+
+def test_calls_on_two_streams_at_once():
+    a, b = S.Seqs([300, 1, 17], [900, 4000, 3], 24, 4, 256, seed=41), S.Seqs([1] * 9, [500 * i for i in range(9)], 8, 2, 128, seed=42)
+    want = [x.attend().clone() for x in (a, b)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = [[torch.empty_like(w) for _ in range(6)] for w in want]
+    scratch = [x.scratch() for x in (a, b)]
+    torch.cuda.synchronize()
+    for i in range(6):
+        for x, st, o, w in zip((a, b), streams, outs, scratch):
+            with torch.cuda.stream(st):
+                x.attend(out=o[i], scratch=w)
+    torch.cuda.synchronize()
+    for w, o in zip(want, outs):
+        assert all(torch.equal(w[:-1].view(torch.int16), x[:-1].view(torch.int16)) for x in o)
+    assert L.load().fnx_device_fault() == 0
+
+
 def test_cache_past_2_to_31_elements():
     """A pool of more than 2^31 halves: the sequence's pages lie at its far end."""
     nq, nkv, hd, page = 2, 2, 256, 64
