@@ -6,8 +6,8 @@
 // and which holder of a shared page keeps it is the lowest, so no order of atomics shows.
 // The tables are a few thousand words: what these calls cost is the latency of a handful of dependent loads and launches, so
 // loads go out before their use is known and divisions are 32 bits wide; the row copies are DRAM's.  Seven forks and their
-// copies of a partly filled page in 24 planes: 14.4 us (alone: fork 5, reserve 9.6, copy 6.3); growth of 32 sequences and
-// their accepted paths in 4 planes: 17.1 (fork 6, reserve 10, copy 3, keep 9.3, trim 3.5).
+// copies of a partly filled page in 24 planes: 12.2 us (a launch, six dependent loads and four barriers of one block in reserve); growth of 32 sequences and
+// their accepted paths in 4 planes: 15.0.
 #include <algorithm>
 #include <climits>
 
@@ -104,31 +104,40 @@ __global__ void __launch_bounds__(256) k_pages_fork(const FnxPagePool p, const i
 }
 
 // ---------------------------------------------------------------- reserve
-// exclusive sums of two values a thread over the block (in ascending thread order); totals in t0, t1
-__device__ __forceinline__ void pg_scan2(long long& a, long long& b, long long& t0, long long& t1, long long (*sh)[2]) {
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const long long a0 = a, b0 = b;
+// Sums that stop at a cap of at most 2^31 (associative over values up to it, so their order is free)
+__device__ __forceinline__ unsigned pg_add(unsigned a, unsigned b, unsigned cap) { return min(a + b, cap); }
+// exclusive sums over the block of two values a thread, in ascending thread order; totals in t0, t1; flags: every thread's or'ed
+__device__ __forceinline__ void pg_scan2(unsigned& a, unsigned& b, unsigned cap_a, unsigned cap_b, unsigned& flags, unsigned& t0, unsigned& t1, unsigned (*sh)[4]) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    auto scan = [&](unsigned& x, unsigned cap) {
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const long long x = __shfl_up_sync(0xffffffffu, a, o), y = __shfl_up_sync(0xffffffffu, b, o);
-        if (lane >= o) a += x, b += y;
-    }
-    if (lane == 31) sh[warp][0] = a, sh[warp][1] = b;
+        for (int o = 1; o < 32; o <<= 1) {
+            const unsigned y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x = pg_add(x, y, cap);
+        }
+    };
+    auto before = [&](unsigned x, int at) {   // what lies before lane `at`
+        const unsigned y = __shfl_sync(0xffffffffu, x, (at - 1) & 31);
+        return at ? y : 0u;
+    };
+    unsigned sa = min(a, cap_a), sb = min(b, cap_b);
+    scan(sa, cap_a), scan(sb, cap_b);
+    flags = __reduce_or_sync(0xffffffffu, flags);
+    if (lane == 31) *reinterpret_cast<uint4*>(sh[warp]) = make_uint4(sa, sb, flags, 0u);
+    const unsigned own_a = __shfl_up_sync(0xffffffffu, sa, 1), own_b = __shfl_up_sync(0xffffffffu, sb, 1);
     __syncthreads();
-    long long pa = 0, pb = 0;
-    t0 = t1 = 0;
-    for (int i = 0; i < PG_WARPS; ++i) {
-        if (i == warp) pa = t0, pb = t1;
-        t0 += sh[i][0], t1 += sh[i][1];
-    }
-    __syncthreads();
-    a += pa - a0, b += pb - b0;
+    const uint4 all = *reinterpret_cast<const uint4*>(sh[lane]);   // (PG_WARPS = 32)
+    unsigned wa = all.x, wb = all.y;
+    scan(wa, cap_a), scan(wb, cap_b);
+    flags = __reduce_or_sync(0xffffffffu, all.z);
+    t0 = __shfl_sync(0xffffffffu, wa, 31), t1 = __shfl_sync(0xffffffffu, wb, 31);
+    a = pg_add(before(wa, warp), lane ? own_a : 0u, cap_a), b = pg_add(before(wb, warp), lane ? own_b : 0u, cap_b);
 }
 
 constexpr int PG_NEAR = 2048;   // places of the list of pages handed out that lie in shared memory
 __global__ void __launch_bounds__(PG_THREADS) k_pages_reserve(const FnxPagePool p, const int* __restrict__ add, int* pos0, int* row0, void* scratch, unsigned* err) {
     const PgScratch w = pg_scratch(p, scratch);
-    __shared__ long long sh[PG_WARPS][2];
+    __shared__ __align__(16) unsigned sh[PG_WARPS][4];
     __shared__ int first[PG_SEQS], near[PG_NEAR], wcount[PG_WARPS];   // first: a sequence's first place in the list of pages handed out
     __shared__ unsigned fresh[PG_SEQS];                                // where its new pages begin in its table, times two, + 1: after a copy
     __shared__ unsigned njobs_s;
@@ -176,24 +185,28 @@ __global__ void __launch_bounds__(PG_THREADS) k_pages_reserve(const FnxPagePool 
     __threadfence_block();
     __syncthreads();
     bool copy[PG_PER];
-    long long a = 0, b = 0, pages, rows;
+    unsigned a = 0u, b = 0u, pages, rows, flags = (bad ? 1u : 0u) | (room ? 0u : 2u);
+    const unsigned cap_pages = (unsigned) p.npages + 1u, cap_rows = 1u << 31;
 #pragma unroll
     for (int k = 0; k < PG_PER; ++k) {
         const int s = tid * per + k;
-        copy[k] = tail[k] >= 0 && (refs[k] > __ldcg(&w.holders[tail[k]]) || __ldcg(&w.lowest[tail[k]]) != INT_MAX - s);
-        if (k < per && s < p.nseq && more[k] >= 0 && room)
+        copy[k] = false;
+        if (k >= per || s >= p.nseq) continue;
+        if (tail[k] >= 0) {
+            const int holders = __ldcg(&w.holders[tail[k]]), lowest = __ldcg(&w.lowest[tail[k]]);
+            copy[k] = refs[k] > holders || lowest != INT_MAX - s;
+        }
+        if (more[k] >= 0 && room)
             want[k] = (int) (pg_pages(p, (unsigned) len[k] + (unsigned) more[k]) - pg_pages(p, (unsigned) len[k])) + (copy[k] ? 1 : 0);
-        a += want[k], b += more[k] > 0 ? more[k] : 0;
+        a = pg_add(a, min((unsigned) want[k], cap_pages), cap_pages), b = pg_add(b, more[k] > 0 ? (unsigned) more[k] : 0u, cap_rows);
     }
-    __syncthreads();   // everyone has looked at the holders
+    pg_scan2(a, b, cap_pages, cap_rows, flags, pages, rows, sh);   // (everyone has looked at the holders when it returns)
 #pragma unroll
     for (int k = 0; k < PG_PER; ++k)
         if (tail[k] >= 0) w.holders[tail[k]] = 0, w.lowest[tail[k]] = 0;
-    pg_scan2(a, b, pages, rows, sh);
-    bad = __syncthreads_or(bad);
-    room = !__syncthreads_or(!room) && rows <= INT_MAX;
+    bad = flags & 1u, room = !(flags & 2u) && rows < cap_rows;
     // ---- the lowest free pages, as many as are wanted
-    int got = 0;
+    unsigned got = 0u;
     if (room && !bad)
         for (int q0 = 0; q0 < p.npages && got < pages; q0 += 4 * PG_THREADS) {
             if (q0) free_bits(q0, is);
@@ -203,11 +216,11 @@ __global__ void __launch_bounds__(PG_THREADS) k_pages_reserve(const FnxPagePool 
             if (lane == 0) wcount[warp] = mine;
             __syncthreads();
             const int others = wcount[lane];   // (PG_WARPS = 32)
-            int below = got + __reduce_add_sync(0xffffffffu, lane < warp ? others : 0);
+            unsigned below = got + __reduce_add_sync(0xffffffffu, lane < warp ? others : 0);
             got += __reduce_add_sync(0xffffffffu, others);
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const int at = below + before[k] + __popc(is[k] & ((1u << lane) - 1u));
+                const unsigned at = below + before[k] + __popc(is[k] & ((1u << lane) - 1u));
                 if ((is[k] >> lane & 1u) && at < pages) (at < PG_NEAR ? near[at] : w.free_list[at]) = q0 + warp * 128 + k * 32 + lane;
             }
             __syncthreads();
