@@ -15,8 +15,8 @@
 // A row goes to one block when there are many, else to as many as the GPU holds at once; the row's last block joins the parts.
 // A pass is bound by DRAM when there are many rows: a thread copies its own values into shared memory three batches ahead
 // (cp.async; nobody else reads them, so no barrier belongs to it), 72 KB in flight a multiprocessor.  2000 rows of 151 936 logits with
-// five alternatives: 230 us (5.3 TB/s); with one batch ahead in registers 342.  16 rows with twenty: 14.4 us, latency - three rounds
-// of choosing the best, the blocks' results through memory to the last one.
+// five alternatives: 214 us (5.7 TB/s); with one batch ahead in registers 342.  16 rows with twenty: 12.3 us, latency - a bound, the
+// lists through memory to the row's last block, a bound and the choice there.
 #include <algorithm>
 
 #include "common.cuh"
@@ -37,13 +37,13 @@ struct LpPart {   // the sums over a block's part of a row
 struct LpArgs {
     const float* logits;
     size_t stride;
-    int rows, n, v0, k, ntok, nsplit;
+    int rows, n, v0, k, ntok, nsplit, ship;   // ship: entries that a block leaves for the row's last block, k at least
     const int* tok;
     float *lse, *ent, *lp, *top_lp;
     int* top_i;
     unsigned* count;             // [T] blocks of the row that are done (left at zero)
     LpPart* part;                // [T][nsplit]
-    unsigned long long* cand;    // [T][nsplit][k]
+    unsigned long long* cand;    // [T][nsplit][ship], zero where there are fewer
     unsigned* err;
 };
 
@@ -63,6 +63,15 @@ __device__ __forceinline__ void lp_join(float& r, float& z, float& s, float r2, 
     s = f1 * (s + d1 * z) + f2 * (s2 + d2 * z2);
     z = f1 * z + f2 * z2;
     r = rn;
+}
+
+// the same of a warp's 32 parts: one reference for all, then plain sums
+__device__ __forceinline__ void lp_join_warp(float& r, float& z, float& s) {
+    const float top = fkey_inv(__reduce_max_sync(0xffffffffu, fkey(r)));
+    const float d = r == top ? 0.f : fmaxf(r - top, -200.f), f = ex2_ftz(d);
+    s = f * (s + d * z), z *= f, r = top;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o), s += __shfl_xor_sync(0xffffffffu, s, o);
 }
 
 // Bisection by a warp: a bound b that between k and k + slack of the entries reach or exceed (a lane has N; 0: no entry), or 0
@@ -104,6 +113,7 @@ struct LpShared {
     unsigned long long list[LP_WARPS][LP_LIST];
     alignas(16) unsigned long long best[LP_THREADS >> 2];   // groups' maxima
     float r[LP_WARPS], z[LP_WARPS], s[LP_WARPS];
+    int cnt[LP_WARPS];
     unsigned long long bound;
     unsigned n, last;
     float lse;
@@ -302,34 +312,34 @@ __global__ void __launch_bounds__(LP_THREADS, 2) k_logprobs(const LpArgs a) {
         }
         // ---- the block's statistics
         float z = z2.x + z2.y, s = s2.x + s2.y;
-#pragma unroll
-        for (int o = 16; o; o >>= 1) {
-            const float ro = __shfl_xor_sync(0xffffffffu, r, o), zo = __shfl_xor_sync(0xffffffffu, z, o), so = __shfl_xor_sync(0xffffffffu, s, o);
-            lp_join(r, z, s, ro, zo, so);
-        }
-        if (lane == 0) sh.r[warp] = r, sh.z[warp] = z, sh.s[warp] = s;
+        lp_join_warp(r, z, s);
+        if (lane == 0) sh.r[warp] = r, sh.z[warp] = z, sh.s[warp] = s, sh.cnt[warp] = cnt;
         unsigned long long e[LP_LIST / 32];
         __syncwarp();
 #pragma unroll
         for (int i = 0; i < LP_LIST / 32; ++i) e[i] = i * 32 + lane < cnt ? list[i * 32 + lane] : 0ull;
         __syncthreads();
         LpPart* parts = a.part + (size_t) t.row * a.nsplit;
-        unsigned long long* cands = a.cand + (size_t) t.row * a.nsplit * a.k;
+        unsigned long long* cands = a.cand + (size_t) t.row * a.nsplit * a.ship;
         if (warp == 0) {
             r = lane < LP_WARPS ? sh.r[lane] : -INFINITY, z = lane < LP_WARPS ? sh.z[lane] : 0.f, s = lane < LP_WARPS ? sh.s[lane] : 0.f;
-#pragma unroll
-            for (int o = 16; o; o >>= 1) {
-                const float ro = __shfl_xor_sync(0xffffffffu, r, o), zo = __shfl_xor_sync(0xffffffffu, z, o), so = __shfl_xor_sync(0xffffffffu, s, o);
-                lp_join(r, z, s, ro, zo, so);
-            }
+            lp_join_warp(r, z, s);
         }
         bool mine = true;   // whether the row's results are this block's to write
         if (a.nsplit > 1) {   // the row's last block joins the parts
             if (tid == 0) parts[t.split] = LpPart{r, z, s, 0.f};
             if (a.k) {
-                for (int i = tid; i < a.k; i += LP_THREADS) cands[(size_t) t.split * a.k + i] = 0ull;
-                __syncthreads();
-                lp_best(sh, e, a.k, [&](int place, unsigned long long c) { cands[(size_t) t.split * a.k + place] = c; });
+                unsigned long long* mine_at = cands + (size_t) t.split * a.ship;
+                const int held = lane < LP_WARPS ? sh.cnt[lane] : 0;
+                const int before = (int) __reduce_add_sync(0xffffffffu, (unsigned) (lane < warp ? held : 0)), total = (int) __reduce_add_sync(0xffffffffu, (unsigned) held);
+                const bool all = total <= a.ship;   // the lists as they are; else the k best
+                for (int i = tid + (all ? total : 0); i < a.ship; i += LP_THREADS) mine_at[i] = 0ull;
+                if (all) {
+                    for (int i = lane; i < cnt; i += 32) mine_at[before + i] = list[i];
+                } else {
+                    __syncthreads();
+                    lp_best(sh, e, a.k, [&](int place, unsigned long long c) { mine_at[place] = c; });
+                }
             }
             __threadfence();
             __syncthreads();
@@ -344,14 +354,10 @@ __global__ void __launch_bounds__(LP_THREADS, 2) k_logprobs(const LpArgs a) {
                         const LpPart p = parts[i];
                         lp_join(r, z, s, p.r, p.z, p.s);
                     }
-#pragma unroll
-                    for (int o = 16; o; o >>= 1) {
-                        const float ro = __shfl_xor_sync(0xffffffffu, r, o), zo = __shfl_xor_sync(0xffffffffu, z, o), so = __shfl_xor_sync(0xffffffffu, s, o);
-                        lp_join(r, z, s, ro, zo, so);
-                    }
+                    lp_join_warp(r, z, s);
                 }
 #pragma unroll
-                for (int i = 0; i < LP_LIST / 32; ++i) e[i] = i * LP_THREADS + tid < a.nsplit * a.k ? cands[i * LP_THREADS + tid] : 0ull;
+                for (int i = 0; i < LP_LIST / 32; ++i) e[i] = i * LP_THREADS + tid < a.nsplit * a.ship ? cands[i * LP_THREADS + tid] : 0ull;
                 if (tid == 0) a.count[t.row] = 0u;
             }
         }
@@ -392,6 +398,9 @@ static int lp_splits(int n, int T, int k) {
     const int per = (batches + s - 1) / s;
     return (batches + per - 1) / per;   // no empty block
 }
+// entries that a block of a row in several parts leaves for the last one: its lists as they are where they have room, which spares
+// choosing the best twice (16 rows, 20 alternatives: 13.8 us with k each, 12.3 so)
+static int lp_ship(int ns, int k) { return k ? std::max(k, std::min(128, LP_CAP / ns)) : 0; }
 
 }  // namespace fnxk
 
@@ -402,7 +411,7 @@ extern "C" {
 size_t fnx_logprobs_scratch_bytes(int n, int T, int k) {
     if (n < 1 || T < 1 || k < 0 || k > FNX_TOPK_N) return 0;
     const size_t s = (size_t) lp_splits(n, T, k);
-    return s == 1 ? 16 : (size_t) LP_BLOCKS * 4 + (size_t) T * s * (sizeof(LpPart) + 8 * (size_t) k);
+    return s == 1 ? 16 : (size_t) LP_BLOCKS * 4 + (size_t) T * s * (sizeof(LpPart) + 8 * (size_t) lp_ship((int) s, k));
 }
 
 int fnx_logprobs(const float* logits, size_t stride, int n, int T, int v0, const int* tok, int ntok, int k, float* lse, float* entropy, float* lp,
@@ -414,7 +423,7 @@ int fnx_logprobs(const float* logits, size_t stride, int n, int T, int v0, const
     FNX_REQUIRE(logits && lse && scratch && err && (!k || (top_lp && top_i)), "logprobs: a null buffer");
     FNX_REQUIRE((uintptr_t) scratch % 16 == 0, "logprobs: scratch not 16-byte aligned");
     const int ns = lp_splits(n, T, k);
-    LpArgs a{logits, stride, T, n, v0, k, ntok, ns, tok, lse, entropy, lp, top_lp, top_i, (unsigned*) scratch, nullptr, nullptr, err};
+    LpArgs a{logits, stride, T, n, v0, k, ntok, ns, lp_ship(ns, k), tok, lse, entropy, lp, top_lp, top_i, (unsigned*) scratch, nullptr, nullptr, err};
     // the counters have their place whatever the call's sizes, so that one scratch serves calls of different ones
     a.part = reinterpret_cast<LpPart*>((char*) scratch + LP_BLOCKS * 4);
     a.cand = reinterpret_cast<unsigned long long*>(a.part + (size_t) T * ns);
