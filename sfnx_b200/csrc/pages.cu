@@ -6,8 +6,8 @@
 // and which holder of a shared page keeps it is the lowest, so no order of atomics shows.
 // The tables are a few thousand words: what these calls cost is the latency of a handful of dependent loads and launches, so
 // loads go out before their use is known and divisions are 32 bits wide; the row copies are DRAM's.  Seven forks and their
-// copies of a partly filled page in 24 planes: 12.2 us (a launch, six dependent loads and four barriers of one block in reserve); growth of 32 sequences and
-// their accepted paths in 4 planes: 15.0.
+// copies of a partly filled page in 24 planes: 11.8 us (three launches; in reserve six dependent loads and four barriers of one
+// block); growth of 32 sequences and their accepted paths in 4 planes: 14.5.
 #include <algorithm>
 #include <climits>
 
@@ -308,7 +308,8 @@ __global__ void __launch_bounds__(256) k_pages_copy(const FnxPagePool p, void* c
 // Block (sequence, plane).  Where each kept row lies goes to shared memory, PK_ROWS at a time; a thread has 16 bytes of a row and
 // walks the path in ascending order, PK_BATCH rows' loads before their stores: a kept row's old place is never before its new
 // one, and the list ascends, so a store meets only rows whose loads are done.  (Scales of int8 rows the same way, 8 bytes a
-// thread.)  The first batch's loads are under way while the pages are still looked at; nothing is stored before that is done.
+// thread.)  The first batch's loads are under way before the block has agreed that the list and its pages are sound; nothing
+// is stored before that.
 constexpr int PK_THREADS = 128, PK_ROWS = PK_THREADS, PK_BATCH = 16;   // (batches of 8: a step of 32 sequences takes 1 us longer)
 struct PkMove {
     int from, from_row, to, to_row;   // page and row in it; from negative: the row stays, or the list is senseless
@@ -340,7 +341,17 @@ __global__ void __launch_bounds__(PK_THREADS, 3) k_pages_keep(const FnxPagePool 
         if (e == i || !pg_valid(p, m.from) || !pg_valid(p, m.to)) m.from = -1;
         return m;
     };
-    if (sound && tid < n) moves[tid] = find(tid);
+    if (sound) {   // the list, and the pages that rows are read from and written to; all first loads together
+        const unsigned rows = (unsigned) p.rows;
+        const int end = (int) pg_pages(p, (unsigned) len), first = (int) ((unsigned) at0 / rows);
+        auto page_bad = [&](int j, int page) { return !pg_valid(p, page) || (n > 0 && j * p.rows < at0 + n && p.ref[page] != 1); };
+        const int page0 = first + tid < end ? pt[first + tid] : 0, l0 = tid < n ? list[tid] : 0, l1 = tid && tid < n ? list[tid - 1] + 1 : 0;
+        const bool page0_bad = first + tid < end && page_bad(first + tid, page0);
+        if (tid < n) moves[tid] = find(tid);
+        bad = page0_bad || (tid < n && (l0 < l1 || l0 >= have));
+        for (int i = tid + PK_THREADS; i < n; i += PK_THREADS) bad = bad || list[i] < list[i - 1] + 1 || list[i] >= have;
+        for (int j = first + tid + PK_THREADS; j < end; j += PK_THREADS) bad = bad || page_bad(j, pt[j]);
+    }
     __syncthreads();
     auto ask = [&](auto* v, int k0, int count, size_t start, size_t row_bytes, size_t c) {
 #pragma unroll
@@ -357,14 +368,6 @@ __global__ void __launch_bounds__(PK_THREADS, 3) k_pages_keep(const FnxPagePool 
     uint4 v[PK_BATCH];
     const bool mine = sound && (size_t) tid * 16 < r.row_bytes;
     if (mine) ask(v, 0, min(n, PK_ROWS), 0, r.row_bytes, (size_t) tid * 16);
-    if (sound) {
-        for (int i = tid; i < n; i += PK_THREADS) bad = bad || list[i] < (i ? list[i - 1] + 1 : 0) || list[i] >= have;
-        const int end = (int) pg_pages(p, (unsigned) len);
-        for (int j = at0 / p.rows + tid; j < end; j += PK_THREADS) {   // the pages that rows are read from and written to
-            const bool ours = pg_valid(p, pt[j]);
-            bad = bad || !ours || (n > 0 && j * p.rows < at0 + n && p.ref[pt[j]] != 1);
-        }
-    }
     bad = __syncthreads_or(bad);
     if (head && tid == 0) {
         w.verdict[s] = bad ? -1 : at0 + n;
