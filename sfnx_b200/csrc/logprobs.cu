@@ -37,7 +37,9 @@ struct LpPart {   // the sums over a block's part of a row
 struct LpArgs {
     const float* logits;
     size_t stride;
-    int rows, n, v0, k, ntok, nsplit, ship;   // ship: entries that a block leaves for the row's last block, k at least
+    int rows, n, v0, k, ntok, nsplit;
+    int per;    // positions a part of a row, whole batches
+    int ship;   // entries that a block leaves for the row's last block, k at least
     const int* tok;
     float *lse, *ent, *lp, *top_lp;
     int* top_i;
@@ -170,13 +172,13 @@ struct LpItem {   // a block's part of a row
     const float* base;   // positions are counted from the 16-byte boundary at or before the row's first logit
     int row, split, shift, lo, hi;
 };
-__device__ __forceinline__ LpItem lp_item(const LpArgs& a, unsigned w) {   // (rows in several parts are few: w is below 2^31)
+__device__ __forceinline__ LpItem lp_item(const LpArgs& a, int row, int split) {
     LpItem t;
-    t.row = (int) (w / (unsigned) a.nsplit), t.split = (int) (w - (unsigned) t.row * (unsigned) a.nsplit);
-    const float* x = a.logits + (size_t) t.row * a.stride;
+    t.row = row, t.split = split;
+    const float* x = a.logits + (size_t) row * a.stride;
     t.shift = (int) (((uintptr_t) x >> 2) & 3u), t.base = x - t.shift;
-    const int end = a.n + t.shift, batches = (end + LP_BATCH - 1) / LP_BATCH, per = (batches + a.nsplit - 1) / a.nsplit;
-    t.lo = (int) min((long long) t.split * per * LP_BATCH, (long long) end), t.hi = (int) min((long long) t.lo + (long long) per * LP_BATCH, (long long) end);
+    const long long end = a.n + t.shift, lo = (long long) split * a.per;
+    t.lo = (int) min(lo, end), t.hi = (int) min(lo + a.per, end);
     return t;
 }
 
@@ -213,12 +215,13 @@ __global__ void __launch_bounds__(LP_THREADS, 2) k_logprobs(const LpArgs a) {
     pdl_wait();
     pdl_go();
     const float L2E = 1.44269504f;
-    const unsigned items = (unsigned) a.rows * (unsigned) a.nsplit;
-    LpItem next = lp_item(a, blockIdx.x);
+    const bool parts_of_rows = a.nsplit > 1;   // a block a part; else a block every gridDim.x-th row
+    const unsigned step = parts_of_rows ? (unsigned) a.rows : gridDim.x;
+    LpItem next = lp_item(a, parts_of_rows ? blockIdx.y : blockIdx.x, parts_of_rows ? blockIdx.x : 0);
     int stage = 0;
 #pragma unroll
     for (int i = 0; i < LP_STAGES - 1; ++i) load(next, next.lo + i * LP_BATCH, slot(i));
-    for (unsigned w = blockIdx.x; w < items; w += gridDim.x) {
+    for (unsigned row = (unsigned) next.row; row < (unsigned) a.rows; row += step) {
         const LpItem t = next;
         float r = -INFINITY, bound_v = -INFINITY;                        // r: the reference, in units of log2
         float2 z2 = make_float2(0.f, 0.f), s2 = make_float2(0.f, 0.f);   // the sums of the even and the odd values
@@ -305,8 +308,8 @@ __global__ void __launch_bounds__(LP_THREADS, 2) k_logprobs(const LpArgs a) {
                 cnt += __popc(who);
             }
         }
-        if (w + gridDim.x < items) {   // the next row's first batches are on their way while this one is finished
-            next = lp_item(a, w + gridDim.x);
+        if (row + step < (unsigned) a.rows) {   // the next row's first batches are on their way while this one is finished
+            next = lp_item(a, (int) (row + step), 0);
 #pragma unroll
             for (int i = 0; i < LP_STAGES - 1; ++i) load(next, next.lo + i * LP_BATCH, slot((stage + i) % LP_STAGES));
         }
@@ -392,10 +395,11 @@ __global__ void __launch_bounds__(LP_THREADS, 2) k_logprobs(const LpArgs a) {
 }
 
 // blocks a row: as many as the GPU holds at once, each with a batch of the row at least; their k best have room in one block
-static int lp_splits(int n, int T, int k) {
+static int lp_splits(int n, int T, int k, int* each = nullptr) {
     const int batches = (n + 3 + LP_BATCH - 1) / LP_BATCH, want = std::max(1, LP_BLOCKS / T);   // n + 3: a row may begin inside a 16-byte run
     const int s = std::max(1, std::min(want, std::min(batches, std::min(64, LP_CAP / std::max(k, 1)))));
     const int per = (batches + s - 1) / s;
+    if (each) *each = per * LP_BATCH;
     return (batches + per - 1) / per;   // no empty block
 }
 // entries that a block of a row in several parts leaves for the last one: its lists as they are where they have room, which spares
@@ -422,14 +426,15 @@ int fnx_logprobs(const float* logits, size_t stride, int n, int T, int v0, const
     FNX_REQUIRE(ntok >= 0 && (!ntok || (tok && lp)), "logprobs: %d given tokens without their buffers", ntok);
     FNX_REQUIRE(logits && lse && scratch && err && (!k || (top_lp && top_i)), "logprobs: a null buffer");
     FNX_REQUIRE((uintptr_t) scratch % 16 == 0, "logprobs: scratch not 16-byte aligned");
-    const int ns = lp_splits(n, T, k);
-    LpArgs a{logits, stride, T, n, v0, k, ntok, ns, lp_ship(ns, k), tok, lse, entropy, lp, top_lp, top_i, (unsigned*) scratch, nullptr, nullptr, err};
+    int per;
+    const int ns = lp_splits(n, T, k, &per);
+    LpArgs a{logits, stride, T, n, v0, k, ntok, ns, per, lp_ship(ns, k), tok, lse, entropy, lp, top_lp, top_i, (unsigned*) scratch, nullptr, nullptr, err};
     // the counters have their place whatever the call's sizes, so that one scratch serves calls of different ones
     a.part = reinterpret_cast<LpPart*>((char*) scratch + LP_BLOCKS * 4);
     a.cand = reinterpret_cast<unsigned long long*>(a.part + (size_t) T * ns);
     constexpr size_t ring = (size_t) LP_STAGES * LP_BATCH * 4;
     if (smem_optin(k_logprobs, ring, "logprobs")) return 1;
-    launch(0, k_logprobs, dim3((unsigned) std::min<long long>((long long) T * ns, LP_BLOCKS)), LP_THREADS, ring, strm(st), a);
+    launch(0, k_logprobs, ns > 1 ? dim3(ns, T) : dim3(std::min(T, LP_BLOCKS)), LP_THREADS, ring, strm(st), a);
     return launch_ok("logprobs");
 }
 }

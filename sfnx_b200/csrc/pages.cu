@@ -145,18 +145,15 @@ __global__ void __launch_bounds__(PG_THREADS) k_pages_reserve(const FnxPagePool 
     if (tid == 0) njobs_s = 0u;
     pdl_wait();
     pdl_go();
-    auto free_bits = [&](int q0, unsigned* is) {   // a warp has 128 neighbouring pages of 4 * PG_THREADS
-        int ref[4];
+    auto ask_refs = [&](int q0, int* ref) {   // a warp has 128 neighbouring pages of 4 * PG_THREADS
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const int q = q0 + warp * 128 + k * 32 + lane;
             ref[k] = q < p.npages ? p.ref[q] : 1;
         }
-#pragma unroll
-        for (int k = 0; k < 4; ++k) is[k] = __ballot_sync(0xffffffffu, ref[k] == 0);
     };
-    unsigned is[4];
-    free_bits(0, is);
+    int ref[4];
+    ask_refs(0, ref);
     // ---- what each sequence holds and wants; thread i has `per` neighbouring sequences
     int len[PG_PER], more[PG_PER], tail[PG_PER], want[PG_PER], refs[PG_PER];
     bool bad = false, room = true;
@@ -209,10 +206,11 @@ __global__ void __launch_bounds__(PG_THREADS) k_pages_reserve(const FnxPagePool 
     unsigned got = 0u;
     if (room && !bad)
         for (int q0 = 0; q0 < p.npages && got < pages; q0 += 4 * PG_THREADS) {
-            if (q0) free_bits(q0, is);
+            if (q0) ask_refs(q0, ref);
+            unsigned is[4];
             int mine = 0, before[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) before[k] = mine, mine += __popc(is[k]);
+            for (int k = 0; k < 4; ++k) is[k] = __ballot_sync(0xffffffffu, ref[k] == 0), before[k] = mine, mine += __popc(is[k]);
             if (lane == 0) wcount[warp] = mine;
             __syncthreads();
             const int others = wcount[lane];   // (PG_WARPS = 32)
