@@ -45,9 +45,9 @@ __global__ void __launch_bounds__(TM_THREADS) k_tree_masks(const int* __restrict
 // A block has a run of neighbouring rows, a warp four heads of a row at a time.  A row's queries and K/V are read in f32 and written in
 // f16, 40 us of copying at 5301 rows of 24 + 2 * 4 heads of 256; what stands in the way is the chain before a row can be written (its
 // sequence, its page, its angles in double precision) and what a head costs in shuffles.  So the next row's heads are on their way
-// into shared memory while one is worked on, eight rows' places and angles are made at once, a warp a row, and a lane's elements
-// lie as they are read without conflicts: 52.2 us (5.0 TB/s).  With a block a row, the loads in registers, 62.2; with three blocks a
-// multiprocessor 53.0, with three rows' copies under way 57.8.
+// into shared memory while one is worked on, the next eight rows' places and angles are made before these eight, a warp a row, and a
+// lane's elements lie as they are read without conflicts: 51.0 us (5.1 TB/s; 52.3 with the eight made when they are wanted).  With a block a row, the loads in registers, 62.2; with three blocks a
+// multiprocessor, or three rows' copies under way, it is slower (by 0.9 and 5).
 struct SaArgs {
     const float *qg, *k, *v, *qn, *kn;
     uint16_t *kc, *vc, *q16;
@@ -95,9 +95,9 @@ template <int HD>
 __global__ void __launch_bounds__(SA_THREADS, SA_BLOCKS) k_seqs_append(const __grid_constant__ SaArgs a) {
     constexpr int E = HD / 32, CHUNK = SA_HEADS * SA_WARPS;
     extern __shared__ __align__(16) unsigned char sa_ring[];   // [2][SA_HEADS][SA_WARPS][HD] floats: a warp's own heads
-    __shared__ __align__(16) float sn[SA_WARPS][64], cs[SA_WARPS][64], wt[2][HD];
+    __shared__ __align__(16) float sn[2][SA_WARPS][64], cs[2][SA_WARPS][64], wt[2][HD];
     __shared__ __align__(16) float sums[SA_WARPS][SA_HEADS][E];
-    __shared__ long long place[SA_WARPS];   // of the rows prepared together: where K and V go (-1: nowhere, -2: not even a query)
+    __shared__ long long place[2][SA_WARPS];   // of the rows prepared together: where K and V go (-1: nowhere, -2: not even a query)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nh = a.nq + 2 * a.nkv, chunks = (nh + CHUNK - 1) / CHUNK;
     const int begin = (int) ((long long) a.sq.rows * blockIdx.x / gridDim.x), end = (int) ((long long) a.sq.rows * (blockIdx.x + 1) / gridDim.x);
     const unsigned ring = (unsigned) __cvta_generic_to_shared(sa_ring) + warp * HD * 4;
@@ -127,35 +127,37 @@ __global__ void __launch_bounds__(SA_THREADS, SA_BLOCKS) k_seqs_append(const __g
     const int half = a.nrot / 2, apart = half % 4 ? 0 : half / 4;
     const bool turned = lane * 4 < a.nrot, lower = lane * 4 < half;
     int stage = 0;
-    for (int t0 = begin; t0 < end; t0 += SA_WARPS) {
-        if (t0 > begin) __syncthreads();   // everyone is done with the angles before these
-        if (t0 + warp < end) {
-            const int t = t0 + warp, s = sq_find(a.sq.row0, a.sq.nseq, t);
-            long long at = -2;
-            if (s >= 0) {
-                const int i0 = t - a.sq.row0[s], p0 = a.sq.pos0[s];
-                const int turn = max(0, p0) + (a.depth ? max(0, a.depth[t]) : i0);
-                for (int i = lane; i < half; i += 32) ex_sincos((double) fmul((float) turn, a.freq[i]), &sn[warp][i], &cs[warp][i]);
-                const long long cell = sq_cell(a.sq, a.g, s, p0 < 0 || i0 > INT_MAX - p0 ? -1 : p0 + i0);
-                if (lane == 0 && cell < 0) atomicOr(a.err, SQ_ERR_ROOM);
-                at = cell < 0 ? -1 : (long long) sq_at(a.sq, a.g, cell, row_elems);
-            }
-            if (lane == 0) place[warp] = at;
+    auto prepare = [&](int t, int set) {   // a warp's row of the eight
+        if (t >= end) return;
+        const int s = sq_find(a.sq.row0, a.sq.nseq, t);
+        long long at = -2;
+        if (s >= 0) {
+            const int i0 = t - a.sq.row0[s], p0 = a.sq.pos0[s];
+            const int turn = max(0, p0) + (a.depth ? max(0, a.depth[t]) : i0);
+            for (int i = lane; i < half; i += 32) ex_sincos((double) fmul((float) turn, a.freq[i]), &sn[set][warp][i], &cs[set][warp][i]);
+            const long long cell = sq_cell(a.sq, a.g, s, p0 < 0 || i0 > INT_MAX - p0 ? -1 : p0 + i0);
+            if (lane == 0 && cell < 0) atomicOr(a.err, SQ_ERR_ROOM);
+            at = cell < 0 ? -1 : (long long) sq_at(a.sq, a.g, cell, row_elems);
         }
-        __syncthreads();
-        for (int t = t0; t < min(t0 + SA_WARPS, end); ++t)
+        if (lane == 0) place[set][warp] = at;
+    };
+    int set = 1;
+    for (int t0 = begin - SA_WARPS; t0 < end; t0 += SA_WARPS, set ^= 1) {
+        prepare(t0 + SA_WARPS + warp, set ^ 1);   // the next eight before these
+        if (t0 >= begin)
+            for (int t = t0; t < min(t0 + SA_WARPS, end); ++t)
             for (int chunk = 0; chunk < chunks; ++chunk, stage ^= 1) {
                 __syncwarp();
                 load(chunk + 1 < chunks ? t : t + 1, chunk + 1 < chunks ? chunk + 1 : 0, stage ^ 1);   // (what lay there is in registers and used)
                 asm volatile("cp.async.wait_group 1;" ::: "memory");
                 __syncwarp();
-                const long long at = place[t - t0];
+                const long long at = place[set][t - t0];
                 if (at == -2) continue;   // behind the last sequence
                 const int h0 = chunk * CHUNK + warp;
                 float x[SA_HEADS][E], c[4], d[4];
                 if (turned && apart) {   // the rotation's factors of this lane's elements and of their partners
                     const int i = lane * 4 - (lower ? 0 : half);
-                    sa_get(c, lower ? &cs[t - t0][i] : &sn[t - t0][i]), sa_get(d, lower ? &sn[t - t0][i] : &cs[t - t0][i]);
+                    sa_get(c, lower ? &cs[set][t - t0][i] : &sn[set][t - t0][i]), sa_get(d, lower ? &sn[set][t - t0][i] : &cs[set][t - t0][i]);
                 }
 #pragma unroll
                 for (int b = 0; b < SA_HEADS; ++b)
@@ -216,7 +218,7 @@ __global__ void __launch_bounds__(SA_THREADS, SA_BLOCKS) k_seqs_append(const __g
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
                                 const int i = lane * 4 + e;
-                                const float *sr = sn[t - t0], *cr = cs[t - t0];
+                                const float *sr = sn[set][t - t0], *cr = cs[set][t - t0];
                                 if (i < half) x[b][e] = ffma(-rot[i + half], sr[i], fmul(x[b][e], cr[i]));
                                 else if (i < a.nrot) x[b][e] = ffma(x[b][e], cr[i - half], fmul(rot[i - half], sr[i - half]));
                             }
@@ -232,6 +234,7 @@ __global__ void __launch_bounds__(SA_THREADS, SA_BLOCKS) k_seqs_append(const __g
                         *reinterpret_cast<uint2*>(to + e * 32 + lane * 4) = make_uint2(sq_pack(x[b][e], x[b][e + 1]), sq_pack(x[b][e + 2], x[b][e + 3]));
                 }
             }
+        __syncthreads();
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
 }
