@@ -414,6 +414,7 @@ __global__ void __launch_bounds__(128) k_pages_trim(const FnxPagePool p, void* s
 static int pg_check(const FnxPagePool* p, const void* scratch, const unsigned* err, const char* what) {
     FNX_REQUIRE(p && p->ref && p->pt && p->len && scratch && err, "%s: a null buffer", what);
     FNX_REQUIRE(p->npages >= 1 && p->rows >= 1 && p->pt_stride >= 1, "%s: %d pages of %d rows, tables of %d", what, p->npages, p->rows, p->pt_stride);
+    FNX_REQUIRE(p->npages <= 1 << 30 && p->pt_stride <= 1 << 30, "%s: %d pages, tables of %d (2^30 at most)", what, p->npages, p->pt_stride);
     FNX_REQUIRE(p->nseq >= 1 && p->nseq <= PG_SEQS, "%s: %d sequences outside 1..%d", what, p->nseq, PG_SEQS);
     FNX_REQUIRE((long long) p->rows * p->pt_stride < (1ll << 31), "%s: a table of %d pages of %d rows holds 2^31 positions or more", what, p->pt_stride, p->rows);
     return 0;

@@ -314,6 +314,25 @@ def test_caches_and_calls_smaller_than_a_tile(page, lens, ctx, nq, nkv, hd):
     _check(s, s.attend(torch.from_numpy(bits.view(np.int32)).to(DEV)), bits)
 
 
+@pytest.mark.parametrize("page", [0, 64])
+def test_sequences_without_any_rows(page):
+    """Nothing is attended, appended or masked; rows that belong to nobody stay as they are."""
+    s = S.Seqs([0, 0, 0], [0, 70, 3], 8, 2, 128, page=page, extra_rows=9)
+    bits = np.zeros((0, 1), np.uint32)
+    _, _, _ = s.tree(1)
+    _check(s, s.attend())
+    anc = torch.full((9, 1), -7, dtype=torch.int32, device=DEV)
+    _check(s, s.attend(anc), bits)
+    par, dep = torch.full((9,), -5, dtype=torch.int32, device=DEV), torch.full((9,), -7, dtype=torch.int32, device=DEV)
+    L.call("fnx_tree_masks", par.data_ptr(), L.byref(s.seqs()), anc.data_ptr(), 1, dep.data_ptr(), s.err.data_ptr(), L.stream())
+    k, w = torch.randn(9, 2, 128, device=DEV), torch.ones(128, device=DEV)
+    before = s.kc.clone()
+    q16 = _append(s, k, k, w, w)
+    torch.cuda.synchronize()
+    assert int(s.err) == 0 and (q16 == -7).all() and (anc == -7).all() and (dep == -7).all()
+    assert torch.equal(s.kc.view(torch.int16), before.view(torch.int16))
+
+
 def test_calls_on_two_streams_at_once():
     a, b = S.Seqs([300, 1, 17], [900, 4000, 3], 24, 4, 256, seed=41), S.Seqs([1] * 9, [500 * i for i in range(9)], 8, 2, 128, seed=42)
     want = [x.attend().clone() for x in (a, b)]

@@ -97,6 +97,12 @@ def test_pools_that_make_no_sense(fnx, pool, text):
         fnx.call("fnx_pages_keep", fnx.byref(p), P, P, 4, P, P, 2, g, 2, 128, P, P, None)
 
 
+@pytest.mark.parametrize("pool", [dict(npages=(1 << 30) + 1), dict(rows=1, pt_stride=(1 << 30) + 1)])
+def test_pools_past_2_to_30(fnx, pool):
+    with pytest.raises(fnx.FnxError, match="2\\^30 at most"):
+        fnx.call("fnx_pages_fork", fnx.byref(_pool(fnx, **pool)), P, None, P, P, None)
+
+
 @pytest.mark.parametrize("change,text", [(dict(planes=None), "planes"), (dict(nplanes=0), "0 planes"), (dict(nplanes=65536), "planes"), (dict(hd=96), "of 96"), (dict(nkv=0), "0 KV"),
                                          (dict(rows=32), "pages of 32"), (dict(page=64 * 256 - 8), "a page of"), (dict(page=64 * 256 + 2), "multiple of 8"),
                                          (dict(page=64 * 136 - 8, q8=1), "a page of"), (dict(add=None), "null")])
