@@ -6,8 +6,8 @@
 // and which holder of a shared page keeps it is the lowest, so no order of atomics shows.
 // The tables are a few thousand words: what these calls cost is the latency of a handful of dependent loads and launches, so
 // loads go out before their use is known and divisions are 32 bits wide; the row copies are DRAM's.  Seven forks and their
-// copies of a partly filled page in 24 planes: 11.8 us (three launches; in reserve six dependent loads and four barriers of one
-// block); growth of 32 sequences and their accepted paths in 4 planes: 14.5.
+// copies of a partly filled page in 24 planes: 12.1 us (three launches; in reserve six dependent loads and four barriers of one
+// block); growth of 32 sequences and their accepted paths in 4 planes: 14.7.
 #include <algorithm>
 #include <climits>
 
@@ -278,12 +278,14 @@ __global__ void __launch_bounds__(256) k_pages_copy(const FnxPagePool p, void* c
     const PgScratch w = pg_scratch(p, scratch);
     pdl_wait();
     pdl_go();
+    // a first job's words (there are as many places as sequences) together with the number of jobs
     const int n = *w.njobs;
+    int from = w.jobs[3 * blockIdx.x], to = w.jobs[3 * blockIdx.x + 1], rows = w.jobs[3 * blockIdx.x + 2];
+    char* base = (char*) planes[blockIdx.y];
     for (int job = blockIdx.x; job < n; job += gridDim.x) {
-        const int rows = w.jobs[3 * job + 2];
-        char* base = (char*) planes[blockIdx.y];
-        const char* src = base + (size_t) w.jobs[3 * job] * r.page_bytes;
-        char* dst = base + (size_t) w.jobs[3 * job + 1] * r.page_bytes;
+        if (job != (int) blockIdx.x) from = w.jobs[3 * job], to = w.jobs[3 * job + 1], rows = w.jobs[3 * job + 2];
+        const char* src = base + (size_t) from * r.page_bytes;
+        char* dst = base + (size_t) to * r.page_bytes;
         const size_t bytes = rows * r.row_bytes, lo = (size_t) blockIdx.z * PG_PIECE, hi = min(bytes, lo + PG_PIECE);
         uint4 v[PG_PIECE / (256 * 16)];
 #pragma unroll
@@ -399,9 +401,9 @@ __global__ void __launch_bounds__(128) k_pages_trim(const FnxPagePool p, void* s
     const PgScratch w = pg_scratch(p, scratch);
     pdl_wait();
     pdl_go();
-    const int s = blockIdx.x, len = w.verdict[s];
+    const int s = blockIdx.x, len = w.verdict[s], was = p.len[s];
     if (len < 0) return;
-    const int held = pg_held(p, p.len[s]);
+    const int held = pg_held(p, was);
     __syncthreads();
     for (int j = pg_held(p, len) + threadIdx.x; j < held; j += 128) {
         int* e = p.pt + (size_t) s * p.pt_stride + j;
