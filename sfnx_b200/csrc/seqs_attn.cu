@@ -875,61 +875,72 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(SA_THREADS, 1) k_att
 }
 
 // The parts of units that were cut, joined: where a pair's run ends, a block takes 32 rows of the unit that it cut, a warp eight of
-// their columns, a lane a row, as the parts lie; four parts' loads are in flight together.  With fewer units than runs there are blocks
-// for the units only, which look their run up (a tree of 16 after 3000 positions: 17.3 us with blocks for all runs, 16.6 so).
-constexpr int SJ_PARTS = 4, SJ_PAIRS = 128;
-template <int HD> __global__ void __launch_bounds__(256, 3) k_attn_seqs_join(const __grid_constant__ SqAttn a) {
+// their columns, a lane a row, as the parts lie; PARTS parts' loads are in flight together.  FEW: fewer units than runs, and blocks
+// for the units only, which look their run up (a tree of 16 after 3000 positions: 17.3 us with blocks for all runs and four parts in
+// flight, 16.6 so, with eight; eight short prompts with more units than runs: 32.7 us, with this form's early gates 33.3).
+constexpr int SJ_PAIRS = 128;
+template <int HD, int PARTS, bool FEW> __global__ void __launch_bounds__(256, PARTS == 4 ? 3 : 2) k_attn_seqs_join(const __grid_constant__ SqAttn a) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rank = blockIdx.y >> 2, quarter = blockIdx.y & 3;   // CTA of the pair, quarter of its rows
+    const int qpk = a.nq / a.nkv, m = quarter * 32 + lane, token = m / qpk, hh = m - token * qpk, c = warp + 8 * blockIdx.z;   // c: which eight columns
     pdl_wait();
     pdl_go();
     int g = blockIdx.x;
-    if ((int) gridDim.x < a.pairs - 1) {   // fewer units than runs: the x-th that is cut
-        int count[SJ_PAIRS / 32], which = g;
-        g = a.pairs - 1;   // (nothing is cut at the last run's end)
+    int4 x = make_int4(0, 0, 0, 0);
+    if constexpr (FEW) {   // the x-th that is cut
+        int4 cut[SJ_PAIRS / 32];
+        int which = g;
 #pragma unroll
-        for (int k = 0; k < SJ_PAIRS / 32; ++k) count[k] = k * 32 + lane < a.pairs ? a.cuts[2 * (k * 32 + lane)].x : 0;
+        for (int k = 0; k < SJ_PAIRS / 32; ++k) cut[k] = k * 32 + lane < a.pairs ? a.cuts[2 * (k * 32 + lane)] : make_int4(0, 0, 0, 0);
 #pragma unroll
         for (int k = 0; k < SJ_PAIRS / 32; ++k) {
-            const unsigned some = __ballot_sync(0xffffffffu, count[k] != 0);
-            const unsigned it = __ballot_sync(0xffffffffu, count[k] != 0 && __popc(some & ((1u << lane) - 1u)) == which);
-            if (it) g = k * 32 + __ffs(it) - 1;
+            const unsigned some = __ballot_sync(0xffffffffu, cut[k].x != 0);
+            const unsigned it = __ballot_sync(0xffffffffu, cut[k].x != 0 && __popc(some & ((1u << lane) - 1u)) == which);
+            if (it) {
+                const int l = __ffs(it) - 1;
+                g = k * 32 + l;
+                x = make_int4(__shfl_sync(0xffffffffu, cut[k].x, l), __shfl_sync(0xffffffffu, cut[k].y, l), __shfl_sync(0xffffffffu, cut[k].z, l),
+                              __shfl_sync(0xffffffffu, cut[k].w, l));
+            }
             which -= __popc(some);
         }
+    } else {
+        x = a.cuts[2 * g];
     }
-    const int4 x = a.cuts[2 * g];
-    const int qpk = a.nq / a.nkv, m = quarter * 32 + lane, rows = min(a.tok, x.w - rank * a.tok) * qpk, n = x.x;
-    if (!n || m >= rows) return;
-    const int head = a.cuts[2 * g + 1].x * qpk + m % qpk, c = warp + 8 * blockIdx.z;   // c: which eight columns
-    const size_t row = (size_t) x.z + rank * a.tok + m / qpk;
-    const float* gate = a.qg ? a.qg + (row * a.nq + head) * 2 * HD + HD + c * 8 : nullptr;
-    if (gate) l2_ask(gate);
+    const int n = x.x;
+    if (!n || m >= min(a.tok, x.w - rank * a.tok) * qpk) return;
+    const int head = a.cuts[2 * g + 1].x * qpk + hh;
+    const size_t row = (size_t) x.z + rank * a.tok + token;
+    const float4* gates = reinterpret_cast<const float4*>(a.qg + (row * a.nq + head) * 2 * HD + HD + c * 8);
+    float4 gate[2];
+    if (!FEW && a.qg) l2_ask(reinterpret_cast<const float*>(gates));
     auto slot = [&](int p) { return (p ? 2 * (g + p) : x.y) * 2 + rank; };
     const float4* part = a.part + (quarter * (HD / 4) + c * 2) * 32 + lane;
     float top = -INFINITY, z = 0.f, acc[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) acc[k] = 0.f;
 #pragma unroll 1
-    for (int p0 = 0; p0 < n; p0 += SJ_PARTS) {
-        float2 q[SJ_PARTS];
-        float4 v[SJ_PARTS][2];
+    for (int p0 = 0; p0 < n; p0 += PARTS) {
+        float2 q[PARTS];
+        float4 v[PARTS][2];
 #pragma unroll
-        for (int i = 0; i < SJ_PARTS; ++i) {
+        for (int i = 0; i < PARTS; ++i) {
             q[i] = make_float2(-INFINITY, 0.f), v[i][0] = v[i][1] = make_float4(0.f, 0.f, 0.f, 0.f);
             if (p0 + i >= n) continue;
             const int at = slot(p0 + i);
             q[i] = a.mz[at * SA_ROWS + m];
             v[i][0] = part[at * (SA_ROWS * HD / 4)], v[i][1] = part[at * (SA_ROWS * HD / 4) + 32];
         }
+        if (FEW && !p0 && a.qg) gate[0] = gates[0], gate[1] = gates[1];   // behind the first parts' loads
         float most = top;
 #pragma unroll
-        for (int i = 0; i < SJ_PARTS; ++i) most = fmaxf(most, q[i].x);
+        for (int i = 0; i < PARTS; ++i) most = fmaxf(most, q[i].x);
         if (most == -INFINITY) continue;   // the row sees nothing there
         const float f0 = top == -INFINITY ? 0.f : ex2_ftz(top - most);
         top = most, z *= f0;
 #pragma unroll
         for (int k = 0; k < 8; ++k) acc[k] *= f0;
 #pragma unroll
-        for (int i = 0; i < SJ_PARTS; ++i) {
+        for (int i = 0; i < PARTS; ++i) {
             const float f = q[i].x == -INFINITY ? 0.f : ex2_ftz(q[i].x - top);
             z = fmaf(f, q[i].y, z);
             acc[0] = fmaf(f, v[i][0].x, acc[0]), acc[1] = fmaf(f, v[i][0].y, acc[1]), acc[2] = fmaf(f, v[i][0].z, acc[2]), acc[3] = fmaf(f, v[i][0].w, acc[3]);
@@ -939,14 +950,12 @@ template <int HD> __global__ void __launch_bounds__(256, 3) k_attn_seqs_join(con
     const float inv = z == 0.f ? 0.f : 1.0f / z;
 #pragma unroll
     for (int k = 0; k < 8; ++k) acc[k] *= inv;
-    if (gate) {
-        const float4 t0 = *reinterpret_cast<const float4*>(gate), t1 = *reinterpret_cast<const float4*>(gate + 4);
-        sa_gate(acc[0], acc[1], t0.x, t0.y), sa_gate(acc[2], acc[3], t0.z, t0.w), sa_gate(acc[4], acc[5], t1.x, t1.y), sa_gate(acc[6], acc[7], t1.z, t1.w);
-    }
-    unsigned u[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) u[e] = sq_pack(acc[2 * e], acc[2 * e + 1]);
-    *reinterpret_cast<uint4*>(a.out + row * a.out_stride + (size_t) head * HD + c * 8) = make_uint4(u[0], u[1], u[2], u[3]);
+    if (!FEW && a.qg) gate[0] = gates[0], gate[1] = gates[1];
+    if (a.qg)
+        sa_gate(acc[0], acc[1], gate[0].x, gate[0].y), sa_gate(acc[2], acc[3], gate[0].z, gate[0].w), sa_gate(acc[4], acc[5], gate[1].x, gate[1].y),
+            sa_gate(acc[6], acc[7], gate[1].z, gate[1].w);
+    *reinterpret_cast<uint4*>(a.out + row * a.out_stride + (size_t) head * HD + c * 8) =
+        make_uint4(sq_pack(acc[0], acc[1]), sq_pack(acc[2], acc[3]), sq_pack(acc[4], acc[5]), sq_pack(acc[6], acc[7]));
 }
 
 static long long sq_units(const FnxSeqs* sq, int tok, int nkv) {   // at most
@@ -969,7 +978,10 @@ template <int HD> static int sq_launch(const SqMaps& maps, const SqAttn& a, long
     if (a.pairs == 1) return 0;
     const int qpk = a.nq / a.nkv, most = std::min(a.sq.rows, 2 * a.tok);   // tokens of a unit
     const int quarters = most > a.tok ? 4 + ((most - a.tok) * qpk + 31) / 32 : (most * qpk + 31) / 32;
-    launch(0, k_attn_seqs_join<HD>, dim3((unsigned) std::min<long long>(a.pairs - 1, units), quarters, HD / 64), 256, 0, st, a);
+    const dim3 grid((unsigned) std::min<long long>(a.pairs - 1, units), quarters, HD / 64);
+    if ((int) grid.x == a.pairs - 1) launch(0, k_attn_seqs_join<HD, 4, false>, grid, 256, 0, st, a);
+    else if (grid.x * grid.y * grid.z > (unsigned) sq_processors()) launch(0, k_attn_seqs_join<HD, 4, true>, grid, 256, 0, st, a);
+    else launch(0, k_attn_seqs_join<HD, 8, true>, grid, 256, 0, st, a);   // few blocks, with many parts each
     return launch_ok(what);
 }
 
