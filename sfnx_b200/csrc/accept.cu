@@ -203,6 +203,10 @@ int fnx_logprobs_merge(const float* lse_s, const float* entropy_s, const float* 
         }
         int head[MOST] = {};
         for (int j = 0; j < k; ++j) {   // every slice's list is in order: the best of the heads
+            if (nan) {   // no order to speak of, in the whole row
+                top_i[(size_t) t * k + j] = -1, top_lp[(size_t) t * k + j] = lse[t];
+                continue;
+            }
             int best = -1, bi = 0;
             float bx = 0.f;
             for (int i = 0; i < nslice; ++i) {
@@ -214,7 +218,7 @@ int fnx_logprobs_merge(const float* lse_s, const float* entropy_s, const float* 
             }
             ++head[best];
             top_i[(size_t) t * k + j] = bi;
-            top_lp[(size_t) t * k + j] = nan ? lse[t] : none || bx == ninf ? ninf : (float) (bx - all);
+            top_lp[(size_t) t * k + j] = none || bx == ninf ? ninf : (float) (bx - all);
         }
     }
     return 0;
