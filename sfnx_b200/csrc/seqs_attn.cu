@@ -12,9 +12,9 @@
 // reference, z), and a second kernel joins the parts.
 // S = Q K^T (256 x 128 fp32, operands in shared memory) and O += P V (P in tensor memory as the A operand, V as it lies: dims
 // contiguous, "MN-major") both accumulate in tensor memory, each CTA's rows in its own.  Roles: warp 0 copies (TMA, K and V
-// boxes found through the page table), warp 2 tells the pair's first CTA what has landed, warp 1 of that CTA issues the MMAs,
-// warps 4 - 11 take the softmax step: a thread has one row and half of a tile's columns, the halves of a row agree on the
-// maximum through shared memory.
+// boxes found through the page table; both CTAs' copies count on the first one's barriers), warp 1 of the first CTA issues the MMAs,
+// warp 2 clears V rows behind a sequence's newest, warps 4 - 11 take the softmax step: a thread has one row and half of a tile's columns,
+// the halves of a row agree on the maximum through shared memory.
 //   tensor memory: O (HD columns), one S tile (128), two P tiles (64 columns each, f16 pairs).  S(i + 1) is issued when the softmax
 //   warps have S(i) in registers, and O += P(i - 1) V(i - 1) behind it, so the tensor core has both to do while they take
 //   exponentials: a tile costs the longer of the two, not the sum.  (With O += P(i) V(i) issued as soon as P(i) is written, S(i + 1)
@@ -67,7 +67,7 @@ struct SqAttn {
     uint16_t* out;
     int out_stride, nq, nkv, words;
     int tok;      // tokens of a CTA's rows: 128 / qpk
-    int box;      // cache rows a copy brings: a power of two that divides a page's rows
+    int box, lg;  // cache rows a copy brings: a power of two that divides a page's rows; its logarithm
     int pairs;    // the scan's pairs of CTAs
     float4* part; // parts of units, as the threads hold them: [2 pairs][2][4 quarters of the rows][HD / 4][32 rows]
     float2* mz;   // their (ref, z): [2 pairs][2][128]
@@ -78,17 +78,15 @@ struct SqAttn {
 __device__ __forceinline__ void sa_init(unsigned long long* bar, unsigned n) {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(um_s32(bar)), "r"(n));
 }
-__device__ __forceinline__ void sa_arrive(unsigned long long* bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(um_s32(bar)) : "memory");
+// arrives at the barrier of the pair's first CTA that lies there where `bar` does in this one (`first`: from this one's addresses to that
+// one's): sa_tell for tensor memory, whose accesses are ordered by the tcgen05 fences; sa_tell_shared for what this CTA's threads have
+// written to shared memory, which is released to the cluster and acquired there at that scope (a release takes 1000 cycles: with one a
+// tile, twelve single tokens took 139 us instead of 104)
+__device__ __forceinline__ void sa_tell(unsigned long long* bar, unsigned first) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(um_s32(bar) + first) : "memory");
 }
-// arrives at the barrier of the pair's first CTA that lies where `bar` does in this one: for what was written to shared memory,
-// and for tensor memory, whose accesses are ordered by the tcgen05 fences (a release to the cluster takes 1000 cycles)
-__device__ __forceinline__ void sa_tell_shared(unsigned long long* bar) {
-    asm volatile("{\n\t.reg .b32 r;\n\tmapa.shared::cluster.u32 r, %0, 0;\n\tmbarrier.arrive.release.cluster.shared::cluster.b64 _, [r];\n\t}" ::"r"(um_s32(bar))
-                 : "memory");
-}
-__device__ __forceinline__ void sa_tell(unsigned long long* bar) {
-    asm volatile("{\n\t.reg .b32 r;\n\tmapa.shared::cluster.u32 r, %0, 0;\n\tmbarrier.arrive.shared::cluster.b64 _, [r];\n\t}" ::"r"(um_s32(bar)) : "memory");
+__device__ __forceinline__ void sa_tell_shared(unsigned long long* bar, unsigned first) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(um_s32(bar) + first) : "memory");
 }
 // both CTAs of the pair, every thread.  Without a release (1000 cycles): before it come the barriers' own fence and a barrier of the
 // CTA for what that shares, or nothing that the other one reads
@@ -96,14 +94,15 @@ __device__ __forceinline__ void sa_cluster() {
     __syncwarp();
     asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ void sa_tma4d(unsigned dst, const CUtensorMap* map, int x, int y, int z, int w, unsigned long long* bar) {
-    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst), "l"(map),
-                 "r"(x), "r"(y), "r"(z), "r"(w), "r"(um_s32(bar))
+// boxes into this CTA's shared memory (plain loads: no multicast), their bytes counted on `bar`, an address in either CTA of the pair
+__device__ __forceinline__ void sa_tma4d(unsigned dst, const CUtensorMap* map, int x, int y, int z, int w, unsigned bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+                 "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
                  : "memory");
 }
-__device__ __forceinline__ void sa_tma3d(unsigned dst, const CUtensorMap* map, int x, int y, int z, unsigned long long* bar) {
-    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(map),
-                 "r"(x), "r"(y), "r"(z), "r"(um_s32(bar))
+__device__ __forceinline__ void sa_tma3d(unsigned dst, const CUtensorMap* map, int x, int y, int z, unsigned bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+                 "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
                  : "memory");
 }
 // the pair's MMAs, 256 rows: D[tmem] (+)= A B, each CTA's half of A's rows and of B's columns in its own memories
@@ -317,6 +316,9 @@ __device__ __forceinline__ void sq_cut(const SqAttn& a, const SqPlan& plan, cons
     head = u.head;
 }
 
+// whether V rows behind the newest position lie in the last 16 that tile t's product takes
+__device__ __forceinline__ bool sq_unclean(int kv_len, int t) { return kv_len - t * SA_KT < SA_KT && kv_len % 16; }
+
 // Waits for a phase of `bar`, at most `spins` polls of up to 16 us (asleep: warps that poll without a break keep the barriers'
 // unit from the one that issues the MMAs); a wait that ran out is reported, and later ones of the thread do not linger
 constexpr int SA_SPINS = 1 << 16;
@@ -324,6 +326,17 @@ __device__ __forceinline__ bool sa_wait(unsigned long long* bar, unsigned parity
     unsigned ok = 0;
     for (int spin = 0; spin < spins && !ok; ++spin)
         asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                     : "=r"(ok)
+                     : "r"(um_s32(bar)), "r"(parity), "r"(16384u)
+                     : "memory");
+    if (!ok) spins = 1, atomicOr(fault, 8u);
+    return ok != 0;
+}
+// the same for what both CTAs' threads have released with sa_tell_shared
+__device__ __forceinline__ bool sa_wait_shared(unsigned long long* bar, unsigned parity, int& spins, unsigned* fault) {
+    unsigned ok = 0;
+    for (int spin = 0; spin < spins && !ok; ++spin)
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
                      : "=r"(ok)
                      : "r"(um_s32(bar)), "r"(parity), "r"(16384u)
                      : "memory");
@@ -373,6 +386,7 @@ __device__ __forceinline__ void sa_gate(float& y0, float& y1, float g0, float g1
 __device__ __forceinline__ bool sa_wait_warp(unsigned long long* bar, unsigned parity, int& spins, unsigned* fault) {
     bool ok = true;
     if (um_elect()) ok = sa_wait(bar, parity, spins, fault);
+    __syncwarp();   // what that lane has seen, all have
     return __all_sync(0xffffffffu, ok);
 }
 
@@ -383,16 +397,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(SA_THREADS, 1) k_att
     unsigned char *Q = sa_smem, *ring = Q + S::QBYTES, *strips = ring + S::SLOTS * S::SLOT;
     float* xmax = reinterpret_cast<float*>(strips + SA_SOFT / 32 * SA_STRIP);   // [2][2][128] the halves' maxima, of odd and even tiles
     unsigned long long* bars = reinterpret_cast<unsigned long long*>(xmax + 4 * SA_ROWS);
-    // full, q_full: this CTA's copies have landed.  ready, q_ready, s_free, p_full, o_free count both CTAs', in the first one's
+    // ready, q_ready: both CTAs' copies have landed (their bytes, which the first CTA expects).  full: this CTA's copy of V rows of which some
+    // are to be cleared; clean: that is done.  ready, q_ready, clean, s_free, p_full, o_free count both CTAs', in the first one's
     // memory.  empty, q_empty, s_full, o_full: MMAs are done, told to both
-    unsigned long long *full = bars, *empty = full + S::SLOTS, *ready = empty + S::SLOTS, *q_full = ready + S::SLOTS, *q_ready = q_full + 1, *q_empty = q_full + 2,
-                       *s_full = q_full + 3, *s_free = q_full + 4, *o_free = q_full + 5, *idle = q_full + 6, *p_full = q_full + 7, *o_full = q_full + 9;
-    volatile unsigned *tmem_at = reinterpret_cast<unsigned*>(q_full + 11), *work_at = tmem_at + 1;
-    volatile int* run_at = reinterpret_cast<int*>(q_full + 12);
+    unsigned long long *full = bars, *empty = full + S::SLOTS, *ready = empty + S::SLOTS, *clean = ready + S::SLOTS, *q_ready = clean + 1, *q_empty = clean + 2,
+                       *s_full = clean + 3, *s_free = clean + 4, *o_free = clean + 5, *idle = clean + 6, *p_full = clean + 7, *o_full = clean + 9;
+    volatile unsigned *tmem_at = reinterpret_cast<unsigned*>(clean + 11), *work_at = tmem_at + 1;
+    volatile int* run_at = reinterpret_cast<int*>(clean + 12);
     const int tid = threadIdx.x, warp = (int) um_uniform(tid >> 5), lane = tid & 31, rank = blockIdx.x & 1, g = blockIdx.x >> 1;
+    unsigned first;
+    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(first) : "r"(um_s32(bars)));
+    first -= um_s32(bars);
     if (tid == 0) {
         for (int i = 0; i < S::SLOTS; ++i) sa_init(&full[i], 1), sa_init(&empty[i], 1), sa_init(&ready[i], 2);
-        sa_init(q_full, 1), sa_init(q_ready, 2), sa_init(q_empty, 1), sa_init(s_full, 1), sa_init(s_free, 2 * SA_SOFT / 32), sa_init(o_free, 2 * SA_SOFT / 32);
+        sa_init(clean, 2), sa_init(q_ready, 1), sa_init(q_empty, 1), sa_init(s_full, 1), sa_init(s_free, 2 * (SA_SOFT / 32 + 1)), sa_init(o_free, 2 * SA_SOFT / 32);
         sa_init(idle, 1);
         for (int i = 0; i < 2; ++i) sa_init(&p_full[i], 2 * SA_SOFT / 32), sa_init(&o_full[i], 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -462,6 +480,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(SA_THREADS, 1) k_att
         // ---- copies.  Load number c of the ring takes slot c % SLOTS; tile i's K load comes before tile i - 2's V load.  A slot
         // holds groups of 64 rows, each as column blocks of 64 dims (8 KB, swizzled)
         int c = 0, nseg = 0, kv0 = 0;
+        unsigned odd = 0u;    // of a slot's bit: how often `full` was used
         bool zeroed = true;   // Q
         SqRun r;
         r.get(run_at);
@@ -475,36 +494,45 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(SA_THREADS, 1) k_att
             const int p = tile * SA_KT + lane * a.box;
             y = a.sq.pt ? p % a.g.rows : kv0 + p, z = !a.sq.pt ? 0 : e >= 0 && e < a.sq.npages ? e : a.sq.npages;
         };
-        // rows lo .. lo + rows - 1 of a tile, nb column blocks from block x on, into the next slot
-        auto load = [&](const CUtensorMap* map, int tile, int y, int z, int lo, int rows, int x, int nb) {
+        // boxes of a tile's rows lo .. lo + rows - 1 that have positions
+        auto boxes = [&](int tile, int lo, int rows) { return max(0, (min(rows, r.u.kv_len - tile * SA_KT - lo) + a.box - 1) >> a.lg); };
+        // those rows, nb column blocks from block x on, into the next slot; `bytes`: of both CTAs' loads; `dirty`: some rows will be cleared
+        auto load = [&](const CUtensorMap* map, int tile, int y, int z, int lo, int rows, int x, int nb, int bytes, bool dirty) {
             const int slot = c % S::SLOTS;
             if (c >= S::SLOTS) alive = alive && sa_wait_warp(&empty[slot], (unsigned) (c / S::SLOTS - 1) & 1u, spins, a.fault);
             if (!alive) return;
-            const int have = min(rows, r.u.kv_len - tile * SA_KT - lo);
-            const unsigned dst = um_s32(ring) + slot * S::SLOT;
+            const int nbox = boxes(tile, lo, rows);
+            const unsigned dst = um_s32(ring) + slot * S::SLOT, bar = dirty ? um_s32(&full[slot]) : um_s32(&ready[slot]) + first;
+            const bool elected = um_elect();
+            if (elected && dirty) um_expect_tx(&full[slot], (unsigned) (nbox * nb * 128 << a.lg));
+            if (dirty) odd ^= 1u << slot;
             if (a.box == 64) {   // a box is a group, with its column blocks
                 const int y0 = __shfl_sync(0xffffffffu, y, lo / 64), z0 = __shfl_sync(0xffffffffu, z, lo / 64), y1 = __shfl_sync(0xffffffffu, y, 1),
                           z1 = __shfl_sync(0xffffffffu, z, 1);
-                if (um_elect()) {
-                    um_expect_tx(&full[slot], (unsigned) (have > 64 ? 2 : have > 0 ? 1 : 0) * nb * 8192);
-                    if (have > 0) sa_tma4d(dst, map, 0, y0, x, z0, &full[slot]);
-                    if (have > 64) sa_tma4d(dst + nb * 8192, map, 0, y1, x, z1, &full[slot]);
-                }
+                if (elected && nbox > 0) sa_tma4d(dst, map, 0, y0, x, z0, bar);
+                if (elected && nbox > 1) sa_tma4d(dst + nb * 8192, map, 0, y1, x, z1, bar);
             } else {
-                const int nbox = max(0, (have + a.box - 1) / a.box);
-                const bool elected = um_elect();
-                if (elected) um_expect_tx(&full[slot], (unsigned) (nbox * nb * a.box * 128));
                 for (int j = 0; j < nbox; ++j) {
                     const int at = lo / a.box + j, yj = __shfl_sync(0xffffffffu, y, at), zj = __shfl_sync(0xffffffffu, z, at), row = j * a.box;
                     if (elected)
-                        for (int b = 0; b < nb; ++b) sa_tma4d(dst + (row / 64 * nb + b) * 8192 + row % 64 * 128, map, 0, yj, x + b, zj, &full[slot]);
+                        for (int b = 0; b < nb; ++b) sa_tma4d(dst + (row / 64 * nb + b) * 8192 + row % 64 * 128, map, 0, yj, x + b, zj, bar);
                 }
+            }
+            if (elected) {   // behind the copies, whose bytes may be counted first: the phase lasts until both CTAs are here
+                if (rank == 0) um_expect_tx(&ready[slot], dirty ? 0u : (unsigned) bytes);
+                else sa_tell(&ready[slot], first);   // (so that no slot goes round without this CTA, which may have no box to load)
             }
             __syncwarp();
             ++c;
         };
-        auto load_k = [&](int t, int y, int z) { load(&maps.k, t, y, z, rank * (SA_KT / 2), SA_KT / 2, r.u.head * (HD / 64), HD / 64); };
-        auto load_v = [&](int t, int y, int z) { load(&maps.v, t, y, z, 0, SA_KT, r.u.head * (HD / 64) + rank * (HD / 128), HD / 128); };
+        auto load_k = [&](int t, int y, int z) {
+            const int both = boxes(t, 0, SA_KT / 2) + boxes(t, SA_KT / 2, SA_KT / 2);
+            load(&maps.k, t, y, z, rank * (SA_KT / 2), SA_KT / 2, r.u.head * (HD / 64), HD / 64, both * (HD / 64) * 128 << a.lg, false);
+        };
+        auto load_v = [&](int t, int y, int z) {
+            const int both = 2 * boxes(t, 0, SA_KT);
+            load(&maps.v, t, y, z, 0, SA_KT, r.u.head * (HD / 64) + rank * (HD / 128), HD / 128, both * (HD / 128) * 128 << a.lg, sq_unclean(r.u.kv_len, t));
+        };
         for (bool more = work; more && alive; more = r.next(a)) {
             if (!r.n) continue;
             kv0 = !a.sq.pt && a.sq.kv0 ? a.sq.kv0[r.u.s] : 0;
@@ -513,20 +541,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(SA_THREADS, 1) k_att
             if (nseg) alive = sa_wait_warp(q_empty, (unsigned) (nseg - 1) & 1u, spins, a.fault);   // the scores before are done
             if (!alive) break;
             const int tok0 = r.u.tok0 + rank * a.tok;
+            if (rank == 0 && um_elect()) um_expect_tx(q_ready, (unsigned) ((tok0 + a.tok < r.u.len ? 2 : 1) * a.tok * qpk * HD * 2));
             if (tok0 < r.u.len) {
-                if (um_elect()) {
-                    um_expect_tx(q_full, (unsigned) (a.tok * qpk * HD * 2));
-                    for (int b = 0; b < HD / 64; ++b) sa_tma3d(um_s32(Q) + b * (SA_ROWS * 128), &maps.q, b * 64, r.u.head * qpk, r.u.r0 + tok0, q_full);
-                }
+                if (um_elect())
+                    for (int b = 0; b < HD / 64; ++b) sa_tma3d(um_s32(Q) + b * (SA_ROWS * 128), &maps.q, b * 64, r.u.head * qpk, r.u.r0 + tok0, um_s32(q_ready) + first);
                 zeroed = false;
-            } else {   // no rows of this CTA's: products with zeros take less power than with what lies there
-                if (!zeroed) {
-                    for (int i = lane; i < S::QBYTES / 16; i += 32) reinterpret_cast<uint4*>(Q)[i] = make_uint4(0u, 0u, 0u, 0u);
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    __syncwarp();
-                    zeroed = true;
-                }
-                if (um_elect()) sa_arrive(q_full);
+            } else if (!zeroed) {   // no rows of this CTA's: products with zeros take less power than with what lies there (no result depends on it)
+                for (int i = lane; i < S::QBYTES / 16; i += 32) reinterpret_cast<uint4*>(Q)[i] = make_uint4(0u, 0u, 0u, 0u);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                zeroed = true;
             }
             __syncwarp();
             ++nseg;
@@ -548,53 +571,46 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(SA_THREADS, 1) k_att
                 y0 = y1, z0 = z1, y1 = y2, z1 = z2;
             }
         }
-        // nothing is in flight when the block ends: the last loads have landed (a load over another waited for that one's use)
+        // nothing is in flight when the blocks end: the last loads have landed (a load over another waited for that one's use).  The second
+        // CTA's count on the first one's barriers, and it waits for that one in leave()
         if (lane == 0) {
             spins = SA_SPINS;
-            if (nseg) sa_wait(q_full, (unsigned) (nseg - 1) & 1u, spins, a.fault);
-            for (int k = max(0, c - S::SLOTS); k < c; ++k) sa_wait(&full[k % S::SLOTS], (unsigned) (k / S::SLOTS) & 1u, spins, a.fault);
+            if (rank == 0) {
+                if (nseg) sa_wait(q_ready, (unsigned) (nseg - 1) & 1u, spins, a.fault);
+                for (int k = max(0, c - S::SLOTS); k < c; ++k) sa_wait(&ready[k % S::SLOTS], (unsigned) (k / S::SLOTS) & 1u, spins, a.fault);
+            }
+            for (int k = 0; k < S::SLOTS; ++k) sa_wait(&full[k], (odd >> k & 1u) ^ 1u, spins, a.fault);   // (true at once where it was not used)
         }
         __syncwarp();
     } else if (warp == 2) {
-        // ---- what has landed here, told to the first CTA in the order of the loads; V rows past the newest position cleared first
-        int c = 0, nseg = 0;
+        // ---- V rows past the newest position, of the last step of 16 that is multiplied, cleared where they have landed.  This warp follows
+        // the tiles by their scores, and S(i + 1) waits for it too: a phase met once, and no wait longer than a tile's
+        int c = 0, j = 0;
+        unsigned odd = 0u;
         SqRun r;
         r.get(run_at);
-        bool alive = true;
-        auto landed = [&](int clear, int upto) {
-            const int slot = c % S::SLOTS;
-            alive = alive && sa_wait_warp(&full[slot], (unsigned) (c / S::SLOTS) & 1u, spins, a.fault);
-            if (!alive) return;
-            if (clear < upto) {
-                for (int x = clear; x < upto; ++x)
-                    for (int y = lane; y < HD / 16; y += 32)
-                        *reinterpret_cast<uint4*>(ring + slot * S::SLOT + ((x >> 6) * (HD / 128) + (y >> 3)) * 8192 + (x & 63) * 128 + (y & 7) * 16) =
-                            make_uint4(0u, 0u, 0u, 0u);
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) sa_tell_shared(&ready[slot]);
-            } else if (lane == 0) {
-                sa_tell(&ready[slot]);
-            }
-            ++c;
-        };
-        for (bool more = work; more && alive; more = r.next(a)) {
+        for (bool more = work; more; more = r.next(a)) {
             if (!r.n) continue;
-            alive = sa_wait_warp(q_full, (unsigned) nseg & 1u, spins, a.fault);
-            if (!alive) break;
-            if (lane == 0) sa_tell(q_ready);
-            ++nseg;
-            landed(0, 0);
-            if (r.n > 1) landed(0, 0);
-            for (int t = r.t0; t < r.t0 + r.n && alive; ++t) {
-                if (t + 2 < r.t0 + r.n) landed(0, 0);
-                const int have = min(SA_KT, r.u.kv_len - t * SA_KT);
-                landed(have, (have + 15) / 16 * 16);   // of the last step of 16 positions
+            for (int i = 0; i < r.n; ++i, ++j) {
+                sa_wait_warp(s_full, (unsigned) j & 1u, spins, a.fault);
+                if (lane == 0) sa_tell(s_free, first);
             }
+            c += 2 * r.n;
+            const int t = r.t0 + r.n - 1;
+            if (!sq_unclean(r.u.kv_len, t)) continue;
+            const int slot = (c - 1) % S::SLOTS, have = r.u.kv_len - t * SA_KT;   // the segment's last load
+            sa_wait_warp(&full[slot], odd >> slot & 1u, spins, a.fault);
+            odd ^= 1u << slot;
+            for (int x = have; x % 16; ++x)
+                for (int y = lane; y < HD / 16; y += 32)
+                    *reinterpret_cast<uint4*>(ring + slot * S::SLOT + ((x >> 6) * (HD / 128) + (y >> 3)) * 8192 + (x & 63) * 128 + (y & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) sa_tell_shared(clean, first);
         }
     } else if (warp == 1 && rank == 0) {
         // ---- the pair's MMAs, one lane's work from wait to commit
-        int c = 0, j = 0, nseg = 0;   // slots used in the order of their loads (the elected lane's); tiles; segments
+        int c = 0, j = 0, nseg = 0, ncl = 0;   // slots used in the order of their loads (the elected lane's); tiles; segments; cleared tiles
         bool alive = true;            // the elected lane's
         SqRun r;
         r.get(run_at);
@@ -624,6 +640,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(SA_THREADS, 1) k_att
             const int slot = c % S::SLOTS, steps = (min(r.u.kv_len - t * SA_KT, SA_KT) + 15) / 16;   // of 16 positions that exist
             wait(&ready[slot], (unsigned) (c / S::SLOTS) & 1u);
             ++c;
+            if (sq_unclean(r.u.kv_len, t)) alive = alive && sa_wait_shared(clean, (unsigned) ncl & 1u, spins, a.fault), ++ncl;
             if (!alive) return;
             unsigned long long dv = um_desc_x(um_s32(ring) + slot * S::SLOT, 8192, 1024, 2);
             unsigned dp = tm + S::COL_P + (j & 1) * (SA_KT / 2), more = (unsigned) (t - r.t0);
@@ -711,12 +728,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(SA_THREADS, 1) k_att
                 }
                 for (int i = 0; i < r.n; ++i, ++j) {
                     wait(s_full, (unsigned) j & 1u);   // (the scores were issued behind p_full of two tiles before: no phase is met twice)
-                    if (lane == 0) sa_tell(s_free), sa_tell(&p_full[j & 1]);
+                    if (lane == 0) sa_tell(s_free, first), sa_tell(&p_full[j & 1], first);
                     agree();
                 }
                 agree(); agree();
                 if (r.n) wait(&o_full[(j - 1) & 1], (unsigned) ((j - 1) >> 1) & 1u);
-                if (r.n && lane == 0) sa_tell(o_free);
+                if (r.n && lane == 0) sa_tell(o_free, first);
                 continue;
             }
             zeroed = false;
@@ -737,7 +754,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(SA_THREADS, 1) k_att
                 sa_wait_ld();
                 sa_before();
                 __syncwarp();
-                if (lane == 0) sa_tell(s_free);
+                if (lane == 0) sa_tell(s_free, first);
                 const int p0 = (r.t0 + i) * SA_KT + half * 64;
                 if (p0 + 64 > clear) {
                     unsigned see0 = sq_first(lim - p0), see1 = sq_first(lim - p0 - 32);
@@ -795,7 +812,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(SA_THREADS, 1) k_att
                 sa_wait_st();
                 sa_before();
                 __syncwarp();
-                if (lane == 0) sa_tell(&p_full[j & 1]);
+                if (lane == 0) sa_tell(&p_full[j & 1], first);
             }
             // ---- the rows' results: through the warp's strip, so that a line of 32 columns leaves (and its gates come) whole
             float* xm = xmax + (j & 1) * 2 * SA_ROWS;   // the last tile's are in the other half
@@ -837,7 +854,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(SA_THREADS, 1) k_att
                     if (st == STRIPS - 1) {   // O is in registers
                         sa_before();
                         __syncwarp();
-                        if (lane == 0) sa_tell(o_free);
+                        if (lane == 0) sa_tell(o_free, first);
                     }
                 }
                 if (__any_sync(0xffffffffu, none || !r.n))   // rows that saw nothing
@@ -995,8 +1012,8 @@ static int attn_seqs(const uint16_t* q16, int q_stride, const float* qg, const u
                 "%s: rows of %d halves %d and %d apart (multiples of 8)", what, nq * hd, q_stride, out_stride);
     FNX_REQUIRE(!sq->pt || g.rows % 8 == 0, "%s: pages of %d rows (a multiple of 8)", what, g.rows);
     const int qpk = nq / nkv, tok = SA_ROWS / qpk;
-    int box = 64;
-    while (sq->pt && g.rows % box) box /= 2;
+    int box = 64, lg = 6;
+    while (sq->pt && g.rows % box) box /= 2, --lg;
     unsigned* fault = device_fault_word();
     UmEncode enc = um_encoder();
     FNX_REQUIRE(fault && enc, "%s: no fault word or no tensor-map encoder", what);
@@ -1020,7 +1037,7 @@ static int attn_seqs(const uint16_t* q16, int q_stride, const float* qg, const u
     const int pairs = (int) std::max(1ll, std::min((long long) std::min(sq_processors() / 2, SJ_PAIRS), (most + SA_LEAST - 1) / SA_LEAST));
     float4* part = (float4*) scratch;
     float2* mz = reinterpret_cast<float2*>(part + (size_t) 4 * pairs * SA_ROWS * (hd / 4));
-    const SqAttn a{qg, g, *sq, anc, out, out_stride, nq, nkv, words, tok, box, pairs, part, mz, reinterpret_cast<int4*>(mz + (size_t) 4 * pairs * SA_ROWS), fault};
+    const SqAttn a{qg, g, *sq, anc, out, out_stride, nq, nkv, words, tok, box, lg, pairs, part, mz, reinterpret_cast<int4*>(mz + (size_t) 4 * pairs * SA_ROWS), fault};
     return hd == 256 ? sq_launch<256>(maps, a, units, what, strm(st)) : sq_launch<128>(maps, a, units, what, strm(st));
 }
 
