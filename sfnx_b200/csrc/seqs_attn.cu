@@ -469,6 +469,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(SA_THREADS, 1) k_att
     auto leave = [&]() {
         sa_before();
         asm volatile("bar.sync 0, %0;" ::"n"(SA_THREADS) : "memory");
+        // the last MMAs' arrival in the second CTA.  Here, where the softmax warps have met the last o_full: from the role's beginning on the
+        // bounded wait would have had to last as long as the whole run of work, which may be seconds
+        if (rank && warp == 1) sa_wait_warp(idle, 0u, spins, a.fault);
         sa_cluster();   // the pair's MMAs read both CTAs' memories
         if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tm), "r"(512));
     };
@@ -687,8 +690,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(SA_THREADS, 1) k_att
             sa_wait(idle, 0u, spins, a.fault);
         }
         __syncwarp();
-    } else if (warp == 1) {
-        sa_wait_warp(idle, 0u, spins, a.fault);   // the last MMAs' arrivals here
     }
     leave();
     } else {
