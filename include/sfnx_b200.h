@@ -297,7 +297,8 @@ typedef struct FnxSeqs {
     const int* pos0; /* device [nseq]: the position of its first row = the positions the cache held before */
     const int* pt;   /* device [nseq][pt_stride]: its page table (FnxKvPages.pt is not used); null: the cache is contiguous */
     int pt_stride, npages; /* entries a table has; pages the pool has */
-    const int* kv0;  /* pt null: device [nseq], the cache row of its position 0 (null: 0), the cache of FnxKvPages.cap rows */
+    const int* kv0;  /* pt null: device [nseq], the cache row of its position 0 (null: 0; not negative), the cache of FnxKvPages.cap rows;
+                      * positions past the cache's (or a table's) end are not appended and not seen */
     int max_pos;     /* no sequence ends past this position after the call (0: unknown); a short call starts fewer blocks for
                       * it, what is computed does not depend on it */
 } FnxSeqs;

@@ -166,7 +166,8 @@ __device__ __forceinline__ long long sq_work(const SqAttn& a, int len, int pos0)
 }
 __device__ __forceinline__ void sq_fill(const SqAttn& a, SqUnit& u) {
     u.end = u.pos0 + (a.anc ? u.len : min(u.tok0 + 2 * a.tok, u.len));
-    u.kv_len = (int) min((long long) u.end, a.sq.pt ? (long long) a.sq.pt_stride * a.g.rows : (long long) a.g.cap);
+    const long long room = a.sq.pt ? (long long) a.sq.pt_stride * a.g.rows : (long long) a.g.cap - (a.sq.kv0 ? a.sq.kv0[u.s] : 0);
+    u.kv_len = (int) max(0ll, min((long long) u.end, room));
 }
 __device__ __forceinline__ long long sq_shfl(long long v, int lane) { return __shfl_sync(0xffffffffu, v, lane); }
 // how the work is dealt: all of it, and the pairs that get any

@@ -1,4 +1,5 @@
 """The attention over sequences at the ends of what it takes: units smaller than a box, runs of seconds."""
+import numpy as np
 import pytest
 import torch
 
@@ -49,3 +50,27 @@ def test_a_run_of_work_longer_than_any_wait():
     share = out.view(nq, hd).double() / v.double()
     assert (share >= 0.5 * (1 - 2.0 ** -10)).all() and (share <= 1).all()
     assert a.elapsed_time(b) > 1074, "%.0f ms: no longer than a wait may last (2^16 polls of 16.4 us)" % a.elapsed_time(b)
+
+
+@pytest.mark.parametrize("tree", [False, True])
+def test_positions_past_a_contiguous_cache_are_not_seen(tree):
+    """A cache that ends inside a sequence which does not begin at its row 0, and before the last one: what append leaves out, attention
+    does not see - not as rows of zeros either."""
+    lens, ctx, short = [3, 40, 2], [50, 200, 10], 33
+    s = S.Seqs(lens, ctx, 8, 2, 128, page=0, seed=23, extra_rows=2)
+    s.cap = s.kv0_host[1] + ctx[1] + lens[1] - short
+    s.kc[s.cap:], s.vc[s.cap:] = float("nan"), float("nan")
+    bits = s.tree()[1] if tree else None
+    out = s.attend(None if bits is None else torch.from_numpy(bits.view(np.int32)).to(DEV), gate=False)
+    for i in range(3):
+        r, m, x = slice(s.row0[i], s.row0[i] + lens[i]), lens[i], ctx[i]
+        have = max(0, min(m + x, s.cap - s.kv0_host[i]))
+        seen = torch.ones(m, m + x, dtype=torch.bool, device=DEV)
+        if tree:
+            seen[:, x:] = torch.tensor([[bool(bits[r][t, j // 32] >> np.uint32(j % 32) & 1) for j in range(m)] for t in range(m)], device=DEV)
+        else:
+            seen[:, x:] = torch.ones(m, m, dtype=torch.bool, device=DEV).tril()
+        at = s.kv0_host[i] + torch.arange(have, device=DEV)
+        ref, tol = S.formula(s.q[r, :1024].view(m, 8, 128).double(), s.k[at].double(), s.v[at].double(), seen[:, :have]) if have else (0.0, 0.0)
+        assert ((out[r].view(m, 8, 128).double() - ref).abs() <= tol).all(), "sequence %d" % i
+    assert (out[s.rows:] == -7).all()
