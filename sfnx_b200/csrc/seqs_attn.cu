@@ -1035,7 +1035,8 @@ static int attn_seqs(const uint16_t* q16, int q_stride, const float* qg, const u
     FNX_REQUIRE(encode(&maps.q, 3, q16, qd, qs, qb) && encode(&maps.k, 4, kc, kd, ks, kb) && encode(&maps.v, 4, vc, kd, ks, vb),
                 "%s: no tensor map for %d rows %d apart or %d pages of %zu halves", what, sq->rows, q_stride, sq->npages, g.page);
     // no more pairs than there can be work for
-    const long long units = sq_units(sq, tok, nkv), most = sq->max_pos ? units * (sq->max_pos + SA_COST) : 1ll << 60;
+    const long long units = sq_units(sq, tok, nkv);   // (2^20 of them are more than enough)
+    const long long most = sq->max_pos ? std::min(units, 1ll << 20) * ((long long) sq->max_pos + SA_COST) : 1ll << 60;
     const int pairs = (int) std::max(1ll, std::min((long long) std::min(sq_processors() / 2, SJ_PAIRS), (most + SA_LEAST - 1) / SA_LEAST));
     float4* part = (float4*) scratch;
     float2* mz = reinterpret_cast<float2*>(part + (size_t) 4 * pairs * SA_ROWS * (hd / 4));

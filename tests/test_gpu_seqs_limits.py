@@ -74,3 +74,9 @@ def test_positions_past_a_contiguous_cache_are_not_seen(tree):
         ref, tol = S.formula(s.q[r, :1024].view(m, 8, 128).double(), s.k[at].double(), s.v[at].double(), seen[:, :have]) if have else (0.0, 0.0)
         assert ((out[r].view(m, 8, 128).double() - ref).abs() <= tol).all(), "sequence %d" % i
     assert (out[s.rows:] == -7).all()
+
+
+def test_the_largest_hint_is_as_good_as_none():
+    """max_pos at its largest splits the work as an unknown one does (how it is split shows in the last bits)."""
+    a, b = (S.Seqs([1, 3], [9000, 2500], 8, 2, 128, seed=29, max_pos=hint) for hint in (0, 2 ** 31 - 1))
+    assert torch.equal(a.attend().view(torch.int16), b.attend().view(torch.int16))
