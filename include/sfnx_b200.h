@@ -315,7 +315,9 @@ int fnx_attn_seqs_append(const float* qg, const float* k, const float* v, const 
  * path.  A parent out of range sets bit 64 of *err and is taken as -1; rows past 32 anc_words (at most 32 words) too */
 int fnx_tree_masks(const int* parent, const FnxSeqs* sq, unsigned* anc, int anc_words, int* depth, unsigned* err, void* st);
 /* attention of the rows over the cache, their own K/V rows appended before: out[t][h] = sum_p softmax(q_t . k_p / sqrt(hd)) v_p,
- * f16 in and out, sums and statistics in 32 bits, the softmax weights rounded to f16 for their product with V.
+ * f16 in and out, sums and statistics in 32 bits, the softmax weights rounded to f16 for their product with V (by 2^-11 of a weight, or
+ * by 2^-32 of the row's largest where that is more).  The product's sums are the tensor core's, which cuts what lies 25 places below a
+ * running sum: values of one sign lose up to 2^-27 of their magnitude for every position that one pair of CTAs takes of a row.
  *   fnx_attn_prompt: row t sees positions 0 .. its own (prompts, chunks of prompts after what the cache holds, single tokens);
  *   fnx_attn_tree:   row t sees the positions before pos0[s] and, of its sequence's rows, those whose bit is set in anc[t].
  * qg not null: the result times sigmoid(gate), gate the second half of each head of qg [rows][nq][2 hd], as fnx_attn_finish.

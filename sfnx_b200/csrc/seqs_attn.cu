@@ -22,11 +22,16 @@
 //   and first scores run while the softmax warps write this one's rows.
 //   shared memory: Q, a ring of slots of half a tile each, asked for in the order of their use: K(0), K(1), K(2), V(0), K(3),
 //   V(1), ..., and a strip a softmax warp to turn rows into whole lines on their way out.
-// Softmax: x = s log2 e / sqrt(hd); weights 2^(x - ref) against a reference that is raised - and O and the sums rescaled - only when
-// a row's maximum has grown by more than 8 over it, so weights stay below 2^8 and (O, ref, z) is an exact partial for any
-// reference.  z sums the weights in 32 bits before they are rounded to f16 for the product (2^-11 of a weight: the
-// result's own rounding is as large; f16 queries, keys and values enter exactly).  A tile's 128 x 128 exponentials are 1024 cycles of
-// the special-function units; part of them is taken by a polynomial on the FMA units instead.
+// Softmax: x = s log2 e / sqrt(hd); weights 2^(x - ref + 7) against a reference that is raised - and O and the sums rescaled - only when
+// a row's maximum has grown by more than 8 over it, so weights stay below 2^15, what f16 holds, and (O, ref, z) is an exact partial
+// for any reference (the 7 is a factor of O and z alike).  z sums the weights in 32 bits before they are rounded to f16 for the
+// product: by 2^-11 of a weight (f16 queries, keys and values enter exactly) or, of a weight below 2^-21 of the reference's, by 2^-32
+// of that one's.  Many such weights can be the whole result, where the position that has the rest holds zeros: without the 7, 3000 of
+// 2^-25.5 of the largest were lost, now they are off by 1 %.  A tile's 128 x 128 exponentials are 1024 cycles of the special-function
+// units; part of them is taken by a polynomial on the FMA units instead.
+// O is summed by the tensor core: in 32 bits, a product cut off 25 places below the sum that it goes to, which for values of one
+// sign costs a part of n positions about 2^-27 n of their weighted magnitude (measured: 4.2e-4 at 65 536 positions of one pair, 8.4e-4
+// at 131 072; values of either sign 3.5e-6).
 // Positions past a unit's last visible one are not loaded beyond their box; V rows there are cleared in shared memory, since a
 // weight of zero times a stray NaN is a NaN.
 // Every wait on an mbarrier is bounded; on a timeout the fault word is set and the CTA ends with nothing in flight.
@@ -44,6 +49,7 @@ constexpr int SA_ROWS = 128, SA_KT = 128, SA_THREADS = 384, SA_SOFT = 256, SA_ST
 // Of a thread's 32 pairs of exponentials a tile, those by polynomial: 1000 rows after 31 000 positions 600 us with 0, 593 with 8, 606
 // with 12
 constexpr int SA_POLY = 8;
+constexpr int SA_LIFT = 7;   // weights are held 2^7 times as large, so that their smallest are not lost in f16
 // What a unit's beginning and end cost, in positions (the dealing of the work): a prompt of 8192 tokens, whose first units are short,
 // 692 us with 640, 647 with 768, 647 with 896; eight packed short prompts 33.0, 32.8, 33.4
 constexpr int SA_COST = 768;
@@ -362,7 +368,7 @@ __device__ __forceinline__ float sa_max(float a, float b) {
 // 2^x of two values on the FMA units: x = n + f, n the nearest integer (by adding and taking away 1.5 2^23, whose low bits then hold
 // n), a polynomial of degree 5 for 2^f on [-1/2, 1/2] (fitted to the relative error: 2.4e-7 with its roundings in 32 bits),
 // n added to the exponent.  Below -126 (and of a NaN, which the row's maximum shows): 2^-126 or so instead of zero, which f16 rounds to
-// zero and no sum notices
+// zero and no sum notices (the lifted weights are 2^7 where the reference is)
 __device__ __forceinline__ float2 sa_ex2_poly(float2 x) {
     const float magic = 12582912.f;
     x.x = fmaxf(x.x, -126.f), x.y = fmaxf(x.y, -126.f);
@@ -794,7 +800,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(SA_THREADS, 1) k_att
                         }
                     }
                 }
-                const float less = ref == -INFINITY ? 0.f : -ref;
+                const float less = ref == -INFINITY ? 0.f : (float) SA_LIFT - ref;
                 const bool p_free = j < 2 || sa_test(&o_full[j & 1], (unsigned) ((j >> 1) - 1) & 1u);   // the P tile's last reader is done
                 unsigned pk[32];
                 float2 sum = make_float2(0.f, 0.f);

@@ -80,3 +80,33 @@ def test_the_largest_hint_is_as_good_as_none():
     """max_pos at its largest splits the work as an unknown one does (how it is split shows in the last bits)."""
     a, b = (S.Seqs([1, 3], [9000, 2500], 8, 2, 128, seed=29, max_pos=hint) for hint in (0, 2 ** 31 - 1))
     assert torch.equal(a.attend().view(torch.int16), b.attend().view(torch.int16))
+
+
+@pytest.mark.parametrize("spread", [0.0, 1.0])
+@pytest.mark.parametrize("lens,ctx", [([1] * 80, 3000), ([1, 100], 1500)])
+def test_a_tail_behind_a_position_that_takes_nearly_all_weight(lens, ctx, spread):
+    """The first position has nearly all the weight and a value of zero, so the result is the others' sum: weights of 2^-25.5, or
+    scattered about e^-17.  A weight is held as f16 of 2^7 times itself against the reference, which is the row's largest or less: off by
+    2^-11 of itself or by 2^-32 of the largest weight; the sums, the scores' products (one product here, rounded once) and e^x add
+    2^-18 of the magnitudes, as in the tests' formula; the result is rounded to f16."""
+    s = S.Seqs(lens, [ctx] * len(lens), 8, 2, 128, seed=37, stale=0.0)
+    g = torch.Generator(device=DEV).manual_seed(37)
+    s.q.zero_()
+    s.q[:, ::128] = 8.0   # the score is the key's first element / sqrt(2)
+    s.k.zero_()
+    s.k[:, :, 0] = (torch.randn(s.k.shape[:2], device=DEV, generator=g) * spread * 2 ** 0.5 + (25 - 17 * 2 ** 0.5) * (spread > 0)).half()
+    s.v[:] = 1000.0 + 100 * torch.randn(s.v.shape, device=DEV, generator=g)
+    for c in s.cells:
+        s.k[c[0], :, 0], s.v[c[0]] = 25.0, 0.0
+    s.kc, s.vc = s._pool(s.k), s._pool(s.v)
+    out = s.attend(gate=False).view(-1, 8, 128)
+    for i, n in enumerate(lens):
+        r, c = slice(s.row0[i], s.row0[i] + n), s.cells[i].to(DEV)
+        q, k, v = s.q[r].view(n, 8, 128).double(), s.k[c].double(), s.v[c].double()
+        seen = torch.ones(n, ctx + n, dtype=torch.bool, device=DEV).tril(ctx)
+        x = torch.einsum("thd,phd->htp", q, k.repeat_interleave(4, 1)) / 128 ** 0.5
+        e = torch.exp(x - x.masked_fill(~seen, -torch.inf).amax(-1, keepdim=True)) * seen
+        z, vv = e.sum(-1, keepdim=True), v.repeat_interleave(4, 1)
+        ref, mag, all_v = (torch.einsum("htp,phd->thd", w, u) for w, u in ((e / z, vv), (e / z, vv.abs()), (seen / z, vv.abs())))
+        tol = 2.0 ** -11 * ref.abs() + (2.0 ** -11 + 2.0 ** -18) * mag + 2.0 ** -32 * all_v + 2.0 ** -25
+        assert ((out[r].double() - ref).abs() <= tol * (1 + 2.0 ** -10)).all(), "sequence %d: %.3g of the result" % (i, float(((out[r].double() - ref).abs() / ref).max()))
