@@ -288,7 +288,7 @@ int fnx_attn_finish(const float* parts, int nparts, int first_part, const float*
  * one after another; how many rows each has and where it stands is read on the device, so a captured call serves later windows
  * of other lengths (the host's `rows` is the most there can be).  Rows behind the last sequence's are not read and their
  * outputs are left as they were.  The K/V rows are f16 and whole on this GPU (a position split over GPUs, and int8 rows, are
- * refused).  Every pointer 16-byte aligned; hd 128 or 256; at most 16 query heads a KV head.
+ * refused).  Every pointer 16-byte aligned; hd 128 or 256; at most 16 query heads a KV head, nq hd <= 2^23.
  * Bits of *err that these calls set: 32: a position without a page (the pool is used up, a table is full, or its entry names
  * no page of the pool); 64: a value in device memory that makes no sense (a parent, a kept row, a source). */
 typedef struct FnxSeqs {
@@ -321,7 +321,7 @@ int fnx_tree_masks(const int* parent, const FnxSeqs* sq, unsigned* anc, int anc_
  *   fnx_attn_prompt: row t sees positions 0 .. its own (prompts, chunks of prompts after what the cache holds, single tokens);
  *   fnx_attn_tree:   row t sees the positions before pos0[s] and, of its sequence's rows, those whose bit is set in anc[t].
  * qg not null: the result times sigmoid(gate), gate the second half of each head of qg [rows][nq][2 hd], as fnx_attn_finish.
- * q_stride, out_stride: halves from a row to the next (multiples of 8, at least nq hd).  A row that sees nothing gives
+ * q_stride, out_stride: halves from a row to the next (multiples of 8, at least nq hd; out_stride at most 2^24).  A row that sees nothing gives
  * zeros; a row that sees a score of NaN or +inf gives NaNs.  K rows that a row does not see may hold anything; V rows are finite up to
  * a sequence's newest one (a weight of zero times a NaN is a NaN), behind it and between the sequences they may hold anything.
  * Table entries that name no page of the pool count as rows of zeros.  out overlaps none of the inputs.  scratch:

@@ -52,6 +52,7 @@ inline int sq_check(const FnxSeqs* sq, const FnxKvPages& g, int nq, int nkv, int
     FNX_REQUIRE(sq->nseq >= 1 && sq->rows >= 1, "%s: %d rows of %d sequences", what, sq->rows, sq->nseq);
     FNX_REQUIRE(hd == 128 || hd == 256, "%s: head dim %d (128 or 256)", what, hd);
     FNX_REQUIRE(nkv >= 1 && nq >= 1 && nq % nkv == 0 && nq / nkv <= 16, "%s: %d query heads over %d KV heads", what, nq, nkv);
+    FNX_REQUIRE((long long) nq * hd <= 1 << 23, "%s: rows of %d heads of %d (2^23 values at most)", what, nq, hd);
     FNX_REQUIRE(!g.q8, "%s: int8 rows are not taken (f16 only)", what);
     FNX_REQUIRE(sq->max_pos >= 0, "%s: max_pos %d", what, sq->max_pos);
     if (sq->pt) {

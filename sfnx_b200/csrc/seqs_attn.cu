@@ -1018,6 +1018,8 @@ static int attn_seqs(const uint16_t* q16, int q_stride, const float* qg, const u
                 "%s: a buffer that is not 16-byte aligned", what);
     FNX_REQUIRE(q_stride >= nq * hd && q_stride % 8 == 0 && out_stride >= nq * hd && out_stride % 8 == 0,
                 "%s: rows of %d halves %d and %d apart (multiples of 8)", what, nq * hd, q_stride, out_stride);
+    // (a CTA's up to 128 rows have 32-bit offsets from its first)
+    FNX_REQUIRE(out_stride <= 1 << 24, "%s: output rows %d halves apart (2^24 at most)", what, out_stride);
     FNX_REQUIRE(!sq->pt || g.rows % 8 == 0, "%s: pages of %d rows (a multiple of 8)", what, g.rows);
     const int qpk = nq / nkv, tok = SA_ROWS / qpk;
     int box = 64, lg = 6;

@@ -110,3 +110,14 @@ def test_a_tail_behind_a_position_that_takes_nearly_all_weight(lens, ctx, spread
         ref, mag, all_v = (torch.einsum("htp,phd->thd", w, u) for w, u in ((e / z, vv), (e / z, vv.abs()), (seen / z, vv.abs())))
         tol = 2.0 ** -11 * ref.abs() + (2.0 ** -11 + 2.0 ** -18) * mag + 2.0 ** -32 * all_v + 2.0 ** -25
         assert ((out[r].double() - ref).abs() <= tol * (1 + 2.0 ** -10)).all(), "sequence %d: %.3g of the result" % (i, float(((out[r].double() - ref).abs() / ref).max()))
+
+
+def test_outputs_as_far_apart_as_they_may_be():
+    """Rows 2^24 halves apart, 128 of them a CTA: the last one's offset from the first is just below 2^31 halves."""
+    s = S.Seqs([129], [3], 1, 1, 128, seed=41)
+    base = torch.full((129 * (1 << 24),), -7.0, dtype=torch.float16, device=DEV)
+    out = base.view(129, 1 << 24)
+    s.attend(out=out)
+    want = s.attend()
+    assert torch.equal(out[:, :128].reshape(129, 128).view(torch.int16), want.view(torch.int16))
+    assert (out[:, 128:1024] == -7).all() and (out[:, -64:] == -7).all()
