@@ -1,10 +1,10 @@
 // Log probabilities of given tokens, the entropy of their distribution and the likeliest alternatives, in one pass over the
 // logits (no counterpart in the reference, which returns tokens only).
 //
-// With t = x log2 e - R for a reference R, z = sum 2^t and s = sum t 2^t:  lse = (R + log2 z) ln 2,  H = (log2 z - s / z) ln 2, and a
-// token's log probability is x - lse (R is a 32-bit number and nothing is rounded between it and the sums, so R ln 2 is taken
-// in double).  The reference is raised - z' = f z, s' = f (s + (R - R') z), f = 2^(R - R') - only when a value exceeds it by more
-// than 8, so a thread rescales once or twice a row and 2^t stays below 2^8.  The centred s keeps H free of the cancellation
+// With t = (x - R) log2 e for a reference R, z = sum 2^t and s = sum t 2^t:  lse = R + ln z,  H = (log2 z - s / z) ln 2, and a
+// token's log probability is x - lse.  R is one of the logits, so it is exact and finite where they are, and x - R is rounded once
+// (R log2 e would leave the type from 2.4e38 on).  The reference is raised - z' = f z, s' = f (s + d z), d = (R - R') log2 e, f = 2^d -
+// only when a value exceeds it by more than 5.5, so a thread rescales once or twice a row and 2^t stays below 2^8.  The centred s keeps H free of the cancellation
 // that sum p x - lse has for large logits.  A NaN or +inf makes z a NaN, which is how the row is found out.
 // The k best: a bound that k values of the row's first batch reach or exceed (the k-th largest of the maxima of groups of
 // threads), made anew from the lists some batches on, and of the rest of the row every warp lists what exceeds it, a few hundredths of a
@@ -53,6 +53,7 @@ __device__ __forceinline__ unsigned long long lp_composite(float v, unsigned idx
     return ((unsigned long long) fkey(fadd(v, 0.f)) << 32) | (0xffffffffu - idx);
 }
 
+constexpr float LP_L2E = 1.44269504f;
 // (r, z, s) of two parts of a row together
 __device__ __forceinline__ void lp_join(float& r, float& z, float& s, float r2, float z2, float s2) {
     const float rn = fmaxf(r, r2);
@@ -60,7 +61,7 @@ __device__ __forceinline__ void lp_join(float& r, float& z, float& s, float r2, 
         z += z2, s += s2;
         return;
     }
-    const float d1 = fmaxf(r - rn, -200.f), d2 = fmaxf(r2 - rn, -200.f);   // 2^-200 is zero: a part of nothing (-inf) drops out
+    const float d1 = fmaxf((r - rn) * LP_L2E, -200.f), d2 = fmaxf((r2 - rn) * LP_L2E, -200.f);   // 2^-200 is zero: a part of nothing (-inf) drops out
     const float f1 = ex2_ftz(d1), f2 = ex2_ftz(d2);
     s = f1 * (s + d1 * z) + f2 * (s2 + d2 * z2);
     z = f1 * z + f2 * z2;
@@ -70,7 +71,7 @@ __device__ __forceinline__ void lp_join(float& r, float& z, float& s, float r2, 
 // the same of a warp's 32 parts: one reference for all, then plain sums
 __device__ __forceinline__ void lp_join_warp(float& r, float& z, float& s) {
     const float top = fkey_inv(__reduce_max_sync(0xffffffffu, fkey(r)));
-    const float d = r == top ? 0.f : fmaxf(r - top, -200.f), f = ex2_ftz(d);
+    const float d = r == top ? 0.f : fmaxf((r - top) * LP_L2E, -200.f), f = ex2_ftz(d);
     s = f * (s + d * z), z *= f, r = top;
 #pragma unroll
     for (int o = 16; o; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o), s += __shfl_xor_sync(0xffffffffu, s, o);
@@ -214,7 +215,6 @@ __global__ void __launch_bounds__(LP_THREADS, 2) k_logprobs(const LpArgs a) {
     auto index = [&](int i0, int j) { return i0 + (j >> 2) * (LP_BATCH / 2) + tid * 4 + (j & 3); };
     pdl_wait();
     pdl_go();
-    const float L2E = 1.44269504f;
     const bool parts_of_rows = a.nsplit > 1;   // a block a part; else a block every gridDim.x-th row
     const unsigned step = parts_of_rows ? (unsigned) a.rows : gridDim.x;
     LpItem next = lp_item(a, parts_of_rows ? blockIdx.y : blockIdx.x, parts_of_rows ? blockIdx.x : 0);
@@ -223,7 +223,7 @@ __global__ void __launch_bounds__(LP_THREADS, 2) k_logprobs(const LpArgs a) {
     for (int i = 0; i < LP_STAGES - 1; ++i) load(next, next.lo + i * LP_BATCH, slot(i));
     for (unsigned row = (unsigned) next.row; row < (unsigned) a.rows; row += step) {
         const LpItem t = next;
-        float r = -INFINITY, bound_v = -INFINITY;                        // r: the reference, in units of log2
+        float r = -INFINITY, bound_v = -INFINITY;                        // r: the reference
         float2 z2 = make_float2(0.f, 0.f), s2 = make_float2(0.f, 0.f);   // the sums of the even and the odd values
         unsigned long long bound = 0ull;                                 // an entry has to be above it
         int cnt = 0;                                                     // this warp's list
@@ -237,17 +237,16 @@ __global__ void __launch_bounds__(LP_THREADS, 2) k_logprobs(const LpArgs a) {
             float mx = v[0];
 #pragma unroll
             for (int j = 1; j < LP_PER; ++j) mx = fmaxf(mx, v[j]);
-            const float top = mx * L2E;
-            if (top > r + 8.f || (r == -INFINITY && mx > -INFINITY)) {
-                const float d = fmaxf(r - top, -200.f), f = ex2_ftz(d);
+            if (mx > r + 5.5f || (r == -INFINITY && mx > -INFINITY)) {
+                const float d = fmaxf((r - mx) * LP_L2E, -200.f), f = ex2_ftz(d);
                 s2.x = f * (s2.x + d * z2.x), s2.y = f * (s2.y + d * z2.y);
                 z2.x *= f, z2.y *= f;
-                r = top;
+                r = mx;
             }
             const float less = r == -INFINITY ? 0.f : -r;
 #pragma unroll
             for (int j = 0; j < LP_PER; j += 2) {
-                float2 q = fma2(make_float2(v[j], v[j + 1]), make_float2(L2E, L2E), make_float2(less, less));
+                float2 q = mul2(add2(make_float2(v[j], v[j + 1]), make_float2(less, less)), make_float2(LP_L2E, LP_L2E));
                 const float2 e = make_float2(ex2_ftz(q.x), ex2_ftz(q.y));
                 q.x = fmaxf(q.x, -200.f), q.y = fmaxf(q.y, -200.f);
                 z2 = add2(z2, e);
@@ -369,7 +368,7 @@ __global__ void __launch_bounds__(LP_THREADS, 2) k_logprobs(const LpArgs a) {
                 const bool bad = z != z, none = r == -INFINITY && !bad;
                 if (bad || none) atomicOr(a.err, 16u);
                 const double ln2 = 0.6931471805599453, lz = log2((double) z);
-                sh.lse = bad ? NAN : none ? -INFINITY : (float) (((double) r + lz) * ln2);
+                sh.lse = bad ? NAN : none ? -INFINITY : (float) ((double) r + lz * ln2);
                 a.lse[t.row] = sh.lse;
                 if (a.ent) a.ent[t.row] = bad ? NAN : none ? 0.f : fmaxf((float) ((lz - (double) s / z) * ln2), 0.f);
             }
