@@ -476,7 +476,7 @@ int fnx_top_tokens(float* logits, int n, int T, int v0, const int* pen_tok, cons
                    const float* pen_par, float* out_v, int* out_i, unsigned* err, void* st);
 
 /* log probabilities over a slice of n logits a row (rows `stride` floats apart; tokens v0 .. v0 + n - 1), no counterpart in the
- * reference: lse[t] = log sum e^x, entropy[t] = -sum p log p, lp[t][j] = x[tok[t][j]] - lse for the ntok given tokens (a token
+ * reference: lse[t] = log sum e^x, entropy[t] = -sum p log p, lp[t][j] = x[tok[t][j]] - lse, never above 0, for the ntok given tokens (a token
  * outside the slice: -inf), and the k <= FNX_TOPK_N likeliest tokens, best first, the lower id on a tie: top_lp, top_i
  * [T][k].  entropy, lp with tok, and top_* with k = 0 may be null.  Logits may have any finite size; -inf logits are tokens that cannot come; a NaN or +inf, or
  * a row of nothing but -inf, sets bit 16 of *err (the row's results are then NaN and top_i -1, or lse -inf and entropy 0).  n >= k.

@@ -119,7 +119,8 @@ struct LpShared {
     int cnt[LP_WARPS];
     unsigned long long bound;
     unsigned n, last;
-    float lse;
+    float ref;
+    double lz;   // lse = ref + lz; a NaN, or ref -inf: the row has no distribution
 };
 
 // A bound that at least k of the threads' entries reach (0 where there are too few): the k-th largest of the maxima of groups of
@@ -368,24 +369,25 @@ __global__ void __launch_bounds__(LP_THREADS, 2) k_logprobs(const LpArgs a) {
                 const bool bad = z != z, none = r == -INFINITY && !bad;
                 if (bad || none) atomicOr(a.err, 16u);
                 const double ln2 = 0.6931471805599453, lz = log2((double) z);
-                sh.lse = bad ? NAN : none ? -INFINITY : (float) ((double) r + lz * ln2);
-                a.lse[t.row] = sh.lse;
+                sh.ref = r, sh.lz = bad ? NAN : lz * ln2;
+                a.lse[t.row] = bad ? NAN : none ? -INFINITY : (float) ((double) r + lz * ln2);
                 if (a.ent) a.ent[t.row] = bad ? NAN : none ? 0.f : fmaxf((float) ((lz - (double) s / z) * ln2), 0.f);
             }
             __syncthreads();
-            const float lse = sh.lse;
-            const bool bad = lse != lse, none = lse == -INFINITY;
+            const double ref = sh.ref, lz = sh.lz;
+            const bool bad = lz != lz, none = ref == -INFINITY;
+            auto log_p = [&](float x) { return none ? -INFINITY : (float) fmin((double) x - ref - lz, 0.0); };   // rounded once
             for (int j = tid; j < a.ntok; j += LP_THREADS) {
                 const long long i = (long long) a.tok[(size_t) t.row * a.ntok + j] - a.v0;
                 const bool in = i >= 0 && i < a.n;
-                a.lp[(size_t) t.row * a.ntok + j] = !in ? -INFINITY : bad ? NAN : none ? -INFINITY : t.base[t.shift + i] - lse;
+                a.lp[(size_t) t.row * a.ntok + j] = !in ? -INFINITY : bad ? NAN : log_p(t.base[t.shift + i]);
             }
             if (a.k && bad) {   // no order to speak of
                 for (int j = tid; j < a.k; j += LP_THREADS) a.top_i[(size_t) t.row * a.k + j] = -1, a.top_lp[(size_t) t.row * a.k + j] = NAN;
             } else if (a.k) {
                 lp_best(sh, e, a.k, [&](int place, unsigned long long c) {
                     a.top_i[(size_t) t.row * a.k + place] = a.v0 + (int) (0xffffffffu - (unsigned) (c & 0xffffffffu));
-                    a.top_lp[(size_t) t.row * a.k + place] = none ? -INFINITY : fkey_inv((unsigned) (c >> 32)) - lse;
+                    a.top_lp[(size_t) t.row * a.k + place] = log_p(fkey_inv((unsigned) (c >> 32)));
                 });
             }
         }

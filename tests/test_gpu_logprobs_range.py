@@ -1,4 +1,4 @@
-"""Log probabilities of logits of any finite size."""
+"""Log probabilities of logits of any finite size, and of tokens that are all but certain."""
 import pytest
 import torch
 
@@ -11,7 +11,8 @@ LOWEST, MOST = torch.finfo(torch.float32).min, torch.finfo(torch.float32).max
 def _check(r, x, tok, k):
     """Against 64 bits, everything taken from the row's largest logit m.  The sum z of e^(x - m) is off by `rel` of itself (a thread adds at
     most n / 384 terms in 32 bits, in two sums, then trees: 2^-24 (n / 512 + 64) covers them; an exponential of what weighs anything
-    2^-18), so its logarithm by as much.  lse is rounded once; the entropy's terms have weights |x - m| <= 100."""
+    2^-18), so its logarithm by as much.  A log probability (x - m) - log z is made in 64 bits and rounded once; lse too; the entropy's
+    terms have weights |x - m| <= 100."""
     n, d = x.shape[1], x.double()
     m = d.amax(1, keepdim=True)
     lz = torch.log(torch.exp(d - m).sum(1, keepdim=True))
@@ -22,8 +23,18 @@ def _check(r, x, tok, k):
     lse = m + lz
     assert ((r["lse"].double() - lse[:, 0]).abs() <= rel + 2.0 ** -24 * lse[:, 0].abs()).all()
     assert ((r["ent"].double() - ent).abs() <= rel * (2 + ent)).all()
+
+    def lp(got, at):
+        want = d.gather(1, at.long()) - m - lz
+        big = want < LOWEST   # (a difference of two logits may be past the type: -inf)
+        assert torch.isinf(got[big]).all() and (got <= 0).all()
+        assert ((got.double() - want).abs() <= rel + 2.0 ** -24 * want.abs())[~big].all()
+
+    if tok is not None:
+        lp(r["lp"], tok)
     order = torch.sort(x + 0.0, dim=1, descending=True, stable=True).indices[:, :k]
     assert torch.equal(r["ti"].long(), order)
+    lp(r["tv"], order)
 
 
 KINDS = ["one past 2^127", "all the lowest", "the lowest and normal", "all the largest", "scattered over the type", "near the lowest", "about 5000", "about -3e7"]
@@ -56,3 +67,15 @@ def test_logits_of_any_size(kind, T, n, k):
     tok = torch.randint(0, n, (T, 3), device=DEV, generator=g).to(torch.int32)
     tok[:, 0] = x.argmax(1)
     _check(_run(x, tok, k), x, tok, k)
+
+
+@pytest.mark.parametrize("T,n", [(1500, 300), (4, 40000)])
+def test_a_certain_token_has_no_positive_log_probability(T, n):
+    g = torch.Generator(device=DEV).manual_seed(T)
+    x = torch.randn(T, n, device=DEV, generator=g)
+    at = torch.randint(0, n, (T, 1), device=DEV, generator=g)
+    x.scatter_(1, at, x.gather(1, at) + torch.rand(T, 1, device=DEV, generator=g) * 30 + 8)
+    tok = at.to(torch.int32)
+    r = _run(x, tok, 5)
+    _check(r, x, tok, 5)
+    assert (r["lp"] <= 0).all() and (r["tv"] <= 0).all()
