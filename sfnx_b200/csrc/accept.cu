@@ -164,8 +164,8 @@ int fnx_top_merge(const float* vs, const int* is, int nslice, int T, float* out_
     return 0;
 }
 
-// the slices' softmax statistics joined: with w_i = e^(lse_i - lse), lse = log sum e^lse_i and, an entropy being lse - sum p x,
-// H = lse - sum w_i (lse_i - H_i).  Sums in double.
+// the slices' softmax statistics joined: with lse = log sum e^lse_i and w_i = e^(lse_i - lse), a log probability of slice i changes by
+// log w_i, and H = sum w_i (H_i - log w_i).  Only differences of the lse_i are formed, in double, so their size costs nothing.
 int fnx_logprobs_merge(const float* lse_s, const float* entropy_s, const float* lp_s, const float* top_lp_s, const int* top_i_s, int nslice, int T,
                        int ntok, int k, float* lse, float* entropy, float* lp, float* top_lp, int* top_i) {
     constexpr int MOST = 64;
@@ -176,7 +176,7 @@ int fnx_logprobs_merge(const float* lse_s, const float* entropy_s, const float* 
         return fnxk::fail("logprobs_merge: a null buffer");
     auto raw = [ninf](float l, float z) { return l == ninf ? ninf : l + z; };   // the logit that a log probability was made of
     for (int t = 0; t < T; ++t) {
-        double m = ninf, z = 0.0, mean = 0.0;
+        double m = ninf, z = 0.0, h = 0.0, shift[MOST];   // shift: log w_i
         bool nan = false;
         for (int i = 0; i < nslice; ++i) {
             const double x = lse_s[(size_t) i * T + t];
@@ -184,22 +184,21 @@ int fnx_logprobs_merge(const float* lse_s, const float* entropy_s, const float* 
             if (x > m) m = x;
         }
         const bool none = !(m > ninf);
-        if (!none && !nan)
+        if (!none && !nan) {
+            for (int i = 0; i < nslice; ++i) z += std::exp(lse_s[(size_t) i * T + t] - m);
             for (int i = 0; i < nslice; ++i) {
-                const double x = lse_s[(size_t) i * T + t], w = std::exp(x - m);
-                z += w;
-                if (w > 0.0 && entropy) mean += w * (x - (double) entropy_s[(size_t) i * T + t]);
+                shift[i] = lse_s[(size_t) i * T + t] - m - std::log(z);
+                const double w = std::exp(shift[i]);
+                if (w > 0.0 && entropy) h += w * ((double) entropy_s[(size_t) i * T + t] - shift[i]);
             }
-        const double all = nan ? std::numeric_limits<double>::quiet_NaN() : none ? (double) ninf : m + std::log(z);
-        lse[t] = (float) all;
-        if (entropy) entropy[t] = nan ? lse[t] : none ? 0.f : (float) (all - mean / z);
+        }
+        lse[t] = nan ? std::numeric_limits<float>::quiet_NaN() : none ? ninf : (float) (m + std::log(z));
+        if (entropy) entropy[t] = nan ? lse[t] : none ? 0.f : (float) std::max(h, 0.0);
+        auto whole = [&](float l, int i) { return none || l == ninf ? ninf : (float) std::min(l + shift[i], 0.0); };   // of a slice's log probability
         for (int j = 0; j < ntok; ++j) {
-            double x = ninf;
-            for (int i = 0; i < nslice; ++i) {
-                const size_t at = (size_t) i * T + t;
-                x = std::max(x, (double) raw(lp_s[at * ntok + j], lse_s[at]));
-            }
-            lp[(size_t) t * ntok + j] = nan ? lse[t] : none || x == ninf ? ninf : (float) (x - all);
+            float x = ninf;
+            for (int i = 0; i < nslice && !nan; ++i) x = std::max(x, whole(lp_s[((size_t) i * T + t) * ntok + j], i));
+            lp[(size_t) t * ntok + j] = nan ? lse[t] : x;
         }
         int head[MOST] = {};
         for (int j = 0; j < k; ++j) {   // every slice's list is in order: the best of the heads
@@ -208,17 +207,17 @@ int fnx_logprobs_merge(const float* lse_s, const float* entropy_s, const float* 
                 continue;
             }
             int best = -1, bi = 0;
-            float bx = 0.f;
+            float bx = 0.f, bl = 0.f;
             for (int i = 0; i < nslice; ++i) {
                 if (head[i] >= k) continue;
                 const size_t at = (size_t) i * T + t;
                 const float x = raw(top_lp_s[at * k + head[i]], lse_s[at]);
                 const int id = top_i_s[at * k + head[i]];
-                if (best < 0 || x > bx || (x == bx && id < bi)) best = i, bx = x, bi = id;
+                if (best < 0 || x > bx || (x == bx && id < bi)) best = i, bx = x, bi = id, bl = top_lp_s[at * k + head[i]];
             }
             ++head[best];
             top_i[(size_t) t * k + j] = bi;
-            top_lp[(size_t) t * k + j] = none || bx == ninf ? ninf : (float) (bx - all);
+            top_lp[(size_t) t * k + j] = j ? std::min(whole(bl, best), top_lp[(size_t) t * k + j - 1]) : whole(bl, best);   // (in order, whatever was rounded)
         }
     }
     return 0;
