@@ -508,31 +508,40 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(SA_THREADS, 1) k_att
         auto boxes = [&](int tile, int lo, int rows) { return max(0, (min(rows, r.u.kv_len - tile * SA_KT - lo) + a.box - 1) >> a.lg); };
         // those rows, nb column blocks from block x on, into the next slot; `bytes`: of both CTAs' loads; `dirty`: some rows will be cleared
         auto load = [&](const CUtensorMap* map, int tile, int y, int z, int lo, int rows, int x, int nb, int bytes, bool dirty) {
-            const int slot = c % S::SLOTS;
-            if (c >= S::SLOTS) alive = alive && sa_wait_warp(&empty[slot], (unsigned) (c / S::SLOTS - 1) & 1u, spins, a.fault);
-            if (!alive) return;
-            const int nbox = boxes(tile, lo, rows);
+            const int slot = c % S::SLOTS, nbox = boxes(tile, lo, rows);
             const unsigned dst = um_s32(ring) + slot * S::SLOT, bar = dirty ? um_s32(&full[slot]) : um_s32(&ready[slot]) + first;
+            const int y0 = __shfl_sync(0xffffffffu, y, lo / 64), z0 = __shfl_sync(0xffffffffu, z, lo / 64), y1 = __shfl_sync(0xffffffffu, y, 1),
+                      z1 = __shfl_sync(0xffffffffu, z, 1);   // of whole groups
+            // the slot may be written; what will land there is expected (the other CTA's bytes may be counted before: the phase lasts until
+            // both CTAs are here)
+            auto claim = [&]() {
+                if (c >= S::SLOTS && !sa_wait(&empty[slot], (unsigned) (c / S::SLOTS - 1) & 1u, spins, a.fault)) return false;
+                if (rank == 0) um_expect_tx(&ready[slot], dirty ? 0u : (unsigned) bytes);
+                else sa_tell(&ready[slot], first);   // (so that no slot goes round without this CTA, which may have no box to load)
+                if (dirty) um_expect_tx(&full[slot], (unsigned) (nbox * nb * 128 << a.lg));
+                return true;
+            };
+            if (!alive) return;
             const bool elected = um_elect();
-            if (elected && dirty) um_expect_tx(&full[slot], (unsigned) (nbox * nb * 128 << a.lg));
-            if (dirty) odd ^= 1u << slot;
+            bool ok = true;
             if (a.box == 64) {   // a box is a group, with its column blocks
-                const int y0 = __shfl_sync(0xffffffffu, y, lo / 64), z0 = __shfl_sync(0xffffffffu, z, lo / 64), y1 = __shfl_sync(0xffffffffu, y, 1),
-                          z1 = __shfl_sync(0xffffffffu, z, 1);
-                if (elected && nbox > 0) sa_tma4d(dst, map, 0, y0, x, z0, bar);
-                if (elected && nbox > 1) sa_tma4d(dst + nb * 8192, map, 0, y1, x, z1, bar);
+                if (elected) {
+                    ok = claim();
+                    if (ok && nbox > 0) sa_tma4d(dst, map, 0, y0, x, z0, bar);
+                    if (ok && nbox > 1) sa_tma4d(dst + nb * 8192, map, 0, y1, x, z1, bar);
+                }
             } else {
+                if (elected) ok = claim();
                 for (int j = 0; j < nbox; ++j) {
                     const int at = lo / a.box + j, yj = __shfl_sync(0xffffffffu, y, at), zj = __shfl_sync(0xffffffffu, z, at), row = j * a.box;
-                    if (elected)
+                    if (elected && ok)
                         for (int b = 0; b < nb; ++b) sa_tma4d(dst + (row / 64 * nb + b) * 8192 + row % 64 * 128, map, 0, yj, x + b, zj, bar);
                 }
             }
-            if (elected) {   // behind the copies, whose bytes may be counted first: the phase lasts until both CTAs are here
-                if (rank == 0) um_expect_tx(&ready[slot], dirty ? 0u : (unsigned) bytes);
-                else sa_tell(&ready[slot], first);   // (so that no slot goes round without this CTA, which may have no box to load)
-            }
             __syncwarp();
+            alive = __all_sync(0xffffffffu, ok);
+            if (!alive) return;
+            if (dirty) odd ^= 1u << slot;
             ++c;
         };
         auto load_k = [&](int t, int y, int z) {
