@@ -404,20 +404,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(SA_THREADS, 1) k_att
     unsigned char *Q = sa_smem, *ring = Q + S::QBYTES, *strips = ring + S::SLOTS * S::SLOT;
     float* xmax = reinterpret_cast<float*>(strips + SA_SOFT / 32 * SA_STRIP);   // [2][2][128] the halves' maxima, of odd and even tiles
     unsigned long long* bars = reinterpret_cast<unsigned long long*>(xmax + 4 * SA_ROWS);
-    // ready, q_ready: both CTAs' copies have landed (their bytes, which the first CTA expects).  full: this CTA's copy of V rows of which some
-    // are to be cleared; clean: that is done.  ready, q_ready, clean, s_free, p_full, o_free count both CTAs', in the first one's
-    // memory.  empty, q_empty, s_full, o_full: MMAs are done, told to both
-    unsigned long long *full = bars, *empty = full + S::SLOTS, *ready = empty + S::SLOTS, *clean = ready + S::SLOTS, *q_ready = clean + 1, *q_empty = clean + 2,
-                       *s_full = clean + 3, *s_free = clean + 4, *o_free = clean + 5, *idle = clean + 6, *p_full = clean + 7, *o_full = clean + 9;
-    volatile unsigned *tmem_at = reinterpret_cast<unsigned*>(clean + 11), *work_at = tmem_at + 1;
-    volatile int* run_at = reinterpret_cast<int*>(clean + 12);
+    // ready, q_ready: both CTAs' copies have landed (their bytes, which the first CTA expects; or both have cleared their V rows).  full: this
+    // CTA's copy of V rows of which some are to be cleared.  ready, q_ready, s_free, p_full, o_free count both CTAs', in the first
+    // one's memory.  empty, q_empty, s_full, o_full: MMAs are done, told to both
+    unsigned long long *full = bars, *empty = full + S::SLOTS, *ready = empty + S::SLOTS, *q_ready = ready + S::SLOTS, *q_empty = q_ready + 1, *s_full = q_ready + 2,
+                       *s_free = q_ready + 3, *o_free = q_ready + 4, *idle = q_ready + 5, *p_full = q_ready + 6, *o_full = q_ready + 8;
+    volatile unsigned *tmem_at = reinterpret_cast<unsigned*>(q_ready + 10), *work_at = tmem_at + 1;
+    volatile int* run_at = reinterpret_cast<int*>(q_ready + 11);
     const int tid = threadIdx.x, warp = (int) um_uniform(tid >> 5), lane = tid & 31, rank = blockIdx.x & 1, g = blockIdx.x >> 1;
     unsigned first;
     asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(first) : "r"(um_s32(bars)));
     first -= um_s32(bars);
     if (tid == 0) {
         for (int i = 0; i < S::SLOTS; ++i) sa_init(&full[i], 1), sa_init(&empty[i], 1), sa_init(&ready[i], 2);
-        sa_init(clean, 2), sa_init(q_ready, 1), sa_init(q_empty, 1), sa_init(s_full, 1), sa_init(s_free, 2 * (SA_SOFT / 32 + 1)), sa_init(o_free, 2 * SA_SOFT / 32);
+        sa_init(q_ready, 1), sa_init(q_empty, 1), sa_init(s_full, 1), sa_init(s_free, 2 * (SA_SOFT / 32 + 1)), sa_init(o_free, 2 * SA_SOFT / 32);
         sa_init(idle, 1);
         for (int i = 0; i < 2; ++i) sa_init(&p_full[i], 2 * SA_SOFT / 32), sa_init(&o_full[i], 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -506,9 +506,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(SA_THREADS, 1) k_att
         };
         // boxes of a tile's rows lo .. lo + rows - 1 that have positions
         auto boxes = [&](int tile, int lo, int rows) { return max(0, (min(rows, r.u.kv_len - tile * SA_KT - lo) + a.box - 1) >> a.lg); };
-        // those rows, nb column blocks from block x on, into the next slot; `bytes`: of both CTAs' loads; `dirty`: some rows will be cleared
-        auto load = [&](const CUtensorMap* map, int tile, int y, int z, int lo, int rows, int x, int nb, int bytes, bool dirty) {
-            const int slot = c % S::SLOTS, nbox = boxes(tile, lo, rows);
+        // half a K tile (64 rows) or V tile (half of the dims) into the next slot.  One body for both: what this warp runs again every tile
+        // takes the softmax warps' place in the instruction cache (with a body for each, eight packed prompts took 33.5 us instead of 32.9)
+        auto load = [&](bool v, int tile, int y, int z) {
+            const CUtensorMap* map = v ? &maps.v : &maps.k;
+            const int lo = v ? 0 : rank * (SA_KT / 2), nb = v ? HD / 128 : HD / 64, x = r.u.head * (HD / 64) + (v ? rank * (HD / 128) : 0);
+            const int slot = c % S::SLOTS, nbox = boxes(tile, lo, v ? SA_KT : SA_KT / 2), bytes = boxes(tile, 0, SA_KT) * (HD / 64) * 128 << a.lg;   // of both CTAs
+            const bool dirty = v && sq_unclean(r.u.kv_len, tile);   // some rows will be cleared
             const unsigned dst = um_s32(ring) + slot * S::SLOT, bar = dirty ? um_s32(&full[slot]) : um_s32(&ready[slot]) + first;
             const int y0 = __shfl_sync(0xffffffffu, y, lo / 64), z0 = __shfl_sync(0xffffffffu, z, lo / 64), y1 = __shfl_sync(0xffffffffu, y, 1),
                       z1 = __shfl_sync(0xffffffffu, z, 1);   // of whole groups
@@ -516,9 +520,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(SA_THREADS, 1) k_att
             // both CTAs are here)
             auto claim = [&]() {
                 if (c >= S::SLOTS && !sa_wait(&empty[slot], (unsigned) (c / S::SLOTS - 1) & 1u, spins, a.fault)) return false;
-                if (rank == 0) um_expect_tx(&ready[slot], dirty ? 0u : (unsigned) bytes);
+                if (dirty) um_expect_tx(&full[slot], (unsigned) (nbox * nb * 128 << a.lg));   // (`ready` is told when they are clean)
+                else if (rank == 0) um_expect_tx(&ready[slot], (unsigned) bytes);
                 else sa_tell(&ready[slot], first);   // (so that no slot goes round without this CTA, which may have no box to load)
-                if (dirty) um_expect_tx(&full[slot], (unsigned) (nbox * nb * 128 << a.lg));
                 return true;
             };
             if (!alive) return;
@@ -544,19 +548,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(SA_THREADS, 1) k_att
             if (dirty) odd ^= 1u << slot;
             ++c;
         };
-        auto load_k = [&](int t, int y, int z) {
-            const int both = boxes(t, 0, SA_KT / 2) + boxes(t, SA_KT / 2, SA_KT / 2);
-            load(&maps.k, t, y, z, rank * (SA_KT / 2), SA_KT / 2, r.u.head * (HD / 64), HD / 64, both * (HD / 64) * 128 << a.lg, false);
-        };
-        auto load_v = [&](int t, int y, int z) {
-            const int both = 2 * boxes(t, 0, SA_KT);
-            load(&maps.v, t, y, z, 0, SA_KT, r.u.head * (HD / 64) + rank * (HD / 128), HD / 128, both * (HD / 128) * 128 << a.lg, sq_unclean(r.u.kv_len, t));
-        };
         for (bool more = work; more && alive; more = r.next(a)) {
             if (!r.n) continue;
             kv0 = !a.sq.pt && a.sq.kv0 ? a.sq.kv0[r.u.s] : 0;
             const int end = r.t0 + r.n;
-            int e = entry(r.t0), y0, z0, y1 = 0, z1 = 0, y2 = 0, z2 = 0;
+            int e = entry(r.t0), y0 = 0, z0 = 0, y1 = 0, z1 = 0, y2 = 0, z2 = 0;
             if (nseg) alive = sa_wait_warp(q_empty, (unsigned) (nseg - 1) & 1u, spins, a.fault);   // the scores before are done
             if (!alive) break;
             const int tok0 = r.u.tok0 + rank * a.tok;
@@ -572,21 +568,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(SA_THREADS, 1) k_att
             }
             __syncwarp();
             ++nseg;
-            place(r.t0, e, y0, z0);
-            e = entry(r.t0 + 1);
-            load_k(r.t0, y0, z0);
-            if (r.n > 1) {
-                place(r.t0 + 1, e, y1, z1);
-                e = entry(r.t0 + 2);
-                load_k(r.t0 + 1, y1, z1);
-            }
-            for (int t = r.t0; t < end && alive; ++t) {
-                if (t + 2 < end) {
-                    place(t + 2, e, y2, z2);
-                    e = entry(t + 3);
-                    load_k(t + 2, y2, z2);
+            // K(t), then V(t - 2)
+#pragma unroll 1
+            for (int t = r.t0; t < end + 2; ++t) {
+                if (t < end) {
+                    place(t, e, y2, z2);
+                    e = entry(t + 1);
                 }
-                load_v(t, y0, z0);
+#pragma unroll 1
+                for (int v = t < end ? 0 : 1; v <= (t >= r.t0 + 2) && alive; ++v) load(v != 0, v ? t - 2 : t, v ? y0 : y2, v ? z0 : z2);
                 y0 = y1, z0 = z1, y1 = y2, z1 = z2;
             }
         }
@@ -610,26 +600,31 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(SA_THREADS, 1) k_att
         r.get(run_at);
         for (bool more = work; more; more = r.next(a)) {
             if (!r.n) continue;
-            for (int i = 0; i < r.n; ++i, ++j) {
-                sa_wait_warp(s_full, (unsigned) j & 1u, spins, a.fault);
-                if (lane == 0) sa_tell(s_free, first);
-            }
             c += 2 * r.n;
-            const int t = r.t0 + r.n - 1;
-            if (!sq_unclean(r.u.kv_len, t)) continue;
-            const int slot = (c - 1) % S::SLOTS, have = r.u.kv_len - t * SA_KT;   // the segment's last load
-            sa_wait_warp(&full[slot], odd >> slot & 1u, spins, a.fault);
-            odd ^= 1u << slot;
-            for (int x = have; x % 16; ++x)
-                for (int y = lane; y < HD / 16; y += 32)
-                    *reinterpret_cast<uint4*>(ring + slot * S::SLOT + ((x >> 6) * (HD / 128) + (y >> 3)) * 8192 + (x & 63) * 128 + (y & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) sa_tell_shared(clean, first);
+            const int t = r.t0 + r.n - 1, slot = (c - 1) % S::SLOTS, have = r.u.kv_len - t * SA_KT, dirty = sq_unclean(r.u.kv_len, t);   // the segment's last load
+            // one wait for both (with a second place of it, whether reached or not, a prompt of 8192 took 674 us instead of 645)
+#pragma unroll 1
+            for (int i = 0; i < r.n + dirty; ++i) {
+                const bool tile = i < r.n;
+                sa_wait_warp(tile ? s_full : &full[slot], (tile ? (unsigned) j : odd >> slot) & 1u, spins, a.fault);
+                if (tile) {
+                    if (lane == 0) sa_tell(s_free, first);
+                    ++j;
+                    continue;
+                }
+                odd ^= 1u << slot;
+                const unsigned row = um_s32(ring) + slot * S::SLOT + (have >> 6) * (HD / 128) * 8192 + (have & 63) * 128;   // the first to clear (all lie in one group)
+#pragma unroll 1
+                for (int k = lane; k < (16 - have % 16) * (HD / 16); k += 32)   // a row is HD / 128 blocks of 8 runs
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(row + k / (HD / 16) * 128 + k / 8 % (HD / 128) * 8192 + k % 8 * 16), "r"(0u) : "memory");
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) sa_tell_shared(&ready[slot], first);
+            }
         }
     } else if (warp == 1 && rank == 0) {
         // ---- the pair's MMAs, one lane's work from wait to commit
-        int c = 0, j = 0, nseg = 0, ncl = 0;   // slots used in the order of their loads (the elected lane's); tiles; segments; cleared tiles
+        int c = 0, j = 0, nseg = 0;   // slots used in the order of their loads (the elected lane's); tiles; segments
         bool alive = true;            // the elected lane's
         SqRun r;
         r.get(run_at);
@@ -657,9 +652,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(SA_THREADS, 1) k_att
         };
         auto output = [&](int t) {
             const int slot = c % S::SLOTS, steps = (min(r.u.kv_len - t * SA_KT, SA_KT) + 15) / 16;   // of 16 positions that exist
-            wait(&ready[slot], (unsigned) (c / S::SLOTS) & 1u);
+            alive = alive && sa_wait_shared(&ready[slot], (unsigned) (c / S::SLOTS) & 1u, spins, a.fault);
             ++c;
-            if (sq_unclean(r.u.kv_len, t)) alive = alive && sa_wait_shared(clean, (unsigned) ncl & 1u, spins, a.fault), ++ncl;
             if (!alive) return;
             unsigned long long dv = um_desc_x(um_s32(ring) + slot * S::SLOT, 8192, 1024, 2);
             unsigned dp = tm + S::COL_P + (j & 1) * (SA_KT / 2), more = (unsigned) (t - r.t0);
