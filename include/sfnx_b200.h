@@ -300,7 +300,7 @@ typedef struct FnxSeqs {
     const int* kv0;  /* pt null: device [nseq], the cache row of its position 0 (null: 0; not negative), the cache of FnxKvPages.cap rows;
                       * positions past the cache's (or a table's) end are not appended and not seen */
     int max_pos;     /* no sequence ends past this position after the call (0: unknown); a short call starts fewer blocks for
-                      * it, what is computed does not depend on it */
+                      * it, what is computed depends on it in the last bits only (how a row's sums are split) */
 } FnxSeqs;
 /* fnx_attn_prep_append for many rows: row t of sequence s, position p = pos0[s] + t - row0[s], is appended at p with the
  * bits that call gives its K and V rows; with `depth` (device [rows]) the row is rotated as position pos0[s] + depth[t]
@@ -476,16 +476,18 @@ int fnx_top_tokens(float* logits, int n, int T, int v0, const int* pen_tok, cons
                    const float* pen_par, float* out_v, int* out_i, unsigned* err, void* st);
 
 /* log probabilities over a slice of n logits a row (rows `stride` floats apart; tokens v0 .. v0 + n - 1), no counterpart in the
- * reference: lse[t] = log sum e^x, entropy[t] = -sum p log p, lp[t][j] = x[tok[t][j]] - lse, never above 0, for the ntok given tokens (a token
- * outside the slice: -inf), and the k <= FNX_TOPK_N likeliest tokens, best first, the lower id on a tie: top_lp, top_i
- * [T][k].  entropy, lp with tok, and top_* with k = 0 may be null.  Logits may have any finite size; -inf logits are tokens that cannot come; a NaN or +inf, or
- * a row of nothing but -inf, sets bit 16 of *err (the row's results are then NaN and top_i -1, or lse -inf and entropy 0).  n >= k.
+ * reference: lse[t] = log sum e^x, entropy[t] = -sum p log p, lp[t][j] = x[tok[t][j]] - lse, never above 0 (-inf where the type ends), for
+ * the ntok given tokens (a token outside the slice: -inf), and the k <= FNX_TOPK_N likeliest tokens, best first, the lower id on a tie: top_lp, top_i
+ * [T][k].  entropy, lp with tok, and top_* with k = 0 may be null.  Logits may have any finite size; -inf logits are tokens that cannot
+ * come; a NaN or +inf, or a row of nothing but -inf (a slice that a mask leaves nothing of is one), sets bit 16 of *err (the row's
+ * results are then NaN and top_i -1, or lse -inf and entropy 0).  n >= k.
  * scratch: fnx_logprobs_scratch_bytes bytes, zeroed once (left usable); calls that overlap need one each. */
 size_t fnx_logprobs_scratch_bytes(int n, int T, int k);
 int fnx_logprobs(const float* logits, size_t stride, int n, int T, int v0, const int* tok, int ntok, int k, float* lse, float* entropy, float* lp,
                  float* top_lp, int* top_i, void* scratch, unsigned* err, void* st);
-/* the slices' results ([nslice][T]..., host) as those of the whole vocabulary (host): fnx_top_merge's counterpart.  The slices' values
- * are log probabilities, so alternatives of two slices whose logits differ by less than their rounding may come in either order */
+/* the slices' results ([nslice][T]..., host) as those of the whole vocabulary (host): fnx_top_merge's counterpart.  A row of which a
+ * slice has NaNs is NaN, its top_i -1.  The slices' values are
+ * log probabilities, so alternatives of two slices whose logits differ by less than their rounding may come in either order */
 int fnx_logprobs_merge(const float* lse_s, const float* entropy_s, const float* lp_s, const float* top_lp_s, const int* top_i_s, int nslice, int T,
                        int ntok, int k, float* lse, float* entropy, float* lp, float* top_lp, int* top_i);
 

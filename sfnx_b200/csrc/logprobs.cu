@@ -15,7 +15,7 @@
 // A row goes to one block when there are many, else to as many as the GPU holds at once; the row's last block joins the parts.
 // A pass is bound by DRAM when there are many rows: a thread copies its own values into shared memory three batches ahead
 // (cp.async; nobody else reads them, so no barrier belongs to it), 72 KB in flight a multiprocessor.  2000 rows of 151 936 logits with
-// five alternatives: 214 us (5.7 TB/s); with one batch ahead in registers 342.  16 rows with twenty: 12.3 us, latency - a bound, the
+// five alternatives: 216 us (5.6 TB/s); with one batch ahead in registers 342.  16 rows with twenty: 12.2 us, latency - a bound, the
 // lists through memory to the row's last block, a bound and the choice there.
 #include <algorithm>
 
@@ -404,7 +404,7 @@ static int lp_splits(int n, int T, int k, int* each = nullptr) {
     return (batches + per - 1) / per;   // no empty block
 }
 // entries that a block of a row in several parts leaves for the last one: its lists as they are where they have room, which spares
-// choosing the best twice (16 rows, 20 alternatives: 13.8 us with k each, 12.3 so)
+// choosing the best twice (16 rows, 20 alternatives: 13.8 us with k each, 12.2 so)
 static int lp_ship(int ns, int k) { return k ? std::max(k, std::min(128, LP_CAP / ns)) : 0; }
 
 }  // namespace fnxk
