@@ -783,9 +783,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(SA_THREADS, 1) k_att
                 float* xm = xmax + (j & 1) * 2 * SA_ROWS;
                 xm[half * SA_ROWS + m] = mx;
                 agree();
-                mx = sa_max(mx, xm[(half ^ 1) * SA_ROWS + m]) * scale;
+                const float top = sa_max(mx, xm[(half ^ 1) * SA_ROWS + m]);
+                mx = top * scale;
                 if (!(mx < INFINITY)) z = NAN;   // a score that is no number, or infinite: so is the row
-                const bool up = real && (mx > ref + 8.0f || (ref == -INFINITY && mx != -INFINITY));   // (other rows hold what was there before)
+                const bool up = real && mx - ref > 8.0f;   // (other rows hold what was there before; nothing is -inf - -inf)
                 if (__any_sync(0xffffffffu, up)) {
                     const float f = !up ? 1.0f : ref == -INFINITY ? 0.f : ex2_ftz(ref - mx);
                     if (up) ref = mx;
@@ -803,7 +804,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(SA_THREADS, 1) k_att
                         }
                     }
                 }
-                const float less = ref == -INFINITY ? 0.f : (float) SA_LIFT - ref;
+                float less = ref == -INFINITY ? 0.f : (float) SA_LIFT - ref;
+                const bool far = fabsf(mx) > 4194304.f && fabsf(mx) < INFINITY;
+                if (__any_sync(0xffffffffu, far)) {   // mx is off by more than a weight can be: the scores against their own maximum first
+                    const float own = far ? top : 0.f;
+#pragma unroll
+                    for (int k = 0; k < 64; ++k) x[k] -= own;
+                    if (far) less = mx - ref + (float) SA_LIFT;
+                }
                 const bool p_free = j < 2 || sa_test(&o_full[j & 1], (unsigned) ((j >> 1) - 1) & 1u);   // the P tile's last reader is done
                 unsigned pk[32];
                 float2 sum = make_float2(0.f, 0.f);

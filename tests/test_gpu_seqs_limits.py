@@ -121,3 +121,31 @@ def test_outputs_as_far_apart_as_they_may_be():
     want = s.attend()
     assert torch.equal(out[:, :128].reshape(129, 128).view(torch.int16), want.view(torch.int16))
     assert (out[:, 128:1024] == -7).all() and (out[:, -64:] == -7).all()
+
+
+@pytest.mark.parametrize("big", [300.0, 3000.0, 10000.0, 30000.0, 65504.0])
+@pytest.mark.parametrize("lens,ctx", [([1, 40], [0, 300]), ([2], [9000])])
+def test_scores_of_any_finite_size(lens, ctx, big):
+    """Queries and keys whose elements are alike, so that a score is 128 times one product, exact in 32 bits, and up to 128^(1/2) 65504^2:
+    some keys share the largest, the others are a sixteenth of it lower or negative, and weigh nothing.  The result is the mean of the
+    values that share it, rounded as in the tests' formula (their weights are alike)."""
+    s = S.Seqs(lens, ctx, 8, 2, 128, seed=43, stale=0.0)
+    g = torch.Generator(device=DEV).manual_seed(43)
+    s.q[:] = big
+    pick = torch.rand(s.k.shape[:2], device=DEV, generator=g)
+    s.k[:] = torch.where(pick < 0.3, big, torch.where(pick < 0.7, big * 15 / 16, -big)).half()[:, :, None]
+    for sign in (1.0, -1.0):   # with the other sign the keys at -big are the largest
+        s.q[:] = sign * big
+        s.kc = s._pool(s.k)
+        out = s.attend(gate=False).view(-1, 8, 128)
+        for i, n in enumerate(lens):
+            c = s.cells[i].to(DEV)
+            x = (sign * s.k[c][:, :, 0].double()).repeat_interleave(4, 1)   # (the score over a positive factor) [positions][heads]
+            v = s.v[c].double().repeat_interleave(4, 1)
+            for t in range(n):
+                seen = x[:ctx[i] + t + 1]
+                w = (seen == seen.amax(0)).double()
+                w = w / w.sum(0)
+                ref, mag = torch.einsum("ph,phd->hd", w, v[:len(seen)]), torch.einsum("ph,phd->hd", w, v[:len(seen)].abs())
+                got = out[s.row0[i] + t].double()
+                assert ((got - ref).abs() <= (2.0 ** -11 * ref.abs() + (2.0 ** -11 + 2.0 ** -18) * mag + 2.0 ** -25) * (1 + 2.0 ** -10)).all(), (i, t, sign)
